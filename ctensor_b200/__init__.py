@@ -31,6 +31,8 @@ ADD, SUB, MUL, DIV, LT, LE, GT, GE, EQ, NE, POW = range(11)
 # reductions
 SUM, MEAN, MAX, MIN, VAR, ARGMAX = range(6)
 DIM_FULL = -1
+# norms of residual_norm
+NORM_NONE, NORM_LAYER, NORM_RMS = range(3)
 
 STATUS_NAMES = {0: "CTB_OK", 1: "CTB_ERR_NULL", 2: "CTB_ERR_SHAPE", 3: "CTB_ERR_DTYPE",
                 4: "CTB_ERR_DIM", 5: "CTB_ERR_ARG", 6: "CTB_ERR_CUDA", 7: "CTB_ERR_WORKSPACE",
@@ -51,6 +53,9 @@ EXPORTED_SYMBOLS = [
     "ctb_div_backward", "ctb_tanh_backward", "ctb_cross_entropy", "ctb_cross_entropy_backward",
     "ctb_shard_range", "ctb_comm_init_all", "ctb_comm_size", "ctb_comm_device", "ctb_comm_stream", "ctb_comm_sync",
     "ctb_comm_destroy", "ctb_allreduce", "ctb_full_reduce_sharded", "ctb_matmul_tc",
+    "ctb_score_softmax", "ctb_score_softmax_workspace_bytes", "ctb_score_softmax_backward",
+    "ctb_residual_norm", "ctb_residual_norm_workspace_bytes", "ctb_residual_norm_backward",
+    "ctb_grad_norm_workspace_bytes", "ctb_grad_norm", "ctb_clip_grad_norm",
 ]
 
 
@@ -70,6 +75,24 @@ class OptimizerHyper(ctypes.Structure):
 
 
 (OPT_SGD, OPT_ADAM, OPT_ADAMW, OPT_ADAMAX, OPT_NADAM, OPT_RADAM, OPT_RMSPROP, OPT_ADAGRAD, OPT_LION) = range(9)
+
+
+class CScoreRules(ctypes.Structure):
+    """struct ctb_score_rules."""
+    _fields_ = [("scale", ctypes.c_double), ("cap", ctypes.c_double), ("causal", ctypes.c_int32), ("reserved", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("query_start", "key_lengths", "prefix", "query_docs", "key_docs", "slopes")]
+
+
+class CResidualNormParams(ctypes.Structure):
+    """struct ctb_residual_norm_params."""
+    _fields_ = [("post_kind", ctypes.c_int32), ("pre_kind", ctypes.c_int32), ("post_eps", ctypes.c_double),
+                ("pre_eps", ctypes.c_double), ("scale", ctypes.c_double)] + [
+        (n, ctypes.c_void_p) for n in ("post_weight", "post_bias", "pre_weight", "pre_bias")]
+
+
+class CResidualNormGrads(ctypes.Structure):
+    """struct ctb_residual_norm_grads."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "f", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias")]
 
 
 class PoolInfo(ctypes.Structure):
@@ -162,6 +185,19 @@ def lib() -> ctypes.CDLL:
     L.ctb_batchnorm_apply.argtypes = [vp, vp, vp, vp, vp, ctypes.c_double, vp, vd]
     L.ctb_cat.argtypes = [ctypes.POINTER(vp), i32, i32, vp, vd]
     L.ctb_adam_step.argtypes = [vp, vp, vd, vd] + [ctypes.c_double] * 4 + [i32, ctypes.c_double, i32, vd]
+    sz, rules_p, params_p = ctypes.c_size_t, ctypes.POINTER(CScoreRules), ctypes.POINTER(CResidualNormParams)
+    L.ctb_score_softmax.argtypes = [vp, rules_p, vp, vd]
+    L.ctb_score_softmax_workspace_bytes.argtypes = [vp]
+    L.ctb_score_softmax_workspace_bytes.restype = sz
+    L.ctb_score_softmax_backward.argtypes = [vp, vp, vp, rules_p, vp, vp, vd, sz, vd]
+    L.ctb_residual_norm.argtypes = [vp, vp, vp, params_p, vp, vp, vp, vd]
+    L.ctb_residual_norm_workspace_bytes.argtypes = [vp, vp]
+    L.ctb_residual_norm_workspace_bytes.restype = sz
+    L.ctb_residual_norm_backward.argtypes = [vp, vp, vp, vp, params_p, vp, vp, ctypes.POINTER(CResidualNormGrads), vd, sz, vd]
+    L.ctb_grad_norm_workspace_bytes.argtypes = [i32]
+    L.ctb_grad_norm_workspace_bytes.restype = sz
+    L.ctb_grad_norm.argtypes = [ctypes.POINTER(vp), i32, ctypes.c_double, vp, vd, sz, vd]
+    L.ctb_clip_grad_norm.argtypes = [ctypes.POINTER(vp), i32, ctypes.c_double, ctypes.c_double, ctypes.POINTER(vp), vp, vd, sz, vd]
     L.ctb_binary_host.argtypes = [i32, vp, vp, vp, i32]
     L.ctb_unary_host.argtypes = [i32, vp, ctypes.c_double, vp, i32]
     L.ctb_reduce_host.argtypes = [i32, vp, i32, vp, i32]
@@ -603,6 +639,200 @@ def layernorm(x, gamma=None, beta=None, eps: float = 1e-5, out=None):
                                           None if b is None else b.cview(), float(eps),
                                           _as_dview(out).cview(), _stream_ptr(x)))
     return out
+
+
+# ---- a transformer block's steps between its matrix products ------------------------------------------------
+def _opt_view(x):
+    return None if x is None else _as_dview(x).cview()
+
+
+def _address(cview):
+    """A pointer member of a C struct; the struct's owner keeps the view alive."""
+    return None if cview is None else ctypes.addressof(cview)
+
+
+def _same_device(first: DView, others, what: str) -> None:
+    for o in others:
+        if o is not None and _as_dview(o).buf.device != first.buf.device:
+            raise CtbError(5, f"{what}: tensors on different devices")
+
+
+def _workspace(nbytes: int, like: DView):
+    """Scratch of one call, from torch's allocator: ordered on the current stream, and a captured graph's
+    own when the call is captured."""
+    return _torch().empty(nbytes, dtype=_torch().uint8, device=like.buf.device) if nbytes else None
+
+
+class ScoreRules:
+    """What ``score_softmax`` does to attention scores: scale, tanh ``cap`` (0: none), ``causal``, and per
+    sequence ``query_start`` (position of its first query; default: keys - queries), ``key_lengths``,
+    ``prefix`` (keys every query may look at) — int32 [batch] —, ``query_docs`` / ``key_docs`` (document
+    numbers, int32 [batch, queries] / [batch, keys]) and ``slopes`` (float32 [heads], bias
+    -slope * |distance|).  Holds its tensors; their contents may change between calls."""
+    _TABLES = ("query_start", "key_lengths", "prefix", "query_docs", "key_docs", "slopes")
+
+    def __init__(self, scale: float = 1.0, cap: float = 0.0, causal: bool = False, query_start=None, key_lengths=None,
+                 prefix=None, query_docs=None, key_docs=None, slopes=None):
+        given = (query_start, key_lengths, prefix, query_docs, key_docs, slopes)
+        self.tables = {n: None if t is None else _as_dview(t) for n, t in zip(self._TABLES, given)}
+        self._views = {n: _opt_view(t) for n, t in self.tables.items()}
+        self.c = CScoreRules(float(scale), float(cap), int(bool(causal)), 0, *(_address(self._views[n]) for n in self._TABLES))
+
+
+def score_softmax(scores, rules: ScoreRules, out=None):
+    """Attention probabilities of ``scores`` [batch, heads, queries, keys] over the keys that ``rules``
+    admit; zeros elsewhere and in the rows of queries that are admitted to nothing."""
+    s = _as_dview(scores)
+    _same_device(s, [out, *rules.tables.values()], "score_softmax")
+    if out is None:
+        out = _new_out(s, s.shape)
+    with _device_guard(s):
+        check(lib().ctb_score_softmax(s.cview(), ctypes.byref(rules.c), _as_dview(out).cview(), _stream_ptr(s)))
+    return out
+
+
+def score_softmax_backward(grad, probs, rules: ScoreRules, scores=None, want_slopes: bool = False, out=None):
+    """(gradient of the scores, gradient of ``rules``' slopes or None) from the gradient of the
+    probabilities; ``scores`` (the forward's input) is needed when the rules have a cap."""
+    g, p = _as_dview(grad), _as_dview(probs)
+    _same_device(p, [grad, scores, out, *rules.tables.values()], "score_softmax_backward")
+    if out is None:
+        out = _new_out(p, p.shape)
+    slopes = ws = None
+    if want_slopes and len(p.shape) == 4:
+        slopes = _new_out(p, (p.shape[1],))
+        ws = _workspace(int(lib().ctb_score_softmax_workspace_bytes(p.cview())), p)
+    with _device_guard(p):
+        check(lib().ctb_score_softmax_backward(g.cview(), p.cview(), _opt_view(scores), ctypes.byref(rules.c), _as_dview(out).cview(),
+                                               _opt_view(slopes), None if ws is None else ws.data_ptr(),
+                                               0 if ws is None else ws.numel(), _stream_ptr(p)))
+    return out, slopes
+
+
+class ResidualNorm:
+    """The weights and kinds of ``residual_norm``: y = x + scale * gate * N_post(f), h = N_pre(y), each norm
+    NORM_NONE, NORM_LAYER or NORM_RMS with an optional float32 weight and bias of the row length.  Holds
+    its tensors; their contents may change between calls."""
+    _VECTORS = ("post_weight", "post_bias", "pre_weight", "pre_bias")
+
+    def __init__(self, pre: int = NORM_LAYER, pre_weight=None, pre_bias=None, pre_eps: float = 1e-5, post: int = NORM_NONE,
+                 post_weight=None, post_bias=None, post_eps: float = 1e-5, scale: float = 1.0):
+        self.pre, self.post = pre, post
+        self.vectors = {n: None if t is None else _as_dview(t)
+                        for n, t in zip(self._VECTORS, (post_weight, post_bias, pre_weight, pre_bias))}
+        self._views = {n: _opt_view(t) for n, t in self.vectors.items()}
+        self.c = CResidualNormParams(int(post), int(pre), float(post_eps), float(pre_eps), float(scale),
+                                     *(_address(self._views[n]) for n in self._VECTORS))
+
+
+def residual_norm(x, f, params: ResidualNorm, gate=None):
+    """(y, h, stats): the residual stream after a block's output ``f`` is added, its norm for the next block,
+    and the rows' statistics [..., 4] for the backward pass.  ``f`` None: y is ``x`` itself; h is None when
+    ``params`` has no pre norm."""
+    xv = _as_dview(x)
+    _same_device(xv, [f, gate, *params.vectors.values()], "residual_norm")
+    y = x if f is None else _new_out(xv, xv.shape)
+    h = None if params.pre == NORM_NONE else _new_out(xv, xv.shape)
+    stats = _new_out(xv, tuple(xv.shape[:-1]) + (4,))
+    with _device_guard(xv):
+        check(lib().ctb_residual_norm(xv.cview(), _opt_view(f), _opt_view(gate), ctypes.byref(params.c),
+                                      None if f is None else _opt_view(y), _opt_view(h), _opt_view(stats), _stream_ptr(xv)))
+    return y, h, stats
+
+
+@dataclass
+class ResidualNormGrads:
+    """Gradients of ``residual_norm``'s inputs; None where there was no such input."""
+    x: "object" = None
+    f: "object" = None
+    gate: "object" = None
+    post_weight: "object" = None
+    post_bias: "object" = None
+    pre_weight: "object" = None
+    pre_bias: "object" = None
+
+
+def residual_norm_backward(f, y, stats, params: ResidualNorm, grad_y=None, grad_h=None, gate=None) -> ResidualNormGrads:
+    """The gradients of x, f, the gate, the weights and the biases, from the forward's f, y and stats and
+    the gradients of y and h (``grad_y`` None: zero; ``grad_h`` goes with a pre norm)."""
+    yv = _as_dview(y)
+    _same_device(yv, [f, stats, grad_y, grad_h, gate, *params.vectors.values()], "residual_norm_backward")
+    out = ResidualNormGrads(x=_new_out(yv, yv.shape))
+    if f is not None:
+        out.f = _new_out(yv, yv.shape)
+    if gate is not None:
+        out.gate = _new_out(yv, _as_dview(gate).shape)
+    for name, vector in params.vectors.items():
+        if vector is not None:
+            setattr(out, name, _new_out(yv, vector.shape))
+    views = [_opt_view(getattr(out, n)) for n, _ in CResidualNormGrads._fields_]
+    c = CResidualNormGrads(*(_address(v) for v in views))
+    gate_view = _opt_view(gate)
+    ws = _workspace(int(lib().ctb_residual_norm_workspace_bytes(yv.cview(), gate_view)), yv)
+    with _device_guard(yv):
+        check(lib().ctb_residual_norm_backward(_opt_view(f), yv.cview(), gate_view, _opt_view(stats), ctypes.byref(params.c),
+                                               _opt_view(grad_y), _opt_view(grad_h), ctypes.byref(c),
+                                               None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+                                               _stream_ptr(yv)))
+    return out
+
+
+class TensorList:
+    """A list of CUDA tensors (a model's gradients) with the C descriptors built once.  It holds the tensors;
+    a tensor that is given other memory afterwards needs a new list."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        views = [_as_dview(t) for t in self.tensors]
+        for v in views:
+            if v.buf.device != views[0].buf.device:
+                raise CtbError(5, "TensorList: tensors on different devices")
+        self.device_view = views[0] if views else None
+        self.has_f64 = any(v.dtype == F64 for v in views)
+        self._views = [v.cview() for v in views]
+        self.c = (ctypes.POINTER(View) * max(1, len(views)))(*[ctypes.pointer(c) for c in self._views])
+
+    def __len__(self):
+        return len(self.tensors)
+
+
+def _grad_norm(grads, max_norm, p, out, norm):
+    torch = _torch()
+    grads = grads if isinstance(grads, TensorList) else TensorList(grads)
+    if out is not None:
+        out = out if isinstance(out, TensorList) else TensorList(out)
+        if len(out) != len(grads):
+            raise CtbError(2, "clip_grad_norm: as many outputs as gradients are needed")
+    like = grads.device_view
+    if like is None:
+        if norm is None:
+            raise CtbError(5, "grad_norm: an empty list needs `norm`, which says where the result goes")
+        like = _as_dview(norm)
+    if norm is None:
+        norm = torch.empty(1, dtype=torch.float64 if grads.has_f64 else torch.float32, device=like.buf.device)
+    _same_device(like, [norm] + ([] if out is None or out.device_view is None else [out.device_view]), "grad_norm")
+    ws = _workspace(int(lib().ctb_grad_norm_workspace_bytes(len(grads))), like)
+    ws_args = (None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+    with _device_guard(like):
+        if max_norm is None:
+            check(lib().ctb_grad_norm(grads.c, len(grads), float(p), _as_dview(norm).cview(), *ws_args, _stream_ptr(like)))
+        else:
+            check(lib().ctb_clip_grad_norm(grads.c, len(grads), float(max_norm), float(p), None if out is None else out.c,
+                                           _as_dview(norm).cview(), *ws_args, _stream_ptr(like)))
+    return norm
+
+
+def grad_norm(grads, p: float = 2.0, norm=None):
+    """(sum |g|^p)^(1/p) over all tensors of ``grads`` (a list or a TensorList), p = 1, 2 or inf, as a
+    one-element CUDA tensor (float64 if any gradient is, else float32)."""
+    return _grad_norm(grads, None, p, None, norm)
+
+
+def clip_grad_norm(grads, max_norm: float, p: float = 2.0, out=None, norm=None):
+    """Scales all of ``grads`` by max_norm / norm when max_norm < norm < inf — in place, or into the tensors
+    of ``out``, which get the values as they are otherwise — and returns the norm (a CUDA tensor: no
+    synchronisation)."""
+    return _grad_norm(grads, max_norm, p, out, norm)
 
 
 # ---- operators (host memory in, host memory out) --------------------------------------------------------

@@ -3,6 +3,8 @@
 // host-buffer entry points.  Error texts equal the reference's exception messages
 // (src/core/opsmp.cpp:138,144,274,595; src/core/ops_dispatch.cpp:428,433) so a C++ shim can
 // re-throw them unchanged.
+#include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -14,6 +16,9 @@
 #include "ctb_math.cuh"
 #include "ctb_reduce.cuh"
 #include "ctb_backward.cuh"
+#include "ctb_clip.cuh"
+#include "ctb_residual_norm.cuh"
+#include "ctb_scores.cuh"
 
 namespace ctb {
 
@@ -1318,6 +1323,433 @@ int ctb_optimizer_step(int kind, const ctb_view* param, const ctb_view* grad, fl
     if (step < 1) return set_error(CTB_ERR_ARG, "optimizer_step: the step count starts at 1");
     return launch_optimizer(kind, (float*)elem_ptr_mut(param), (const float*)elem_ptr(grad), state1, state2,
                             view_numel(param), *hyper, step, (cudaStream_t)stream);
+}
+
+// ---- a transformer block's steps between its matrix products -------------------------------------------
+namespace {
+
+// The caller's scratch, or the part of the per-device workspace behind the ticket region (which has to
+// stay zero for the reductions that use it).
+int scratch_for(void* given, size_t given_bytes, size_t need, const char* who, void** out, cudaStream_t st) {
+    *out = nullptr;
+    if (need == 0) return CTB_OK;
+    if (given) {
+        if (given_bytes < need) return set_error(CTB_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, given_bytes);
+        if (!is_aligned(given, 256)) return set_error(CTB_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+        *out = given;
+        return CTB_OK;
+    }
+    void* ws = nullptr;
+    int rc = ensure_workspace(kTicketBytes + need, &ws, st);
+    if (rc) return rc;
+    *out = (char*)ws + kTicketBytes;
+    return CTB_OK;
+}
+
+// No output overlaps an input or another output (entries may be NULL).
+int check_outputs_apart(const ctb_view* const* outs, int nout, const ctb_view* const* ins, int nin, const char* who) {
+    int rc;
+    for (int i = 0; i < nout; ++i) {
+        if (!outs[i]) continue;
+        if ((rc = check_no_alias(outs[i], ins, nin, who))) return rc;
+        if (check_no_alias(outs[i], outs, i, who)) return set_error(CTB_ERR_ARG, "%s: two outputs overlap", who);
+    }
+    return CTB_OK;
+}
+
+// A kernel reads and writes elements at their natural alignment.
+int check_element_alignment(const ctb_view* v, const char* who) {
+    if (v && v->base && !is_aligned(elem_ptr(v), dtype_bytes(v->dtype))) return set_error(CTB_ERR_ARG, "%s: misaligned data", who);
+    return CTB_OK;
+}
+
+bool same_shape(const ctb_view* a, const ctb_view* b) {
+    if (a->ndim != b->ndim) return false;
+    for (int d = 0; d < a->ndim; ++d)
+        if (a->shape[d] != b->shape[d]) return false;
+    return true;
+}
+
+// ---- scores
+int score_operand(const ctb_view* v, const char* null_msg, const char* who, const ctb_view* like, ScoreRows* out) {
+    int rc;
+    if ((rc = check_view(v, null_msg, who))) return rc;
+    if (v->dtype != CTB_F32) return set_error(CTB_ERR_DTYPE, "%s: only Float32 is supported", who);
+    if (v->ndim != 4) return set_error(CTB_ERR_SHAPE, "%s: scores must be 4D [batch, heads, queries, keys]", who);
+    if (like && !same_shape(v, like)) return set_error(CTB_ERR_SHAPE, "%s: shapes differ", who);
+    if (v->shape[3] > 1 && v->stride[3] != 1) return set_error(CTB_ERR_SHAPE, "%s: the keys must be contiguous", who);
+    if ((rc = check_element_alignment(v, who))) return rc;
+    *out = {(const float*)elem_ptr(v), v->stride[0], v->stride[1], v->stride[2]};
+    return CTB_OK;
+}
+
+int score_table(const ctb_view* v, const char* name, const char* who, int ndim, int64_t n0, int64_t n1, int dtype) {
+    if (!v) return CTB_OK;
+    int rc;
+    if ((rc = check_view(v, "score_softmax: null rule table", who))) return rc;
+    if (v->dtype != dtype) return set_error(CTB_ERR_DTYPE, "%s: %s must be %s", who, name, dtype == CTB_I32 ? "Int32" : "Float32");
+    if (v->ndim != ndim || v->shape[0] != n0 || (ndim == 2 && v->shape[1] != n1)) return set_error(CTB_ERR_SHAPE, "%s: %s has the wrong shape", who, name);
+    return check_element_alignment(v, who);
+}
+
+int score_geometry(const ctb_view* scores, const ctb_score_rules* r, const char* who, ScoreGeom* g) {
+    memset(g, 0, sizeof *g);
+    if (!r) return set_error(CTB_ERR_NULL, "%s: null rules", who);
+    g->batch = scores->shape[0];
+    g->heads = scores->shape[1];
+    g->queries = scores->shape[2];
+    g->keys = scores->shape[3];
+    if (!std::isfinite(r->scale)) return set_error(CTB_ERR_ARG, "%s: scale must be finite", who);
+    if (!(r->cap >= 0.0) || !std::isfinite(r->cap)) return set_error(CTB_ERR_ARG, "%s: cap must be finite and not negative", who);
+    g->scale = (float)r->scale;
+    g->cap = (float)r->cap;
+    g->over_cap = r->cap > 0.0 ? (float)(r->scale / r->cap) : 0.0f;
+    if (!std::isfinite(g->scale) || !std::isfinite(g->cap) || !std::isfinite(g->over_cap) || (r->cap > 0.0 && g->cap == 0.0f))
+        return set_error(CTB_ERR_ARG, "%s: scale or cap beyond Float32", who);
+    g->causal = r->causal != 0;
+    int rc;
+    if ((rc = score_table(r->query_start, "query_start", who, 1, g->batch, 0, CTB_I32))) return rc;
+    if ((rc = score_table(r->key_lengths, "key_lengths", who, 1, g->batch, 0, CTB_I32))) return rc;
+    if ((rc = score_table(r->prefix, "prefix", who, 1, g->batch, 0, CTB_I32))) return rc;
+    if ((rc = score_table(r->query_docs, "query_docs", who, 2, g->batch, g->queries, CTB_I32))) return rc;
+    if ((rc = score_table(r->key_docs, "key_docs", who, 2, g->batch, g->keys, CTB_I32))) return rc;
+    if ((rc = score_table(r->slopes, "slopes", who, 1, g->heads, 0, CTB_F32))) return rc;
+    if (!r->query_docs != !r->key_docs) return set_error(CTB_ERR_ARG, "%s: query_docs and key_docs come together", who);
+    auto table = [](const ctb_view* v) {
+        ScoreTable t{nullptr, 0, 0};
+        if (v) t = {(const int32_t*)elem_ptr(v), v->stride[0], v->ndim == 2 ? v->stride[1] : 0};
+        return t;
+    };
+    g->query_start = table(r->query_start);
+    g->key_lengths = table(r->key_lengths);
+    g->prefix = table(r->prefix);
+    g->query_docs = table(r->query_docs);
+    g->key_docs = table(r->key_docs);
+    if (r->slopes) {
+        g->slopes = (const float*)elem_ptr(r->slopes);
+        g->slope_stride = r->slopes->stride[0];
+    }
+    return CTB_OK;
+}
+
+// ---- residual norm
+// The rows of a view: one distance between neighbouring rows, columns contiguous.
+int norm_rows(const ctb_view* v, const char* null_msg, const char* who, const ctb_view* like, RowsIn* out) {
+    int rc;
+    if ((rc = check_view(v, null_msg, who))) return rc;
+    if (v->dtype != CTB_F32) return set_error(CTB_ERR_DTYPE, "%s: only Float32 is supported", who);
+    if (v->ndim < 1) return set_error(CTB_ERR_SHAPE, "%s: needs at least one dim", who);
+    if (like && !same_shape(v, like)) return set_error(CTB_ERR_SHAPE, "%s: shapes differ", who);
+    const int last = v->ndim - 1;
+    if (v->shape[last] > 1 && v->stride[last] != 1) return set_error(CTB_ERR_SHAPE, "%s: the last dim must be contiguous", who);
+    if ((rc = check_element_alignment(v, who))) return rc;
+    int64_t stride = 0, expect = 0;
+    bool first = true;
+    for (int d = last - 1; d >= 0; --d) {
+        if (v->shape[d] <= 1) continue;
+        if (first) stride = v->stride[d];
+        else if (v->stride[d] != expect) return set_error(CTB_ERR_SHAPE, "%s: the rows must lie at one fixed distance", who);
+        first = false;
+        expect = v->stride[d] * v->shape[d];
+    }
+    *out = {(const float*)elem_ptr(v), stride};
+    return CTB_OK;
+}
+
+int norm_vector(const ctb_view* v, int64_t cols, const char* who, const float** out) {
+    *out = nullptr;
+    if (!v) return CTB_OK;
+    int rc;
+    if ((rc = check_view(v, "residual_norm: null weight or bias", who))) return rc;
+    if (v->dtype != CTB_F32) return set_error(CTB_ERR_DTYPE, "%s: weights and biases must be Float32", who);
+    if (v->ndim != 1 || v->shape[0] != cols || (cols > 1 && v->stride[0] != 1)) return set_error(CTB_ERR_SHAPE, "%s: weights and biases must be contiguous and hold one value per column", who);
+    if ((rc = check_element_alignment(v, who))) return rc;
+    *out = (const float*)elem_ptr(v);
+    return CTB_OK;
+}
+
+int norm_gate(const ctb_view* gate, const ctb_view* x, const char* who, ResidualNormGeom* g) {
+    g->gate_mode = kGateNone;
+    g->gate_rows = 1;
+    if (!gate) return CTB_OK;
+    int rc;
+    if ((rc = check_view(gate, "residual_norm: null gate", who))) return rc;
+    if (gate->dtype != CTB_F32) return set_error(CTB_ERR_DTYPE, "%s: the gate must be Float32", who);
+    if (gate->ndim < 1 || gate->ndim > x->ndim) return set_error(CTB_ERR_SHAPE, "Shape mismatch in binary op");
+    if ((rc = check_element_alignment(gate, who))) return rc;
+    const int last = x->ndim - 1, pad = x->ndim - gate->ndim;
+    const int64_t width = gate->shape[gate->ndim - 1];
+    if (width != g->cols && width != 1) return set_error(CTB_ERR_SHAPE, "Shape mismatch in binary op");
+    g->gate_mode = width == g->cols ? kGateRow : kGateScalar;
+    if (g->gate_mode == kGateRow && width > 1 && gate->stride[gate->ndim - 1] != 1) return set_error(CTB_ERR_SHAPE, "%s: the gate's last dim must be contiguous or of extent 1", who);
+    int64_t shared = 1, stride = 0, expect = 0;
+    bool full_seen = false;
+    for (int d = last - 1; d >= 0; --d) {
+        const int64_t have = d - pad < 0 ? 1 : gate->shape[d - pad], want = x->shape[d];
+        if (have != want && have != 1) return set_error(CTB_ERR_SHAPE, "Shape mismatch in binary op");
+        if (want == 1) continue;
+        if (have == 1) {
+            if (full_seen) return set_error(CTB_ERR_SHAPE, "%s: the gate's dims of extent 1 must come after its full ones", who);
+            shared *= want;
+            continue;
+        }
+        if (!full_seen) stride = gate->stride[d - pad];
+        else if (gate->stride[d - pad] != expect) return set_error(CTB_ERR_SHAPE, "%s: the gate's rows must lie at one fixed distance", who);
+        full_seen = true;
+        expect = gate->stride[d - pad] * want;
+    }
+    g->gate_rows = shared > 0 ? shared : 1;
+    g->gate = {(const float*)elem_ptr(gate), stride};
+    return CTB_OK;
+}
+
+int norm_geometry(const ctb_view* x, const ctb_view* gate, const ctb_residual_norm_params* p, const char* who, ResidualNormGeom* g) {
+    memset(g, 0, sizeof *g);
+    if (!p) return set_error(CTB_ERR_NULL, "%s: null parameters", who);
+    g->cols = x->shape[x->ndim - 1];
+    if (g->cols > CTB_RESIDUAL_NORM_MAX_COLS) return set_error(CTB_ERR_LIMIT, "%s: rows of more than %d columns", who, CTB_RESIDUAL_NORM_MAX_COLS);
+    g->rows = 1;
+    for (int d = 0; d + 1 < x->ndim; ++d) g->rows *= x->shape[d];
+    for (int kind : {p->post_kind, p->pre_kind})
+        if (kind != CTB_NORM_NONE && kind != CTB_NORM_LAYER && kind != CTB_NORM_RMS) return set_error(CTB_ERR_ARG, "%s: unknown norm %d", who, kind);
+    if (!(p->post_eps >= 0.0) || !(p->pre_eps >= 0.0) || !std::isfinite(p->post_eps) || !std::isfinite(p->pre_eps)) return set_error(CTB_ERR_ARG, "%s: eps must be finite and not negative", who);
+    if (!std::isfinite(p->scale) || !std::isfinite((float)p->scale)) return set_error(CTB_ERR_ARG, "%s: scale must be finite", who);
+    g->post_kind = p->post_kind;
+    g->pre_kind = p->pre_kind;
+    g->post_eps = (float)p->post_eps;
+    g->pre_eps = (float)p->pre_eps;
+    g->scale = (float)p->scale;
+    int rc;
+    if ((rc = norm_vector(p->post_weight, g->cols, who, &g->post_weight))) return rc;
+    if ((rc = norm_vector(p->post_bias, g->cols, who, &g->post_bias))) return rc;
+    if ((rc = norm_vector(p->pre_weight, g->cols, who, &g->pre_weight))) return rc;
+    if ((rc = norm_vector(p->pre_bias, g->cols, who, &g->pre_bias))) return rc;
+    if (g->post_kind == CTB_NORM_NONE && (p->post_weight || p->post_bias)) return set_error(CTB_ERR_ARG, "%s: a weight or bias without its norm", who);
+    if (g->pre_kind == CTB_NORM_NONE && (p->pre_weight || p->pre_bias)) return set_error(CTB_ERR_ARG, "%s: a weight or bias without its norm", who);
+    return norm_gate(gate, x, who, g);
+}
+
+int norm_stats(const ctb_view* stats, const ResidualNormGeom& g, const char* who) {
+    int rc = check_out(stats, g.rows * 4, CTB_F32, who);
+    if (rc) return rc;
+    if (g.rows > 0 && !is_aligned(elem_ptr(stats), 16)) return set_error(CTB_ERR_ARG, "%s: stats must be 16-byte aligned", who);
+    return CTB_OK;
+}
+
+size_t norm_workspace(const ResidualNormGeom& g) {
+    if (g.rows == 0 || g.cols == 0) return 0;
+    const bool folded = g.gate_mode == kGateScalar || (g.gate_mode == kGateRow && g.gate_rows > 1);
+    return residual_norm_workspace_bytes(g.rows, g.cols, folded ? g.rows / g.gate_rows : 0, g.gate_mode == kGateRow ? g.cols : 1);
+}
+
+// ---- gradient clipping
+int clip_entry(const ctb_view* const* grads, int count, int scale, double max_norm, double p, const ctb_view* const* outs,
+               const ctb_view* norm, void* workspace, size_t workspace_bytes, void* stream, const char* who) {
+    int rc;
+    if (count < 0) return set_error(CTB_ERR_ARG, "%s: negative count", who);
+    if (count > 0 && !grads) return set_error(CTB_ERR_NULL, "%s: null gradient list", who);
+    int kind;
+    if (p == 2.0) kind = kNormP2;
+    else if (p == 1.0) kind = kNormP1;
+    else if (std::isinf(p) && p > 0) kind = kNormInf;
+    else return set_error(CTB_ERR_ARG, "%s: p must be 1, 2 or infinity", who);
+    if (scale && !(max_norm >= 0.0)) return set_error(CTB_ERR_ARG, "%s: max_norm must not be negative or NaN", who);
+    if ((rc = check_view(norm, "output: null view", who))) return rc;
+    if (norm->dtype != CTB_F32 && norm->dtype != CTB_F64) return set_error(CTB_ERR_DTYPE, "%s: the norm must be Float32 or Double64", who);
+    if (view_numel(norm) != 1) return set_error(CTB_ERR_SHAPE, "%s: the norm must hold one element", who);
+    if ((rc = check_element_alignment(norm, who))) return rc;
+    struct Range { const char *lo, *hi; bool written; };
+    try {
+        std::vector<ClipTensor> lists[2];
+        std::vector<Range> ranges;
+        ranges.reserve((size_t)count * (outs ? 2 : 1) + 1);
+        auto add_range = [&](const ctb_view* v, bool written) {
+            Range r;
+            view_bytes(v, &r.lo, &r.hi);
+            r.written = written;
+            if (r.lo != r.hi) ranges.push_back(r);
+        };
+        add_range(norm, true);
+        for (int i = 0; i < count; ++i) {
+            const ctb_view* g = grads[i];
+            if ((rc = check_view(g, "clip_grad_norm: null gradient", who))) return rc;
+            if (g->dtype != CTB_F32 && g->dtype != CTB_F64) return set_error(CTB_ERR_DTYPE, "%s: gradients must be Float32 or Double64", who);
+            const int64_t n = view_numel(g);
+            if (n > 0 && !view_dense(g)) return set_error(CTB_ERR_SHAPE, "%s: gradients must be dense", who);
+            if ((rc = check_element_alignment(g, who))) return rc;
+            add_range(g, scale && !outs);
+            ClipTensor t{elem_ptr(g), const_cast<void*>(elem_ptr(g)), n};
+            if (outs) {
+                const ctb_view* o = outs[i];
+                if ((rc = check_view(o, "output: null view", who))) return rc;
+                if (o->dtype != g->dtype) return set_error(CTB_ERR_DTYPE, "%s: output dtype mismatch", who);
+                bool same = same_shape(o, g);
+                for (int d = 0; same && d < g->ndim; ++d)
+                    if (g->shape[d] > 1 && o->stride[d] != g->stride[d]) same = false;
+                if (!same) return set_error(CTB_ERR_SHAPE, "%s: an output must have its gradient's shape and strides", who);
+                if ((rc = check_element_alignment(o, who))) return rc;
+                add_range(o, true);
+                t.dst = elem_ptr_mut(o);
+            }
+            if (n > 0) lists[g->dtype == CTB_F64].push_back(t);
+        }
+        std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+        const char *read_to = nullptr, *written_to = nullptr;
+        for (const Range& r : ranges) {
+            if (r.lo < written_to || (r.written && r.lo < read_to)) return set_error(CTB_ERR_ARG, "%s: a tensor that is written overlaps another", who);
+            if (r.written) written_to = r.hi > written_to ? r.hi : written_to;
+            else read_to = r.hi > read_to ? r.hi : read_to;
+        }
+        void* ws = nullptr;
+        const int64_t n32 = (int64_t)lists[0].size(), n64 = (int64_t)lists[1].size();
+        if ((rc = scratch_for(workspace, workspace_bytes, clip_workspace_bytes(n32, n64), who, &ws, (cudaStream_t)stream))) return rc;
+        return launch_clip(kind, lists[0].data(), n32, lists[1].data(), n64, scale, max_norm, elem_ptr_mut(norm), norm->dtype, ws, (cudaStream_t)stream);
+    } catch (...) {
+        return set_error(CTB_ERR_LIMIT, "%s: out of host memory", who);
+    }
+}
+
+}  // namespace
+
+int ctb_score_softmax(const ctb_view* scores, const ctb_score_rules* rules, const ctb_view* out, void* stream) {
+    const char* who = "score_softmax";
+    int rc;
+    ScoreRows s;
+    ScoreGeom g;
+    if ((rc = score_operand(scores, "score_softmax: null input", who, nullptr, &s))) return rc;
+    if ((rc = score_geometry(scores, rules, who, &g))) return rc;
+    if ((rc = check_out(out, view_numel(scores), CTB_F32, who))) return rc;
+    if ((rc = check_element_alignment(out, who))) return rc;
+    const ctb_view* ins[7] = {scores, rules->query_start, rules->key_lengths, rules->prefix, rules->query_docs, rules->key_docs, rules->slopes};
+    if ((rc = check_no_alias(out, ins, 7, who))) return rc;
+    return launch_score_softmax(g, s, (float*)elem_ptr_mut(out), (cudaStream_t)stream);
+}
+
+size_t ctb_score_softmax_workspace_bytes(const ctb_view* probs) {
+    if (check_view(probs, "score_softmax: null input", "score_softmax") || probs->ndim != 4) return 0;
+    return ((size_t)probs->shape[0] * (size_t)probs->shape[1] * (size_t)probs->shape[2] * sizeof(double) + 255) / 256 * 256;
+}
+
+int ctb_score_softmax_backward(const ctb_view* grad, const ctb_view* probs, const ctb_view* scores, const ctb_score_rules* rules,
+                               const ctb_view* grad_scores, const ctb_view* grad_slopes, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+    const char* who = "score_softmax_backward";
+    int rc;
+    ScoreRows pr, dp, s{nullptr, 0, 0, 0};
+    ScoreGeom g;
+    if ((rc = score_operand(probs, "score_softmax: null input", who, nullptr, &pr))) return rc;
+    if ((rc = score_operand(grad, "backward: null gradient", who, probs, &dp))) return rc;
+    if ((rc = score_geometry(probs, rules, who, &g))) return rc;
+    if (g.cap > 0.0f && (rc = score_operand(scores, "score_softmax_backward: the scores are needed with a cap", who, probs, &s))) return rc;
+    if ((rc = check_out(grad_scores, view_numel(probs), CTB_F32, who))) return rc;
+    if ((rc = check_element_alignment(grad_scores, who))) return rc;
+    if (grad_slopes) {
+        if (!rules->slopes) return set_error(CTB_ERR_ARG, "%s: a gradient of slopes without slopes", who);
+        if ((rc = check_out(grad_slopes, g.heads, CTB_F32, who))) return rc;
+        if ((rc = check_element_alignment(grad_slopes, who))) return rc;
+    }
+    const ctb_view* ins[9] = {grad, probs, g.cap > 0.0f ? scores : nullptr, rules->query_start, rules->key_lengths, rules->prefix, rules->query_docs, rules->key_docs, rules->slopes};
+    const ctb_view* outs[2] = {grad_scores, grad_slopes};
+    if ((rc = check_outputs_apart(outs, 2, ins, 9, who))) return rc;
+    void* ws = nullptr;
+    if (grad_slopes && (rc = scratch_for(workspace, workspace_bytes, ctb_score_softmax_workspace_bytes(probs), who, &ws, (cudaStream_t)stream))) return rc;
+    return launch_score_softmax_backward(g, dp, pr, s, (float*)elem_ptr_mut(grad_scores), grad_slopes ? (float*)elem_ptr_mut(grad_slopes) : nullptr,
+                                         (double*)ws, (cudaStream_t)stream);
+}
+
+int ctb_residual_norm(const ctb_view* x, const ctb_view* f, const ctb_view* gate, const ctb_residual_norm_params* params,
+                      const ctb_view* y, const ctb_view* h, const ctb_view* stats, void* stream) {
+    const char* who = "residual_norm";
+    int rc;
+    RowsIn xr, fr{nullptr, 0};
+    ResidualNormGeom g;
+    if ((rc = norm_rows(x, "residual_norm: null input", who, nullptr, &xr))) return rc;
+    if (f && (rc = norm_rows(f, "residual_norm: null block output", who, x, &fr))) return rc;
+    if ((rc = norm_geometry(x, gate, params, who, &g))) return rc;
+    if (!f && (gate || g.post_kind != CTB_NORM_NONE)) return set_error(CTB_ERR_ARG, "%s: a gate or a post norm without a block output", who);
+    if (!f != !y) return set_error(CTB_ERR_ARG, "%s: y is written when there is a block output, and only then", who);
+    if ((g.pre_kind == CTB_NORM_NONE) != !h) return set_error(CTB_ERR_ARG, "%s: h is written when there is a pre norm, and only then", who);
+    if (y && (rc = check_out(y, g.rows * g.cols, CTB_F32, who))) return rc;
+    if (h && (rc = check_out(h, g.rows * g.cols, CTB_F32, who))) return rc;
+    if (stats && (rc = norm_stats(stats, g, who))) return rc;
+    const ctb_view* ins[7] = {x, f, gate, params->post_weight, params->post_bias, params->pre_weight, params->pre_bias};
+    const ctb_view* outs[3] = {y, h, stats};
+    for (const ctb_view* o : outs)
+        if ((rc = check_element_alignment(o, who))) return rc;
+    if ((rc = check_outputs_apart(outs, 3, ins, 7, who))) return rc;
+    if (!y && !h && !stats) return set_error(CTB_ERR_NULL, "%s: no output requested", who);
+    return launch_residual_norm(g, xr, fr, y ? (float*)elem_ptr_mut(y) : nullptr, h ? (float*)elem_ptr_mut(h) : nullptr,
+                                stats ? (float*)elem_ptr_mut(stats) : nullptr, (cudaStream_t)stream);
+}
+
+size_t ctb_residual_norm_workspace_bytes(const ctb_view* y, const ctb_view* gate) {
+    const char* who = "residual_norm_backward";
+    RowsIn r;
+    ResidualNormGeom g;
+    ctb_residual_norm_params none;
+    memset(&none, 0, sizeof none);
+    if (norm_rows(y, "residual_norm: null input", who, nullptr, &r) || norm_geometry(y, gate, &none, who, &g)) return 0;
+    return norm_workspace(g);
+}
+
+int ctb_residual_norm_backward(const ctb_view* f, const ctb_view* y, const ctb_view* gate, const ctb_view* stats,
+                               const ctb_residual_norm_params* params, const ctb_view* grad_y, const ctb_view* grad_h,
+                               const ctb_residual_norm_grads* grads, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "residual_norm_backward";
+    int rc;
+    RowsIn fr{nullptr, 0}, yr, dy{nullptr, 0}, dh{nullptr, 0};
+    ResidualNormGeom g;
+    if ((rc = norm_rows(y, "residual_norm: null input", who, nullptr, &yr))) return rc;
+    if (f && (rc = norm_rows(f, "residual_norm: null block output", who, y, &fr))) return rc;
+    if ((rc = norm_geometry(y, gate, params, who, &g))) return rc;
+    if (!f && (gate || g.post_kind != CTB_NORM_NONE)) return set_error(CTB_ERR_ARG, "%s: a gate or a post norm without a block output", who);
+    if ((g.pre_kind == CTB_NORM_NONE) != !grad_h) return set_error(CTB_ERR_ARG, "%s: the gradient of h goes with a pre norm", who);
+    if (!grad_y && !grad_h) return set_error(CTB_ERR_NULL, "backward: null gradient");
+    if (grad_y && (rc = norm_rows(grad_y, "backward: null gradient", who, y, &dy))) return rc;
+    if (grad_h && (rc = norm_rows(grad_h, "backward: null gradient", who, y, &dh))) return rc;
+    if ((rc = norm_stats(stats, g, who))) return rc;
+    if (!grads) return set_error(CTB_ERR_NULL, "%s: no output requested", who);
+    if ((!f && (grads->f || grads->post_weight || grads->post_bias)) || (!gate && grads->gate) ||
+        (g.post_kind == CTB_NORM_NONE && (grads->post_weight || grads->post_bias)) || (g.pre_kind == CTB_NORM_NONE && (grads->pre_weight || grads->pre_bias)))
+        return set_error(CTB_ERR_ARG, "%s: a gradient of something that did not go in", who);
+    const int64_t all = g.rows * g.cols;
+    const ctb_view* outs[7] = {grads->x, grads->f, grads->gate, grads->post_weight, grads->post_bias, grads->pre_weight, grads->pre_bias};
+    const int64_t sizes[7] = {all, all, gate ? view_numel(gate) : 0, g.cols, g.cols, g.cols, g.cols};
+    bool any = false;
+    for (int i = 0; i < 7; ++i) {
+        if (!outs[i]) continue;
+        any = true;
+        if ((rc = check_out(outs[i], sizes[i], CTB_F32, who))) return rc;
+        if ((rc = check_element_alignment(outs[i], who))) return rc;
+    }
+    if (!any) return set_error(CTB_ERR_NULL, "%s: no output requested", who);
+    const ctb_view* ins[10] = {f, y, gate, stats, params->post_weight, params->post_bias, params->pre_weight, params->pre_bias, grad_y, grad_h};
+    if ((rc = check_outputs_apart(outs, 7, ins, 10, who))) return rc;
+    if (all == 0) {                                      // sums over nothing
+        for (int i = 2; i < 7; ++i)
+            if (outs[i] && sizes[i]) CTB_CUDA_TRY(cudaMemsetAsync(elem_ptr_mut(outs[i]), 0, (size_t)sizes[i] * sizeof(float), (cudaStream_t)stream));
+        return CTB_OK;
+    }
+    void* ws = nullptr;
+    if ((rc = scratch_for(workspace, workspace_bytes, norm_workspace(g), who, &ws, (cudaStream_t)stream))) return rc;
+    auto at = [](const ctb_view* v) { return v ? (float*)elem_ptr_mut(v) : nullptr; };
+    const ResidualNormGrads o{at(grads->x), at(grads->f), at(grads->gate), at(grads->post_weight), at(grads->post_bias), at(grads->pre_weight), at(grads->pre_bias)};
+    return launch_residual_norm_backward(g, fr, yr, (const float*)elem_ptr(stats), dy, dh, o, ws, (cudaStream_t)stream);
+}
+
+size_t ctb_grad_norm_workspace_bytes(int count) {
+    // the tensors of each of the two dtypes go out in lists of their own
+    return count > 0 ? clip_workspace_bytes(count, 1) : 0;
+}
+
+int ctb_grad_norm(const ctb_view* const* grads, int count, double p, const ctb_view* norm, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+    return clip_entry(grads, count, 0, 0.0, p, nullptr, norm, workspace, workspace_bytes, stream, "grad_norm");
+}
+
+int ctb_clip_grad_norm(const ctb_view* const* grads, int count, double max_norm, double p, const ctb_view* const* outs,
+                       const ctb_view* norm, void* workspace, size_t workspace_bytes, void* stream) {
+    return clip_entry(grads, count, 1, max_norm, p, outs, norm, workspace, workspace_bytes, stream, "clip_grad_norm");
 }
 
 // ---- host-buffer entry points --------------------------------------------------------------------------

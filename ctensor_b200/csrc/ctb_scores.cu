@@ -1,0 +1,505 @@
+// Attention scores to probabilities, and back: softmax over the admitted keys of every query with a scale,
+// a tanh cap, a bias that falls with distance, and causal / prefix / document / length masks.
+//
+//   t_j = cap * tanh(scale * s_j / cap) - slope * |pos - j|,  p_j = exp(t_j - max t) / sum exp(t - max t)
+//   D = sum_j p_j * dp_j,  ds_j = scale * (1 - tanh^2) * p_j * (dp_j - D)
+//   dslope = -sum_j |pos - j| * p_j * (dp_j - D)
+//
+// Causal, prefix and length rules admit a run of keys [0, live); only the document rule is decided key by
+// key.  Keys outside are neither read nor evaluated, their results are written as zeros.
+//
+// Bound by HBM: 4 bytes per admitted score in, 4 per element out; backward 8 (12 with a cap) in, 4 out.
+// Rows that fit are held in the registers of a warp or a CTA and read once (ScoreRow kernels); longer rows,
+// and few rows that are long, are swept twice by a cluster of CTAs (second sweep from L2).
+#include "ctb_scores.cuh"
+#include "ctb_team.cuh"
+
+namespace ctb {
+
+namespace {
+
+struct ScoreArgs {
+    ScoreGeom g;
+    ScoreRows s, p, dp;
+    float* out;
+    double* slope_part;                 // one per row; NULL: not wanted
+    int64_t rows;
+    FastDiv by_queries, by_heads;
+};
+
+// Where a row is and what its query may look at.
+struct ScorePlace {
+    int64_t b, h, i;
+    int live;                           // keys [0, live) may be admitted
+    int centre;                         // the key position nearest to the query's within [0, live)
+    float beyond;                       // |pos - centre|
+    float slope;
+    int doc;
+};
+__device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, int64_t row) {
+    const ScoreGeom& g = a.g;
+    ScorePlace w;
+    const uint32_t bh = fast_div((uint32_t)row, a.by_queries);
+    w.i = (uint32_t)row - bh * a.by_queries.d;
+    w.b = fast_div(bh, a.by_heads);
+    w.h = bh - (uint32_t)w.b * a.by_heads.d;
+    const int64_t pos = (g.query_start.p ? (int64_t)g.query_start.p[w.b * g.query_start.sb] : g.keys - g.queries) + w.i;
+    int64_t live = g.keys;
+    if (g.key_lengths.p) live = min(live, (int64_t)g.key_lengths.p[w.b * g.key_lengths.sb]);
+    if (g.causal) {
+        int64_t reach = pos + 1;
+        if (g.prefix.p) reach = max(reach, (int64_t)g.prefix.p[w.b * g.prefix.sb]);
+        live = min(live, reach);
+    }
+    live = max(live, (int64_t)0);
+    const int64_t centre = max(min(pos, live - 1), (int64_t)0);
+    w.live = (int)live;
+    w.centre = (int)centre;
+    w.beyond = (float)(pos > centre ? pos - centre : centre - pos);
+    w.slope = g.slopes ? g.slopes[w.h * g.slope_stride] : 0.0f;
+    w.doc = g.query_docs.p ? g.query_docs.p[w.b * g.query_docs.sb + w.i * g.query_docs.si] : 0;
+    return w;
+}
+__device__ __forceinline__ const float* score_row(const ScoreRows& r, const ScorePlace& w) { return r.p + w.b * r.sb + w.h * r.sh + w.i * r.sq; }
+
+// Rows start at any multiple of four bytes.  Columns are dealt out in fours counted from the output row's
+// address rounded down to 16 bytes, so whole fours of the output are aligned; a four holds the columns
+// c0 .. c0 + 3, of which some may lie outside the row.
+__device__ __forceinline__ int score_phase(const float* row) { return (int)(((uintptr_t)row >> 2) & 3); }
+
+// The admitted ones of the columns c0 .. c0 + 3, as bits.
+template <bool DOCS>
+__device__ __forceinline__ uint32_t score_admitted(const ScoreArgs& a, const ScorePlace& w, int c0) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) bits |= (uint32_t)(c0 + k >= 0 && c0 + k < w.live) << k;
+    if (DOCS && bits) {
+        const int32_t* docs = a.g.key_docs.p + w.b * a.g.key_docs.sb;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if ((bits >> k) & 1u)
+                if (docs[(int64_t)(c0 + k) * a.g.key_docs.si] != w.doc) bits &= ~(1u << k);
+    }
+    return bits;
+}
+
+// The admitted values of four columns (0 elsewhere).  `aligned`: the row's fours are 16-byte aligned.
+__device__ __forceinline__ void score_load(float (&v)[4], const float* row, int c0, uint32_t bits, bool aligned) {
+    if (bits == 15u && aligned) {
+        const Vec<float, 4> q = ldg_stream(reinterpret_cast<const Vec<float, 4>*>(row + c0));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = q.v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (bits >> k) & 1u ? row[c0 + k] : 0.0f;
+    }
+}
+__device__ __forceinline__ void score_store(float* row, int c0, int keys, const float (&v)[4]) {
+    if (c0 >= 0 && c0 + 4 <= keys) {
+        Vec<float, 4> q;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q.v[k] = v[k];
+        stg_stream(reinterpret_cast<Vec<float, 4>*>(row + c0), q);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (c0 + k >= 0 && c0 + k < keys) row[c0 + k] = v[k];
+    }
+}
+
+// t of one column.  The bias is taken from the key nearest to the query, which changes no probability
+// (a softmax does not see a constant) and keeps t small where the query is far from every key.
+template <bool CAP>
+__device__ __forceinline__ float score_logit(const ScoreGeom& g, const ScorePlace& w, float s, int col) {
+    float t = CAP ? g.cap * tanhf(s * g.over_cap) : s * g.scale;
+    if (g.slopes) t = fmaf(-w.slope, (float)abs(col - w.centre), t);
+    return t;
+}
+
+template <int THREADS, int T, int NV, bool CAP, bool DOCS>
+__global__ void __launch_bounds__(THREADS)
+score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
+    static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
+    __shared__ TeamSlots<THREADS, 1, float> sh;
+    const int tid = threadIdx.x % T;
+    const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
+    if (row >= a.rows) return;                           // whole teams leave together
+    const ScorePlace w = score_place(a, row);
+    const int keys = (int)a.g.keys;
+    float* out = a.out + row * (int64_t)keys;
+    const float* s = score_row(a.s, w);
+    const int phase = score_phase(out);
+    const bool aligned = score_phase(s) == phase;
+    int turn = 0;
+    float t[NV][4];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(a, w, (v * T + tid) * 4 - phase) << (4 * v);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) score_load(t[v], s, (v * T + tid) * 4 - phase, (bits >> (4 * v)) & 15u, aligned);
+    float m[1] = {-INFINITY};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const uint32_t four = (bits >> (4 * v)) & 15u;
+        if (four) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                t[v][k] = (four >> k) & 1u ? score_logit<CAP>(a.g, w, t[v][k], (v * T + tid) * 4 - phase + k) : -INFINITY;
+                m[0] = fmaxf(m[0], t[v][k]);
+            }
+        }
+    }
+    team_fold<FoldMax, THREADS, T>(m, sh, turn, 1);
+    const float top = m[0] == -INFINITY ? 0.0f : m[0];
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        if ((bits >> (4 * v)) & 15u) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                t[v][k] = expf(t[v][k] - top);
+                part[k] = part[k] + t[v][k];
+            }
+        }
+    }
+    float z[1] = {(part[0] + part[1]) + (part[2] + part[3])};
+    team_fold<FoldSum, THREADS, T>(z, sh, turn, 1);
+    const float inv = z[0] == 0.0f ? 0.0f : __frcp_rn(z[0]);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int c0 = (v * T + tid) * 4 - phase;
+        if (c0 < keys) {
+            float p[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) p[k] = (bits >> (4 * v + k)) & 1u ? t[v][k] * inv : 0.0f;
+            score_store(out, c0, keys, p);
+        }
+    }
+}
+
+template <int THREADS, int T, int NV, bool CAP, bool DOCS>
+__global__ void __launch_bounds__(THREADS)
+score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
+    static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
+    __shared__ TeamSlots<THREADS, 1, float> sh;
+    __shared__ TeamSlots<THREADS, 1, double> sh_slope;
+    const int tid = threadIdx.x % T;
+    const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
+    if (row >= a.rows) return;
+    const ScorePlace w = score_place(a, row);
+    const int keys = (int)a.g.keys;
+    float* out = a.out + row * (int64_t)keys;
+    const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
+    const int phase = score_phase(out);
+    const bool p_aligned = score_phase(pr) == phase, g_aligned = score_phase(gr) == phase, s_aligned = CAP && score_phase(sr) == phase;
+    int turn = 0;
+    float p[NV][4], dp[NV][4], s[CAP ? NV : 1][4];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(a, w, (v * T + tid) * 4 - phase) << (4 * v);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int c0 = (v * T + tid) * 4 - phase;
+        const uint32_t four = (bits >> (4 * v)) & 15u;
+        score_load(p[v], pr, c0, four, p_aligned);
+        score_load(dp[v], gr, c0, four, g_aligned);
+        if (CAP) score_load(s[v], sr, c0, four, s_aligned);
+    }
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[k] = fmaf(p[v][k], dp[v][k], part[k]);
+    float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
+    team_fold<FoldSum, THREADS, T>(d, sh, turn, 1);
+    float slope_sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int c0 = (v * T + tid) * 4 - phase;
+        if (c0 < keys) {
+            float r[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float dt = p[v][k] * (dp[v][k] - d[0]);
+                if (a.slope_part && ((bits >> (4 * v + k)) & 1u)) slope_sum = fmaf((float)abs(c0 + k - w.centre) + w.beyond, dt, slope_sum);
+                r[k] = dt * a.g.scale;
+                if (CAP) {
+                    const float th = tanhf(s[v][k] * a.g.over_cap);
+                    r[k] = r[k] * fmaf(-th, th, 1.0f);
+                }
+                if (!((bits >> (4 * v + k)) & 1u)) r[k] = 0.0f;
+            }
+            score_store(out, c0, keys, r);
+        }
+    }
+    if (a.slope_part) {
+        double sum[1] = {(double)slope_sum};
+        team_fold<FoldSum, THREADS, T>(sum, sh_slope, turn, 1);
+        if (tid == 0) a.slope_part[row] = sum[0];
+    }
+}
+
+// ---- rows swept by a cluster ----------------------------------------------------------------------------
+// CTA `rank` of the row's `cs` CTAs has the fours [rank * share, (rank + 1) * share).
+constexpr int kSweepThreads = 512;
+constexpr int kSweepBatch = 4;                           // fours in flight per thread and operand
+
+struct SweepSpan { int64_t lo, hi; };
+__device__ __forceinline__ SweepSpan sweep_span(int64_t keys, int phase, int cs) {
+    const int64_t fours = (keys + phase + 3) / 4, share = (fours + cs - 1) / cs;
+    const int64_t lo = share * (cs > 1 ? cluster_rank() : 0);
+    return {lo, min(fours, lo + share)};
+}
+
+template <bool CAP, bool DOCS>
+__global__ void __launch_bounds__(kSweepThreads)
+score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
+    __shared__ TeamSlots<kSweepThreads, 1, float> sh;
+    const int64_t row = blockIdx.x / cs;
+    const ScorePlace w = score_place(a, row);
+    const int keys = (int)a.g.keys;
+    float* out = a.out + row * (int64_t)keys;
+    const float* s = score_row(a.s, w);
+    const int phase = score_phase(out);
+    const bool aligned = score_phase(s) == phase;
+    const SweepSpan span = sweep_span(keys, phase, cs);
+    const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
+    int turn = 0;
+    // first sweep: the thread's maximum and its sum of exponentials relative to that maximum
+    float m = -INFINITY, z = 0.0f;
+    for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
+        float t[kSweepBatch][4];
+        uint32_t bits[kSweepBatch];
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) {
+            const int64_t at = f + (int64_t)u * kSweepThreads;
+            bits[u] = at < live_end ? score_admitted<DOCS>(a, w, (int)(at * 4) - phase) : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                t[u][k] = (bits[u] >> k) & 1u ? score_logit<CAP>(a.g, w, t[u][k], (int)((f + (int64_t)u * kSweepThreads) * 4) - phase + k) : -INFINITY;
+                top = fmaxf(top, t[u][k]);
+            }
+        if (m != -INFINITY) z = z * expf(m - top);
+        m = top;
+        const float from = m == -INFINITY ? 0.0f : m;
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u)
+            if (bits[u]) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) part[k] = part[k] + expf(t[u][k] - from);
+            }
+        z = z + ((part[0] + part[1]) + (part[2] + part[3]));
+    }
+    float top[1] = {m};
+    team_fold<FoldMax, kSweepThreads, kSweepThreads>(top, sh, turn, cs);
+    const float from = top[0] == -INFINITY ? 0.0f : top[0];
+    float sum[1] = {m == -INFINITY ? z : z * expf(m - from)};
+    team_fold<FoldSum, kSweepThreads, kSweepThreads>(sum, sh, turn, cs);
+    const float inv = sum[0] == 0.0f ? 0.0f : __frcp_rn(sum[0]);
+    // second sweep
+    for (int64_t f = span.lo + threadIdx.x; f < span.hi; f += kSweepThreads * kSweepBatch) {
+        float t[kSweepBatch][4];
+        uint32_t bits[kSweepBatch];
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) {
+            const int64_t at = f + (int64_t)u * kSweepThreads;
+            bits[u] = at < live_end ? score_admitted<DOCS>(a, w, (int)(at * 4) - phase) : 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) {
+            const int64_t at = f + (int64_t)u * kSweepThreads;
+            if (at >= span.hi) break;
+            const int c0 = (int)(at * 4) - phase;
+            float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if ((bits[u] >> k) & 1u) p[k] = expf(score_logit<CAP>(a.g, w, t[u][k], c0 + k) - from) * inv;
+            score_store(out, c0, keys, p);
+        }
+    }
+}
+
+template <bool CAP, bool DOCS>
+__global__ void __launch_bounds__(kSweepThreads)
+score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
+    __shared__ TeamSlots<kSweepThreads, 1, float> sh;
+    __shared__ TeamSlots<kSweepThreads, 1, double> sh_slope;
+    const int64_t row = blockIdx.x / cs;
+    const ScorePlace w = score_place(a, row);
+    const int keys = (int)a.g.keys;
+    float* out = a.out + row * (int64_t)keys;
+    const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
+    const int phase = score_phase(out);
+    const bool p_aligned = score_phase(pr) == phase, g_aligned = score_phase(gr) == phase, s_aligned = CAP && score_phase(sr) == phase;
+    const SweepSpan span = sweep_span(keys, phase, cs);
+    const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
+    int turn = 0;
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
+        float p[kSweepBatch][4], dp[kSweepBatch][4];
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) {
+            const int64_t at = f + (int64_t)u * kSweepThreads;
+            const int c0 = (int)(at * 4) - phase;
+            const uint32_t bits = at < live_end ? score_admitted<DOCS>(a, w, c0) : 0u;
+            score_load(p[u], pr, c0, bits, p_aligned);
+            score_load(dp[u], gr, c0, bits, g_aligned);
+        }
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) part[k] = fmaf(p[u][k], dp[u][k], part[k]);
+    }
+    float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
+    team_fold<FoldSum, kSweepThreads, kSweepThreads>(d, sh, turn, cs);
+    double slope_sum = 0.0;
+    for (int64_t f = span.lo + threadIdx.x; f < span.hi; f += kSweepThreads * kSweepBatch) {
+        float p[kSweepBatch][4], dp[kSweepBatch][4], s[kSweepBatch][4];
+        uint32_t bits[kSweepBatch];
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) {
+            const int64_t at = f + (int64_t)u * kSweepThreads;
+            const int c0 = (int)(at * 4) - phase;
+            bits[u] = at < live_end ? score_admitted<DOCS>(a, w, c0) : 0u;
+            score_load(p[u], pr, c0, bits[u], p_aligned);
+            score_load(dp[u], gr, c0, bits[u], g_aligned);
+            if (CAP) score_load(s[u], sr, c0, bits[u], s_aligned);
+        }
+        float slope_part = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) {
+            const int64_t at = f + (int64_t)u * kSweepThreads;
+            if (at >= span.hi) break;
+            const int c0 = (int)(at * 4) - phase;
+            float r[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool in = (bits[u] >> k) & 1u;
+                const float dt = p[u][k] * (dp[u][k] - d[0]);
+                if (a.slope_part && in) slope_part = fmaf((float)abs(c0 + k - w.centre) + w.beyond, dt, slope_part);
+                r[k] = dt * a.g.scale;
+                if (CAP) {
+                    const float th = tanhf(s[u][k] * a.g.over_cap);
+                    r[k] = r[k] * fmaf(-th, th, 1.0f);
+                }
+                if (!in) r[k] = 0.0f;
+            }
+            score_store(out, c0, keys, r);
+        }
+        slope_sum = slope_sum + (double)slope_part;
+    }
+    if (a.slope_part) {
+        double sum[1] = {slope_sum};
+        team_fold<FoldSum, kSweepThreads, kSweepThreads>(sum, sh_slope, turn, cs);
+        if (threadIdx.x == 0 && (cs == 1 || cluster_rank() == 0)) a.slope_part[row] = sum[0];
+    }
+}
+
+// grad_slopes[h] = -sum over the head's rows of part, in a fixed order.
+__global__ void __launch_bounds__(256)
+score_slope_fold_kernel(const double* __restrict__ part, int64_t batch, int64_t heads, int64_t queries, float* __restrict__ out) {
+    __shared__ TeamSlots<256, 1, double> sh;
+    const int64_t h = blockIdx.x;
+    double sum[1] = {0.0};
+    for (int64_t b = 0; b < batch; ++b)
+        for (int64_t i = threadIdx.x; i < queries; i += 256) sum[0] = sum[0] + part[(b * heads + h) * queries + i];
+    int turn = 0;
+    team_fold<FoldSum, 256, 256>(sum, sh, turn, 1);
+    if (threadIdx.x == 0) out[h] = (float)-sum[0];
+}
+
+// ---- host -----------------------------------------------------------------------------------------------
+template <int THREADS, int T, int NV>
+int rows_as(const ScoreArgs& a, bool backward, bool cap, bool docs, cudaStream_t st) {
+    const int64_t blocks = ceil_div(a.rows, (int64_t)(THREADS / T));
+    const char* who = "score_softmax";
+    if (backward) {
+        if (cap) return docs ? launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, true, true>, blocks, THREADS, 0, 1, st, a)
+                             : launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, true, false>, blocks, THREADS, 0, 1, st, a);
+        return docs ? launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, false, true>, blocks, THREADS, 0, 1, st, a)
+                    : launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, false, false>, blocks, THREADS, 0, 1, st, a);
+    }
+    if (cap) return docs ? launch_clusters(who, score_softmax_kernel<THREADS, T, NV, true, true>, blocks, THREADS, 0, 1, st, a)
+                         : launch_clusters(who, score_softmax_kernel<THREADS, T, NV, true, false>, blocks, THREADS, 0, 1, st, a);
+    return docs ? launch_clusters(who, score_softmax_kernel<THREADS, T, NV, false, true>, blocks, THREADS, 0, 1, st, a)
+                : launch_clusters(who, score_softmax_kernel<THREADS, T, NV, false, false>, blocks, THREADS, 0, 1, st, a);
+}
+
+int sweep(const ScoreArgs& a, bool backward, bool cap, bool docs, int sm_count, cudaStream_t st) {
+    // as many CTAs per row as it takes to occupy the machine, while each has at least 4096 keys
+    int cs = 1;
+    while (cs < kMaxCluster && a.rows * cs < 2 * sm_count && a.g.keys / (2 * cs) >= 4096) cs *= 2;
+    const int64_t blocks = a.rows * cs;
+    const char* who = "score_softmax";
+    if (backward) {
+        if (cap) return docs ? launch_clusters(who, score_softmax_backward_sweep_kernel<true, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
+                             : launch_clusters(who, score_softmax_backward_sweep_kernel<true, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
+        return docs ? launch_clusters(who, score_softmax_backward_sweep_kernel<false, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
+                    : launch_clusters(who, score_softmax_backward_sweep_kernel<false, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
+    }
+    if (cap) return docs ? launch_clusters(who, score_softmax_sweep_kernel<true, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
+                         : launch_clusters(who, score_softmax_sweep_kernel<true, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
+    return docs ? launch_clusters(who, score_softmax_sweep_kernel<false, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
+                : launch_clusters(who, score_softmax_sweep_kernel<false, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
+}
+
+int launch_scores(ScoreArgs& a, bool backward, cudaStream_t st) {
+    a.rows = a.g.batch * a.g.heads * a.g.queries;
+    if (a.rows == 0 || a.g.keys == 0) return CTB_OK;
+    if (a.rows > 0x7FFFFFFFll || a.g.keys > (1ll << 30)) return set_error(CTB_ERR_LIMIT, "score_softmax: more than 2^31 - 1 rows or 2^30 keys");
+    DeviceInfo di;
+    if (int rc = current_device_info(&di)) return rc;
+    a.by_queries = make_fastdiv((uint32_t)a.g.queries);
+    a.by_heads = make_fastdiv((uint32_t)a.g.heads);
+    const bool cap = a.g.cap > 0.0f, docs = a.g.key_docs.p != nullptr;
+    // columns to deal out: up to three more than the keys where rows do not start on 16 bytes
+    const int64_t n = a.g.keys % 4 == 0 && is_aligned(a.out, 16) ? a.g.keys : a.g.keys + 3;
+    if (n <= 128) return rows_as<256, 32, 1>(a, backward, cap, docs, st);
+    if (n <= 256) return rows_as<256, 32, 2>(a, backward, cap, docs, st);
+    if (n <= 512) return rows_as<256, 32, 4>(a, backward, cap, docs, st);
+    if (n <= 1024) return rows_as<256, 32, 8>(a, backward, cap, docs, st);
+    if (n <= 2048) return rows_as<256, 128, 4>(a, backward, cap, docs, st);
+    if (n <= 4096) return rows_as<256, 256, 4>(a, backward, cap, docs, st);
+    if (n <= 8192) return rows_as<512, 512, 4>(a, backward, cap, docs, st);
+    return sweep(a, backward, cap, docs, di.sm_count, st);
+}
+
+}  // namespace
+
+int launch_score_softmax(const ScoreGeom& g, ScoreRows scores, float* out, cudaStream_t st) {
+    ScoreArgs a{};
+    a.g = g;
+    a.s = scores;
+    a.out = out;
+    return launch_scores(a, false, st);
+}
+
+int launch_score_softmax_backward(const ScoreGeom& g, ScoreRows grad, ScoreRows probs, ScoreRows scores, float* grad_scores,
+                                  float* grad_slopes, double* partials, cudaStream_t st) {
+    ScoreArgs a{};
+    a.g = g;
+    a.s = scores;
+    a.p = probs;
+    a.dp = grad;
+    a.out = grad_scores;
+    a.slope_part = grad_slopes ? partials : nullptr;
+    if (int rc = launch_scores(a, true, st)) return rc;
+    if (!grad_slopes || g.heads == 0) return CTB_OK;
+    if (a.rows == 0 || g.keys == 0) {                    // sums over nothing
+        CTB_CUDA_TRY(cudaMemsetAsync(grad_slopes, 0, (size_t)g.heads * sizeof(float), st));
+        return CTB_OK;
+    }
+    score_slope_fold_kernel<<<(unsigned)g.heads, 256, 0, st>>>(partials, g.batch, g.heads, g.queries, grad_slopes);
+    return cuda_error(cudaGetLastError(), "score_softmax_backward launch");
+}
+
+}  // namespace ctb

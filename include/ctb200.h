@@ -408,6 +408,99 @@ typedef struct ctb_optimizer_hyper {
 int ctb_optimizer_step(int kind, const ctb_view* param, const ctb_view* grad, float* state1,
                        float* state2, const ctb_optimizer_hyper* hyper, int step, void* stream);
 
+/* ---- a transformer block's steps between its matrix products -----------------------------------
+ * (The reference has no attention, no LayerNorm or RMS norm module and no gradient clipping; its users
+ * would spell these steps as operator chains like Loss::CrossEntropy's, src/neuralnet/loss.cpp:97-104.)
+ *
+ * Attention scores to probabilities, and the gradient of that step.  `scores` [batch, heads, queries,
+ * keys], Float32, keys contiguous, any strides outside them.  Query i of sequence b is at position
+ *   pos = query_start[b] + i       (query_start NULL: keys - queries, the last positions)
+ * and key j at position j.  A key is admitted when all of these hold:
+ *   j < key_lengths[b];  query_docs[b, i] == key_docs[b, j];  not causal, or j <= pos, or j < prefix[b].
+ * Over the admitted keys
+ *   t = scale * s;  cap > 0: t = cap * tanh(t / cap);  t -= slopes[head] * |pos - j|;  p = softmax(t)
+ * and p = 0 elsewhere, whatever the scores hold there (NaN included: masked places need not even be
+ * initialised).  A query that is admitted to no key, or only to scores of -inf, gets a row of zeros.
+ * An admitted NaN or +inf makes its row NaN in the admitted places, as the formula says.
+ * Unlike ctb_softmax_lastdim, whose mask and exponential follow the reference's chain, masked places are
+ * left out rather than lowered, and the exponential is the accurate one.
+ * Every pointer of ctb_score_rules may be NULL (that rule is then absent; query_docs and key_docs come
+ * together): query_start, key_lengths, prefix: Int32 [batch]; query_docs: Int32 [batch, queries];
+ * key_docs: Int32 [batch, keys]; slopes: Float32 [heads]; any strides.  Values outside 0..keys mean what
+ * the inequalities say.  cap 0: none. */
+typedef struct ctb_score_rules {
+    double scale, cap;
+    int32_t causal, reserved;
+    const ctb_view *query_start, *key_lengths, *prefix, *query_docs, *key_docs, *slopes;
+} ctb_score_rules;
+int ctb_score_softmax(const ctb_view* scores, const ctb_score_rules* rules, const ctb_view* out, void* stream);
+/* grad_scores = scale * (1 - tanh^2) * p * (grad - sum_j p * grad) at the admitted keys, 0 elsewhere (`grad`
+ * and `probs` are not looked at there).  `probs`: what ctb_score_softmax returned; `scores` is needed when
+ * cap > 0 and may be NULL otherwise.  grad_slopes (may be NULL): Float32 [heads], contiguous,
+ *   grad_slopes[h] = -sum over b, i, j of |pos - j| * p * (grad - sum_j p * grad).
+ * `workspace`: 256-byte aligned device memory of ctb_score_softmax_workspace_bytes(probs) bytes, used for
+ * grad_slopes only; NULL: the library's per-device workspace (see ctb_reduce). */
+size_t ctb_score_softmax_workspace_bytes(const ctb_view* probs);
+int ctb_score_softmax_backward(const ctb_view* grad, const ctb_view* probs, const ctb_view* scores,
+                               const ctb_score_rules* rules, const ctb_view* grad_scores,
+                               const ctb_view* grad_slopes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The norms on both sides of a residual block with the block's gate and residual scale, over the last dim:
+ *   n = N_post(f);  y = x + scale * gate * n;  h = N_pre(y)
+ * N(v) = (v - mean) * (var + eps)^-1/2 * weight + bias (CTB_NORM_LAYER, biased variance), or
+ * v * (mean(v^2) + eps)^-1/2 * weight + bias (CTB_NORM_RMS), or v (CTB_NORM_NONE).
+ * x, f: Float32, same shape, last dim contiguous and of at most CTB_RESIDUAL_NORM_MAX_COLS, the rows at one
+ * fixed distance (a slice of the columns of a wider buffer will do).  f may be NULL: y = x is then not
+ * written (y NULL), h = N_pre(x).  h is NULL when pre_kind is CTB_NORM_NONE.  Weights and biases: Float32
+ * [cols], contiguous, NULL = 1 / 0.  gate (NULL = 1): Float32 that broadcasts against x; outside the last dim
+ * its dims of extent 1 come after its full ones ([cols], [b, 1, cols], [b, t, cols], and the same with a last
+ * extent of 1).  y, h: contiguous, x's shape.  stats (may be NULL): Float32, contiguous, 16-byte aligned, 4
+ * values for every row: mean and rstd of f, mean and rstd of y (mean 0 for RMS; 0 and 1 without a norm). */
+enum ctb_norm_kind { CTB_NORM_NONE = 0, CTB_NORM_LAYER = 1, CTB_NORM_RMS = 2 };
+#define CTB_RESIDUAL_NORM_MAX_COLS 32768
+typedef struct ctb_residual_norm_params {
+    int32_t post_kind, pre_kind;
+    double post_eps, pre_eps, scale;
+    const ctb_view *post_weight, *post_bias, *pre_weight, *pre_bias;
+} ctb_residual_norm_params;
+int ctb_residual_norm(const ctb_view* x, const ctb_view* f, const ctb_view* gate,
+                      const ctb_residual_norm_params* params, const ctb_view* y, const ctb_view* h,
+                      const ctb_view* stats, void* stream);
+/* The gradients of everything that went in, from f, the forward's y (x when f was NULL) and stats, and the
+ * gradients of y and h.  grad_y may be NULL (zero) unless pre_kind is CTB_NORM_NONE, whose grad_h is NULL.
+ * Every member of `grads` may be NULL (not wanted); x, f: contiguous, the rows' shape; gate: contiguous, the
+ * gate's shape (summed over the dims in which it was broadcast); weights and biases: [cols].  Column sums are
+ * Float32 within up to a few thousand rows of one team and fp64 across teams, always in the same order.
+ * `workspace`: 256-byte aligned device memory of at least ctb_residual_norm_workspace_bytes(y, gate) bytes
+ * (gate as given to the call); NULL: the library's per-device workspace (see ctb_reduce). */
+typedef struct ctb_residual_norm_grads {
+    const ctb_view *x, *f, *gate, *post_weight, *post_bias, *pre_weight, *pre_bias;
+} ctb_residual_norm_grads;
+size_t ctb_residual_norm_workspace_bytes(const ctb_view* y, const ctb_view* gate);
+int ctb_residual_norm_backward(const ctb_view* f, const ctb_view* y, const ctb_view* gate, const ctb_view* stats,
+                               const ctb_residual_norm_params* params, const ctb_view* grad_y,
+                               const ctb_view* grad_h, const ctb_residual_norm_grads* grads, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* The norm of all gradients of a model as one vector, and scaling them down to a given norm before an
+ * optimizer step: norm = (sum |g|^p)^(1/p) with p = 1, 2 or infinity, summed in fp64.
+ * `grads`: `count` Float32 / Double64 views, each dense (some permutation of a gap-free block of memory),
+ * possibly empty; `norm`: one Float32 or Double64 element.
+ * ctb_clip_grad_norm also multiplies every gradient by max_norm / norm when max_norm < norm < infinity (the
+ * factor rounded to the gradient's type) and leaves it as it is otherwise: a norm that is infinite or NaN is
+ * for the caller to act on, the gradients then still show where it came from.  `outs` NULL: in place (no
+ * two gradients may overlap; where nothing is scaled nothing is written).  Otherwise the scaled — or unscaled —
+ * values go to outs[i] (grads[i]'s dtype, shape and strides), which must not overlap any gradient or each other.
+ * `workspace`: 256-byte aligned device memory of ctb_grad_norm_workspace_bytes(count) bytes; NULL: the
+ * library's per-device workspace (see ctb_reduce).  Give a workspace of its own to a call that is captured
+ * into a graph. */
+size_t ctb_grad_norm_workspace_bytes(int count);
+int ctb_grad_norm(const ctb_view* const* grads, int count, double p, const ctb_view* norm, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int ctb_clip_grad_norm(const ctb_view* const* grads, int count, double max_norm, double p,
+                       const ctb_view* const* outs, const ctb_view* norm, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* ---- host-buffer entry points ---------------------------------------------------------------
  * Same semantics as ctb_binary / ctb_unary / ctb_reduce, but every view points to HOST memory
  * (pinned memory gives full PCIe speed).  Inputs are staged to `device`, the kernel runs there
