@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -642,8 +643,58 @@ def layernorm(x, gamma=None, beta=None, eps: float = 1e-5, out=None):
 
 
 # ---- a transformer block's steps between its matrix products ------------------------------------------------
-def _opt_view(x):
-    return None if x is None else _as_dview(x).cview()
+# These calls take several tensors and return several, often around kernels of a few microseconds, so their
+# descriptors are packed in one go and results take their descriptor from an input of the same shape.
+_VIEW_PACK = [struct.Struct(f"=qqii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x") for n in range(MAX_DIMS + 1)]
+
+
+def _raw_view(x):
+    """The C descriptor of a tensor or DView (None stays None)."""
+    if x is None:
+        return None
+    if isinstance(x, DView):
+        return x.cview()
+    shape, n = x.shape, x.dim()
+    if n > MAX_DIMS:
+        raise CtbError(5, f"ndim {n} not in 0..{MAX_DIMS}")
+    return View.from_buffer_copy(_VIEW_PACK[n].pack(x.data_ptr(), 0, _dtype_code(x), n, *shape, *x.stride()))
+
+
+def _device_of(x) -> int:
+    """Index of the CUDA device that holds ``x``."""
+    index = (x.buf if isinstance(x, DView) else x).get_device()
+    if index < 0:
+        raise CtbError(6, "device entry point called with host memory")
+    return index
+
+
+def _on_device(index: int, what: str, tensors) -> None:
+    for t in tensors:
+        if t is not None and (t.buf if isinstance(t, DView) else t).get_device() != index:
+            raise CtbError(5, f"{what}: tensors on different devices")
+
+
+def _device_scope(index: int):
+    cuda = _torch().cuda
+    return _NO_GUARD if cuda.current_device() == index else cuda.device(index)
+
+
+def _stream_of(index: int) -> int:
+    return _torch().cuda.current_stream(index).cuda_stream
+
+
+def _new_like(x, view):
+    """A fresh contiguous tensor of x's shape and dtype, and its descriptor."""
+    torch = _torch()
+    if isinstance(x, DView):
+        out = _new_out(x, x.shape)
+        return out, _raw_view(out)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if not x.is_contiguous():
+        return out, _raw_view(out)
+    v = View.from_buffer_copy(view)
+    v.base = out.data_ptr()
+    return out, v
 
 
 def _address(cview):
@@ -651,16 +702,14 @@ def _address(cview):
     return None if cview is None else ctypes.addressof(cview)
 
 
-def _same_device(first: DView, others, what: str) -> None:
-    for o in others:
-        if o is not None and _as_dview(o).buf.device != first.buf.device:
-            raise CtbError(5, f"{what}: tensors on different devices")
-
-
-def _workspace(nbytes: int, like: DView):
-    """Scratch of one call, from torch's allocator: ordered on the current stream, and a captured graph's
-    own when the call is captured."""
-    return _torch().empty(nbytes, dtype=_torch().uint8, device=like.buf.device) if nbytes else None
+def _scratch(nbytes: int, index: int):
+    """(tensor, address, size) of one call's scratch, from torch's allocator: ordered on the current stream,
+    and a captured graph's own when the call is captured."""
+    if not nbytes:
+        return None, None, 0
+    torch = _torch()
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    return ws, ws.data_ptr(), nbytes
 
 
 class ScoreRules:
@@ -668,75 +717,84 @@ class ScoreRules:
     sequence ``query_start`` (position of its first query; default: keys - queries), ``key_lengths``,
     ``prefix`` (keys every query may look at) — int32 [batch] —, ``query_docs`` / ``key_docs`` (document
     numbers, int32 [batch, queries] / [batch, keys]) and ``slopes`` (float32 [heads], bias
-    -slope * |distance|).  Holds its tensors; their contents may change between calls."""
+    -slope * |distance|).  Holds its tensors; their contents may change between calls, their memory may not."""
     _TABLES = ("query_start", "key_lengths", "prefix", "query_docs", "key_docs", "slopes")
 
     def __init__(self, scale: float = 1.0, cap: float = 0.0, causal: bool = False, query_start=None, key_lengths=None,
                  prefix=None, query_docs=None, key_docs=None, slopes=None):
-        given = (query_start, key_lengths, prefix, query_docs, key_docs, slopes)
-        self.tables = {n: None if t is None else _as_dview(t) for n, t in zip(self._TABLES, given)}
-        self._views = {n: _opt_view(t) for n, t in self.tables.items()}
-        self.c = CScoreRules(float(scale), float(cap), int(bool(causal)), 0, *(_address(self._views[n]) for n in self._TABLES))
+        self.tables = (query_start, key_lengths, prefix, query_docs, key_docs, slopes)
+        self._views = [_raw_view(t) for t in self.tables]
+        self.c = CScoreRules(float(scale), float(cap), int(bool(causal)), 0, *(_address(v) for v in self._views))
 
 
 def score_softmax(scores, rules: ScoreRules, out=None):
     """Attention probabilities of ``scores`` [batch, heads, queries, keys] over the keys that ``rules``
     admit; zeros elsewhere and in the rows of queries that are admitted to nothing."""
-    s = _as_dview(scores)
-    _same_device(s, [out, *rules.tables.values()], "score_softmax")
-    if out is None:
-        out = _new_out(s, s.shape)
-    with _device_guard(s):
-        check(lib().ctb_score_softmax(s.cview(), ctypes.byref(rules.c), _as_dview(out).cview(), _stream_ptr(s)))
+    dev = _device_of(scores)
+    _on_device(dev, "score_softmax", rules.tables)
+    sv = _raw_view(scores)
+    with _device_scope(dev):
+        if out is None:
+            out, ov = _new_like(scores, sv)
+        else:
+            _on_device(dev, "score_softmax", (out,))
+            ov = _raw_view(out)
+        check(lib().ctb_score_softmax(sv, rules.c, ov, _stream_of(dev)))
     return out
 
 
 def score_softmax_backward(grad, probs, rules: ScoreRules, scores=None, want_slopes: bool = False, out=None):
     """(gradient of the scores, gradient of ``rules``' slopes or None) from the gradient of the
     probabilities; ``scores`` (the forward's input) is needed when the rules have a cap."""
-    g, p = _as_dview(grad), _as_dview(probs)
-    _same_device(p, [grad, scores, out, *rules.tables.values()], "score_softmax_backward")
-    if out is None:
-        out = _new_out(p, p.shape)
-    slopes = ws = None
-    if want_slopes and len(p.shape) == 4:
-        slopes = _new_out(p, (p.shape[1],))
-        ws = _workspace(int(lib().ctb_score_softmax_workspace_bytes(p.cview())), p)
-    with _device_guard(p):
-        check(lib().ctb_score_softmax_backward(g.cview(), p.cview(), _opt_view(scores), ctypes.byref(rules.c), _as_dview(out).cview(),
-                                               _opt_view(slopes), None if ws is None else ws.data_ptr(),
-                                               0 if ws is None else ws.numel(), _stream_ptr(p)))
+    dev = _device_of(probs)
+    _on_device(dev, "score_softmax_backward", (grad, scores, out) + rules.tables)
+    pv = _raw_view(probs)
+    slopes = slopes_view = None
+    with _device_scope(dev):
+        if out is None:
+            out, ov = _new_like(probs, pv)
+        else:
+            ov = _raw_view(out)
+        ws, at, nbytes = None, None, 0
+        if want_slopes and pv.ndim == 4:
+            slopes = _torch().empty(pv.shape[1], dtype=_torch().float32, device=out.device if not isinstance(out, DView) else out.buf.device)
+            slopes_view = _raw_view(slopes)
+            ws, at, nbytes = _scratch(lib().ctb_score_softmax_workspace_bytes(pv), dev)
+        check(lib().ctb_score_softmax_backward(_raw_view(grad), pv, _raw_view(scores), rules.c, ov, slopes_view, at, nbytes, _stream_of(dev)))
     return out, slopes
 
 
 class ResidualNorm:
     """The weights and kinds of ``residual_norm``: y = x + scale * gate * N_post(f), h = N_pre(y), each norm
     NORM_NONE, NORM_LAYER or NORM_RMS with an optional float32 weight and bias of the row length.  Holds
-    its tensors; their contents may change between calls."""
+    its tensors; their contents may change between calls, their memory may not."""
     _VECTORS = ("post_weight", "post_bias", "pre_weight", "pre_bias")
 
     def __init__(self, pre: int = NORM_LAYER, pre_weight=None, pre_bias=None, pre_eps: float = 1e-5, post: int = NORM_NONE,
                  post_weight=None, post_bias=None, post_eps: float = 1e-5, scale: float = 1.0):
         self.pre, self.post = pre, post
-        self.vectors = {n: None if t is None else _as_dview(t)
-                        for n, t in zip(self._VECTORS, (post_weight, post_bias, pre_weight, pre_bias))}
-        self._views = {n: _opt_view(t) for n, t in self.vectors.items()}
+        self.vectors = (post_weight, post_bias, pre_weight, pre_bias)
+        self._views = [_raw_view(t) for t in self.vectors]
         self.c = CResidualNormParams(int(post), int(pre), float(post_eps), float(pre_eps), float(scale),
-                                     *(_address(self._views[n]) for n in self._VECTORS))
+                                     *(_address(v) for v in self._views))
 
 
 def residual_norm(x, f, params: ResidualNorm, gate=None):
     """(y, h, stats): the residual stream after a block's output ``f`` is added, its norm for the next block,
     and the rows' statistics [..., 4] for the backward pass.  ``f`` None: y is ``x`` itself; h is None when
     ``params`` has no pre norm."""
-    xv = _as_dview(x)
-    _same_device(xv, [f, gate, *params.vectors.values()], "residual_norm")
-    y = x if f is None else _new_out(xv, xv.shape)
-    h = None if params.pre == NORM_NONE else _new_out(xv, xv.shape)
-    stats = _new_out(xv, tuple(xv.shape[:-1]) + (4,))
-    with _device_guard(xv):
-        check(lib().ctb_residual_norm(xv.cview(), _opt_view(f), _opt_view(gate), ctypes.byref(params.c),
-                                      None if f is None else _opt_view(y), _opt_view(h), _opt_view(stats), _stream_ptr(xv)))
+    dev = _device_of(x)
+    _on_device(dev, "residual_norm", (f, gate) + params.vectors)
+    xv = _raw_view(x)
+    y, yv, h, hv = x, None, None, None
+    with _device_scope(dev):
+        if f is not None:
+            y, yv = _new_like(x, xv)
+        if params.pre != NORM_NONE:
+            h, hv = _new_like(x, xv)
+        like = x.buf if isinstance(x, DView) else x
+        stats = like.new_empty(tuple(x.shape[:-1]) + (4,))
+        check(lib().ctb_residual_norm(xv, _raw_view(f), _raw_view(gate), params.c, yv, hv, _raw_view(stats), _stream_of(dev)))
     return y, h, stats
 
 
@@ -755,26 +813,17 @@ class ResidualNormGrads:
 def residual_norm_backward(f, y, stats, params: ResidualNorm, grad_y=None, grad_h=None, gate=None) -> ResidualNormGrads:
     """The gradients of x, f, the gate, the weights and the biases, from the forward's f, y and stats and
     the gradients of y and h (``grad_y`` None: zero; ``grad_h`` goes with a pre norm)."""
-    yv = _as_dview(y)
-    _same_device(yv, [f, stats, grad_y, grad_h, gate, *params.vectors.values()], "residual_norm_backward")
-    out = ResidualNormGrads(x=_new_out(yv, yv.shape))
-    if f is not None:
-        out.f = _new_out(yv, yv.shape)
-    if gate is not None:
-        out.gate = _new_out(yv, _as_dview(gate).shape)
-    for name, vector in params.vectors.items():
-        if vector is not None:
-            setattr(out, name, _new_out(yv, vector.shape))
-    views = [_opt_view(getattr(out, n)) for n, _ in CResidualNormGrads._fields_]
-    c = CResidualNormGrads(*(_address(v) for v in views))
-    gate_view = _opt_view(gate)
-    ws = _workspace(int(lib().ctb_residual_norm_workspace_bytes(yv.cview(), gate_view)), yv)
-    with _device_guard(yv):
-        check(lib().ctb_residual_norm_backward(_opt_view(f), yv.cview(), gate_view, _opt_view(stats), ctypes.byref(params.c),
-                                               _opt_view(grad_y), _opt_view(grad_h), ctypes.byref(c),
-                                               None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-                                               _stream_ptr(yv)))
-    return out
+    dev = _device_of(y)
+    _on_device(dev, "residual_norm_backward", (f, stats, grad_y, grad_h, gate) + params.vectors)
+    yv, gv = _raw_view(y), _raw_view(gate)
+    with _device_scope(dev):
+        outs = [_new_like(y, yv), (None, None) if f is None else _new_like(y, yv), (None, None) if gate is None else _new_like(gate, gv)]
+        outs += [(None, None) if t is None else _new_like(t, v) for t, v in zip(params.vectors, params._views)]
+        c = CResidualNormGrads(*(_address(v) for _, v in outs))
+        ws, at, nbytes = _scratch(lib().ctb_residual_norm_workspace_bytes(yv, gv), dev)
+        check(lib().ctb_residual_norm_backward(_raw_view(f), yv, gv, _raw_view(stats), params.c, _raw_view(grad_y), _raw_view(grad_h), c,
+                                               at, nbytes, _stream_of(dev)))
+    return ResidualNormGrads(*(t for t, _ in outs))
 
 
 class TensorList:
@@ -783,14 +832,12 @@ class TensorList:
 
     def __init__(self, tensors):
         self.tensors = list(tensors)
-        views = [_as_dview(t) for t in self.tensors]
-        for v in views:
-            if v.buf.device != views[0].buf.device:
-                raise CtbError(5, "TensorList: tensors on different devices")
-        self.device_view = views[0] if views else None
-        self.has_f64 = any(v.dtype == F64 for v in views)
-        self._views = [v.cview() for v in views]
-        self.c = (ctypes.POINTER(View) * max(1, len(views)))(*[ctypes.pointer(c) for c in self._views])
+        self.device = _device_of(self.tensors[0]) if self.tensors else None
+        if self.tensors:
+            _on_device(self.device, "TensorList", self.tensors)
+        self._views = [_raw_view(t) for t in self.tensors]
+        self.has_f64 = any(v.dtype == F64 for v in self._views)
+        self.c = (ctypes.POINTER(View) * max(1, len(self._views)))(*[ctypes.pointer(v) for v in self._views])
 
     def __len__(self):
         return len(self.tensors)
@@ -803,22 +850,23 @@ def _grad_norm(grads, max_norm, p, out, norm):
         out = out if isinstance(out, TensorList) else TensorList(out)
         if len(out) != len(grads):
             raise CtbError(2, "clip_grad_norm: as many outputs as gradients are needed")
-    like = grads.device_view
-    if like is None:
+    dev = grads.device
+    if dev is None:
         if norm is None:
             raise CtbError(5, "grad_norm: an empty list needs `norm`, which says where the result goes")
-        like = _as_dview(norm)
-    if norm is None:
-        norm = torch.empty(1, dtype=torch.float64 if grads.has_f64 else torch.float32, device=like.buf.device)
-    _same_device(like, [norm] + ([] if out is None or out.device_view is None else [out.device_view]), "grad_norm")
-    ws = _workspace(int(lib().ctb_grad_norm_workspace_bytes(len(grads))), like)
-    ws_args = (None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-    with _device_guard(like):
+        dev = _device_of(norm)
+    if out is not None and out.device is not None and out.device != dev:
+        raise CtbError(5, "clip_grad_norm: tensors on different devices")
+    _on_device(dev, "grad_norm", (norm,))
+    with _device_scope(dev):
+        if norm is None:
+            norm = torch.empty(1, dtype=torch.float64 if grads.has_f64 else torch.float32, device=torch.device("cuda", dev))
+        ws, at, nbytes = _scratch(lib().ctb_grad_norm_workspace_bytes(len(grads)), dev)
         if max_norm is None:
-            check(lib().ctb_grad_norm(grads.c, len(grads), float(p), _as_dview(norm).cview(), *ws_args, _stream_ptr(like)))
+            check(lib().ctb_grad_norm(grads.c, len(grads), float(p), _raw_view(norm), at, nbytes, _stream_of(dev)))
         else:
             check(lib().ctb_clip_grad_norm(grads.c, len(grads), float(max_norm), float(p), None if out is None else out.c,
-                                           _as_dview(norm).cview(), *ws_args, _stream_ptr(like)))
+                                           _raw_view(norm), at, nbytes, _stream_of(dev)))
     return norm
 
 

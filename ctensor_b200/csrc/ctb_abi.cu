@@ -19,6 +19,7 @@
 #include "ctb_clip.cuh"
 #include "ctb_residual_norm.cuh"
 #include "ctb_scores.cuh"
+#include "ctb_team.cuh"
 
 namespace ctb {
 
@@ -71,6 +72,36 @@ int current_device_info(DeviceInfo* info) {
     }
     info->device = dev;
     info->sm_count = s.sm_count;
+    return CTB_OK;
+}
+
+// The query costs as much as a launch: its answers are kept (they depend on kernel, sizes and device only).
+int resident_clusters(const void* kernel, int threads, size_t smem, int cs, int* count) {
+    struct Known { const void* kernel; size_t smem; int device, threads, cs, count; };
+    static Known known[64];
+    static int n = 0;
+    int device = -1;
+    CTB_CUDA_TRY(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> lk(g_mu);
+    for (int i = 0; i < n; ++i)
+        if (known[i].kernel == kernel && known[i].smem == smem && known[i].device == device && known[i].threads == threads && known[i].cs == cs) {
+            *count = known[i].count;
+            return CTB_OK;
+        }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cs);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (smem > 48 * 1024) CTB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    CTB_CUDA_TRY(cudaOccupancyMaxActiveClusters(count, kernel, &cfg));
+    if (*count < 1) *count = 1;
+    if (n < 64) known[n++] = {kernel, smem, device, threads, cs, *count};
     return CTB_OK;
 }
 
@@ -1510,6 +1541,7 @@ int norm_geometry(const ctb_view* x, const ctb_view* gate, const ctb_residual_no
     if (g->cols > CTB_RESIDUAL_NORM_MAX_COLS) return set_error(CTB_ERR_LIMIT, "%s: rows of more than %d columns", who, CTB_RESIDUAL_NORM_MAX_COLS);
     g->rows = 1;
     for (int d = 0; d + 1 < x->ndim; ++d) g->rows *= x->shape[d];
+    if (g->rows > 0x7FFFFFFFll) return set_error(CTB_ERR_LIMIT, "%s: more than 2^31 - 1 rows", who);
     for (int kind : {p->post_kind, p->pre_kind})
         if (kind != CTB_NORM_NONE && kind != CTB_NORM_LAYER && kind != CTB_NORM_RMS) return set_error(CTB_ERR_ARG, "%s: unknown norm %d", who, kind);
     if (!(p->post_eps >= 0.0) || !(p->pre_eps >= 0.0) || !std::isfinite(p->post_eps) || !std::isfinite(p->pre_eps)) return set_error(CTB_ERR_ARG, "%s: eps must be finite and not negative", who);

@@ -70,6 +70,24 @@ __device__ __forceinline__ void store_part(float* row, int c, const float (&v)[V
     }
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+}
+
+// The thread's own four (or one) values of a stage slot.
+template <int VEC>
+__device__ __forceinline__ void read_own(float (&v)[VEC], const float* p) {
+    if constexpr (VEC == 4) {
+        const float4 q = *reinterpret_cast<const float4*>(p);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+        v[0] = *p;
+    }
+}
+
 // ---- forward ------------------------------------------------------------------------------------------
 // mean and rstd of a row from fp64 sums of v and v^2: one sum over the team instead of two, and no
 // cancellation that fp64 would notice until |mean| / sigma is about 1e6.
@@ -99,8 +117,13 @@ __device__ __forceinline__ void row_statistics(const float (&v)[E], int kind, fl
     *rstd = __frsqrt_rn((float)(var + (double)eps));
 }
 
+// Wide rows keep x in shared memory (each thread its own columns) until it is needed: 40 registers instead of
+// 59, so three CTAs of 512 threads share an SM and one row's folds hide behind the loads of two others.
+template <int THREADS, int T, int E, int VEC> constexpr bool kStageX = T == THREADS && E == 16 && VEC == 4;
+template <int THREADS, int T, int E, int VEC> constexpr int kForwardCtas = kStageX<THREADS, T, E, VEC> ? 1536 / THREADS : T == THREADS ? 1 : E == 32 ? 2 : 4;
+
 template <int THREADS, int T, int E, int VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, (kForwardCtas<THREADS, T, E, VEC>))
 residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ y, float* __restrict__ h, float* __restrict__ stats, int cs) {
     __shared__ TeamSlots<THREADS, 2, double> sh;
     const int tid = threadIdx.x % T;
@@ -111,20 +134,40 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
     const int64_t begin = slice * rank;
     const int width = (int)(begin >= g.cols ? 0 : (g.cols - begin < slice ? g.cols - begin : slice));
     int turn = 0;
+    constexpr bool STAGED = kStageX<THREADS, T, E, VEC>;
+    __shared__ __align__(16) float staged[STAGED ? E * THREADS : 1];
     float v[E], fv[E];
-    load_share<T, E, VEC>(v, x.p + row * x.stride + begin, width, tid);
+    if (STAGED && f.p) {
+#pragma unroll
+        for (int i = 0; i < E / VEC; ++i) {
+            const int c = col_of<T, VEC>(i, tid);
+            if (c < width) copy_async<VEC * 4>(staged + (i * THREADS + threadIdx.x) * VEC, x.p + row * x.stride + begin + c);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    } else {
+        load_share<T, E, VEC>(v, x.p + row * x.stride + begin, width, tid);
+    }
     float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
     if (f.p) {
         load_share<T, E, VEC>(fv, f.p + row * f.stride + begin, width, tid);
         if (g.post_kind != CTB_NORM_NONE) row_statistics<THREADS, T, E>(fv, g.post_kind, g.post_eps, g.inv_cols, sh, turn, cs, &st.x, &st.y);
-        const int64_t group = g.gate_mode == kGateNone ? 0 : row / g.gate_rows;
-        const float* gate = g.gate.p + group * g.gate.stride;
+        const float* gate = g.gate.p + (int64_t)fast_div((uint32_t)row, g.by_gate_rows) * g.gate.stride;
         const float one_gate = g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
+        if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < E / VEC; ++i) {
             const int c = col_of<T, VEC>(i, tid);
+            if (STAGED) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[i * VEC + k] = 0.0f;
+            }
             if (c < width) {
-                float n[VEC], out[VEC];
+                float n[VEC], out[VEC], xv[VEC];
+                if (STAGED) read_own<VEC>(xv, staged + (i * THREADS + threadIdx.x) * VEC);
+                else {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) xv[k] = v[i * VEC + k];
+                }
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) n[k] = fv[i * VEC + k];
                 if (g.post_kind != CTB_NORM_NONE) {
@@ -151,7 +194,7 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
                 }
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    out[k] = fmaf(one_gate, n[k], v[i * VEC + k]);
+                    out[k] = fmaf(one_gate, n[k], xv[k]);
                     v[i * VEC + k] = out[k];
                 }
                 store_part<VEC>(y + row * g.cols + begin, c, out);
@@ -187,287 +230,361 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
 }
 
 // ---- backward -------------------------------------------------------------------------------------------
-// Teams walk consecutive rows.  While a row is being worked on, the next one's operands are on their way
-// into shared memory (cp.async): each thread copies and later reads its own columns only, so there is
-// nothing to synchronise but the thread's own copies.  Column sums (weights, biases, a gate shared by
-// rows) stay in registers until the team's last row — a shared gate's until its last row in the team —
-// and are then written as partials; a second launch adds the partials in order.
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
-}
-
-enum { kInF = 0, kInY = 1, kInDy = 2, kInDh = 3, kInGate = 4, kInCount = 5 };
+// Teams walk consecutive rows.  While a row is being worked on, the next ones' operands are on their way
+// into shared memory (cp.async, a ring of two to four rows): each thread copies and later reads its own columns
+// only, so there is nothing to synchronise but the thread's own copies.
+//
+// One fold over the team per row.  The sums that df needs contain dx, which needs sums itself; but dx is
+// linear in them, dx = e - rstd_y * (m1 + yhat * m2) with e = dy + rstd_y * a, so with k = scale * gate * w_post
+//     sum(k dx)      = sum(k e)      - rstd_y * (m1 * sum(k)      + m2 * sum(k yhat))
+//     sum(k dx fhat) = sum(k e fhat) - rstd_y * (m1 * sum(k fhat) + m2 * sum(k fhat yhat))
+// and all eight sums are taken together.  Without a LayerNorm (m1 and the mean of k dx drop out) three remain.
+//
+// Column sums (weights, biases, a gate shared by rows) stay in registers until the team's last row — a shared
+// gate's until its last row in the team — and go out as partials, which a second launch adds in order.
+enum { kInY = 0, kInDh = 1, kInDy = 2, kInF = 3, kInGate = 4, kInCount = 5 };
 
 struct ResidualBwd {
     ResidualNormGeom g;
     RowsIn in[kInCount];            // p == NULL: not read; [kInGate] only where the gate has a row for every row
+    int32_t stages;                 // rows in the ring, 2..4
     const float* stats;
     ResidualNormGrads out;
     int32_t shared_gate;            // the gate's gradient is summed over rows (kGateRow, gate_rows > 1)
     int64_t teams;
-    float* part;                    // [pre_weight, pre_bias, post_weight, post_bias][teams][cols]
+    int64_t parts;                  // rows of partial column sums: one per CTA (column slice)
+    float* part;                    // [pre_weight, pre_bias, post_weight, post_bias, gate][parts][cols]
     float* gate_part;               // [teams + groups][cols or 1]: slot team + group
+    int32_t one_gate_row;           // all rows share one gate row: its sums go to `part`
 };
 
-template <int E, int VEC>
-__device__ __forceinline__ void read_staged(float (&v)[VEC], const float* stage, int threads, int i) {
-    if constexpr (VEC == 4) {
-        const float4 q = reinterpret_cast<const float4*>(stage)[i * threads + threadIdx.x];
-        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else {
-        v[0] = stage[i * threads + threadIdx.x];
-    }
-}
+// What a launch is specialised for.  A specialised kernel (FAST) has a pre norm with a weight, the gradient of y
+// and, if POST, a post norm with a weight; all of its gradients are wanted, the gate's for GATE != 0: 1 = a row
+// that rows share, 2 = a row for every row.  Otherwise every one of these is looked up at run time, the
+// flags then only say that the sums have a place: that took 640 instructions per warp and row where the
+// specialised kernel takes a third of it, and instructions, not bytes, bound narrow rows.
+// FULL: there may be LayerNorms and biases.
+template <bool FAST_, bool POST_, bool FULL_, int GATE_>
+struct BwdFlags {
+    static constexpr bool FAST = FAST_, POST = POST_, FULL = FULL_;
+    static constexpr int GATE = GATE_;
+    static constexpr int SLOTS = !FAST ? kInCount : 3 + (POST || GATE) + (GATE == 2);       // operands in a stage of the ring
+};
 
-// POST: sums for the post norm's weight and bias; BIAS: sums for biases; GATE: sums for a gate row shared by rows.
-template <int THREADS, int T, int E, int VEC, bool POST, bool BIAS, bool GATE>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS)
+template <int THREADS, int T, int E, int VEC, typename F>
+__global__ void __launch_bounds__(THREADS)
 residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
-    extern __shared__ __align__(16) float staged[];      // [2][kInCount][E][THREADS]
-    __shared__ TeamSlots<THREADS, 3, float> sh;
-    constexpr int STAGE = E * THREADS;
+    extern __shared__ __align__(16) float staged[];      // [stages][SLOTS][E][THREADS]
+    constexpr bool FAST = F::FAST, POST = F::POST, FULL = F::FULL, GATE = F::GATE == 1 || !FAST;
+    constexpr int SUMS = POST ? (FULL ? 8 : 4) : (FULL ? 2 : 1);
+    __shared__ TeamSlots<THREADS, SUMS, float> sh;
+    __shared__ TeamSlots<THREADS, 1, float> sh_gate;
+    constexpr int SLOT = E * THREADS;
+    constexpr int TEAMS = THREADS / T;
     const ResidualNormGeom& g = a.g;
     const int tid = threadIdx.x % T;
     const uint32_t rank = cs > 1 ? cluster_rank() : 0;
-    const int64_t team = (int64_t)(blockIdx.x / cs) * (THREADS / T) + threadIdx.x / T;
-    if (team >= a.teams) return;                         // whole teams leave together; never in a cluster
-    const int64_t lo = g.rows * team / a.teams, hi = g.rows * (team + 1) / a.teams;
+    const int64_t team = (int64_t)(blockIdx.x / cs) * TEAMS + threadIdx.x / T;
+    const bool present = team < a.teams;
+    const int64_t lo = present ? g.rows * team / a.teams : 0, hi = present ? g.rows * (team + 1) / a.teams : 0;
     const int64_t slice = cs > 1 ? ((g.cols + cs - 1) / cs + 3) / 4 * 4 : g.cols;
     const int64_t begin = slice * rank;
     const int width = (int)(begin >= g.cols ? 0 : (g.cols - begin < slice ? g.cols - begin : slice));
     const float inv = (float)g.inv_cols;
-    int turn = 0;
+    int turn = 0, gate_turn = 0;
 
-    float pre_w[E], pre_b[BIAS ? E : 1], post_w[POST ? E : 1], post_b[POST && BIAS ? E : 1], gate_sum[GATE ? E : 1];
+    float pre_w[E], pre_b[FULL ? E : 1], post_w[POST ? E : 1], post_b[POST && FULL ? E : 1], gate_sum[GATE ? E : 1];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         pre_w[e] = 0.0f;
-        if (BIAS) pre_b[e] = 0.0f;
+        if (FULL) pre_b[e] = 0.0f;
         if (POST) post_w[e] = 0.0f;
-        if (POST && BIAS) post_b[e] = 0.0f;
+        if (POST && FULL) post_b[e] = 0.0f;
         if (GATE) gate_sum[e] = 0.0f;
     }
     float scalar_gate_sum = 0.0f;
-    const bool shared_gate = GATE && a.shared_gate;
-    const bool scalar_gate = g.gate_mode == kGateScalar && a.out.gate;
-    const bool want_n = g.gate_mode != kGateNone && a.out.gate;
+    const bool pre = FAST || g.pre_kind != CTB_NORM_NONE, post = FAST ? POST : g.post_kind != CTB_NORM_NONE;
+    const bool has_dy = FAST || a.in[kInDy].p, has_f = FAST ? POST || F::GATE != 0 : a.in[kInF].p != nullptr;
+    const bool pre_weight = FAST || g.pre_weight, post_weight = FAST ? POST : g.post_weight != nullptr;
+    const bool row_gate = FAST ? F::GATE != 0 : g.gate_mode == kGateRow, staged_gate = FAST ? F::GATE == 2 : a.in[kInGate].p != nullptr;
+    const bool want_n = FAST ? F::GATE != 0 : g.gate_mode != kGateNone && a.out.gate;
+    const bool shared_gate = FAST ? F::GATE == 1 : a.shared_gate != 0;
+    const bool scalar_gate = !FAST && g.gate_mode == kGateScalar && a.out.gate;
 
-    auto fetch = [&](int64_t row, int which) {
+    // the thread's place in each operand's next row to fetch, and in its own stage slots
+    const float* next[kInCount];
 #pragma unroll
-        for (int q = 0; q < kInCount; ++q) {
-            if (!a.in[q].p) continue;
-            const float* src = a.in[q].p + row * a.in[q].stride + begin;
-            float* dst = staged + (which * kInCount + q) * STAGE;
+    for (int q = 0; q < kInCount; ++q) next[q] = a.in[q].p + lo * a.in[q].stride + begin + tid * VEC;
+    float* const mine = staged + threadIdx.x * VEC;
+    int64_t fetched = lo;
+    auto fetch = [&](int stage_at) {                     // always commits, so that groups count rows
+        if (fetched < hi) {
 #pragma unroll
-            for (int i = 0; i < E / VEC; ++i) {
-                const int c = col_of<T, VEC>(i, tid);
-                if (c < width) copy_async<VEC * 4>(dst + (i * THREADS + threadIdx.x) * VEC, src + c);
+            for (int q = 0; q < F::SLOTS; ++q) {
+                constexpr int kinds[kInCount] = {kInY, kInDh, kInDy, kInF, kInGate};
+                const int op = kinds[q];
+                if (!FAST && !a.in[op].p) continue;
+#pragma unroll
+                for (int i = 0; i < E / VEC; ++i)
+                    if (col_of<T, VEC>(i, tid) < width) copy_async<VEC * 4>(mine + stage_at + q * SLOT + i * THREADS * VEC, next[op] + i * T * VEC);
+                next[op] += a.in[op].stride;
             }
         }
+        ++fetched;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const float4* stats = reinterpret_cast<const float4*>(a.stats);
+    constexpr int STAGE = F::SLOTS * SLOT;
+    const int ring = a.stages * STAGE;
+    for (int s = 0; s + 1 < a.stages; ++s) fetch(s * STAGE);
+    int64_t group = fast_div((uint32_t)lo, g.by_gate_rows);
+    int64_t left = (group + 1) * g.gate_rows - lo;       // rows of this gate row that are still to come
+    const float4* stats = reinterpret_cast<const float4*>(a.stats) + lo;
     float4 next_st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
-    if (lo < hi) {
-        fetch(lo, 0);
-        next_st = stats[lo];
-    }
-    for (int64_t row = lo; row < hi; ++row) {
-        const int which = (int)((row - lo) & 1);
+    if (lo < hi) next_st = *stats;
+    int stage_at = 0, ahead_at = (a.stages - 1) * STAGE;
+    int64_t out_at = lo * g.cols + begin + tid * VEC;
+    for (int64_t row = lo; row < hi; ++row, out_at += g.cols) {
         const float4 st = next_st;
-        if (row + 1 < hi) {
-            fetch(row + 1, which ^ 1);
-            next_st = stats[row + 1];
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-        } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-        }
-        const float* in = staged + which * (kInCount * STAGE);
-        float dx[E];                                     // first a = dh * w, then the gradient of y and x
-        float hat[E];
-        float m1 = 0.0f, m2 = 0.0f;
-        if (g.pre_kind != CTB_NORM_NONE) {
-            float s[3] = {0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < E / VEC; ++i) {
-                const int c = col_of<T, VEC>(i, tid);
-                float yv[VEC], dh[VEC], w[VEC];
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) { yv[k] = st.z; dh[k] = 0.0f; w[k] = 1.0f; }
-                if (c < width) {
-                    read_staged<E, VEC>(yv, in + kInY * STAGE, THREADS, i);
-                    read_staged<E, VEC>(dh, in + kInDh * STAGE, THREADS, i);
-                    if (g.pre_weight) load_part<T, VEC>(w, g.pre_weight + begin, c);
-                }
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const int e = i * VEC + k;
-                    hat[e] = (yv[k] - st.z) * st.w;
-                    pre_w[e] = fmaf(dh[k], hat[e], pre_w[e]);
-                    if (BIAS) pre_b[e] = pre_b[e] + dh[k];
-                    dx[e] = dh[k] * w[k];
-                    s[0] = s[0] + dx[e];
-                    s[1] = fmaf(dx[e], hat[e], s[1]);
-                }
-            }
-            team_fold<FoldSum, THREADS, T>(s, sh, turn, cs);
-            m1 = g.pre_kind == CTB_NORM_LAYER ? s[0] * inv : 0.0f;
-            m2 = s[1] * inv;
-        }
-        const int64_t group = g.gate_mode == kGateNone ? 0 : row / g.gate_rows;
-        const float* gate = g.gate.p + group * g.gate.stride;
-        const float one_gate = g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
-        float s[3] = {0.0f, 0.0f, 0.0f};
+        fetch(ahead_at);                                 // into the place of the row before this one, which is done with
+        if (row + 1 < hi) next_st = *++stats;
+        if (a.stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        else if (a.stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else asm volatile("cp.async.wait_group 1;" ::: "memory");
+        const float* in = mine + stage_at;
+        stage_at = stage_at + STAGE == ring ? 0 : stage_at + STAGE;
+        ahead_at = ahead_at + STAGE == ring ? 0 : ahead_at + STAGE;
+        const float* gate = g.gate.p + group * g.gate.stride + (row_gate ? begin : 0);
+        const float one_gate = !FAST && g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
+        const float mean_f = FULL ? st.x : 0.0f, mean_y = FULL ? st.z : 0.0f;
+
+        float e_[E], hat[E];                             // e = dy + rstd_y * a, and yhat
+        // sums of a yhat, k e fhat, k fhat yhat; and of a, k e, k, k fhat, k yhat
+        float s_ay = 0.0f, s_kef = 0.0f, s_kfy = 0.0f, s_a = 0.0f, s_ke = 0.0f, s_k = 0.0f, s_kf = 0.0f, s_ky = 0.0f;
 #pragma unroll
         for (int i = 0; i < E / VEC; ++i) {
             const int c = col_of<T, VEC>(i, tid);
+            const float* at = in + i * THREADS * VEC;
             if (c < width) {
-                float dy[VEC], fv[VEC], part[VEC], w[VEC];
+                float dy[VEC], fv[VEC], k[VEC], w[VEC];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) dy[k] = 0.0f;
-                if (a.in[kInDy].p) read_staged<E, VEC>(dy, in + kInDy * STAGE, THREADS, i);
+                for (int q = 0; q < VEC; ++q) dy[q] = 0.0f;
+                if (has_dy) read_own<VEC>(dy, at + kInDy * SLOT);
+                if (pre) {
+                    float yv[VEC], dh[VEC];
+                    read_own<VEC>(yv, at + kInY * SLOT);
+                    read_own<VEC>(dh, at + kInDh * SLOT);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const int e = i * VEC + k;
-                    part[k] = dy[k];
-                    if (g.pre_kind != CTB_NORM_NONE) part[k] = fmaf(st.w, dx[e] - m1 - hat[e] * m2, dy[k]);
+                    for (int q = 0; q < VEC; ++q) w[q] = 1.0f;
+                    if (pre_weight) load_part<T, VEC>(w, g.pre_weight + begin, c);
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) {
+                        const int e = i * VEC + q;
+                        hat[e] = FULL ? (yv[q] - mean_y) * st.w : yv[q] * st.w;
+                        pre_w[e] = fmaf(dh[q], hat[e], pre_w[e]);
+                        if (FULL) pre_b[e] = pre_b[e] + dh[q];
+                        const float av = dh[q] * w[q];
+                        if (FULL) s_a = s_a + av;
+                        s_ay = fmaf(av, hat[e], s_ay);
+                        e_[e] = fmaf(st.w, av, dy[q]);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) { hat[i * VEC + q] = 0.0f; e_[i * VEC + q] = dy[q]; }
                 }
-                if (a.out.x) store_part<VEC>(a.out.x + row * g.cols + begin, c, part);
+                if (post) {
+                    read_own<VEC>(fv, at + kInF * SLOT);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) { fv[k] = 0.0f; w[k] = 1.0f; }
-                if (a.in[kInF].p) read_staged<E, VEC>(fv, in + kInF * STAGE, THREADS, i);
-                // fhat, and n where the gate's gradient wants it
-                if (POST && g.post_kind != CTB_NORM_NONE) {
+                    for (int q = 0; q < VEC; ++q) k[q] = one_gate;
+                    if (row_gate) {
+                        float gv[VEC];
+                        if (staged_gate) read_own<VEC>(gv, at + kInGate * SLOT);
+                        else load_part<T, VEC>(gv, gate, c);
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) fv[k] = (fv[k] - st.x) * st.y;
-                    if (g.post_weight) load_part<T, VEC>(w, g.post_weight + begin, c);
+                        for (int q = 0; q < VEC; ++q) k[q] = gv[q] * g.scale;
+                    }
+                    if (post_weight) {
+                        load_part<T, VEC>(w, g.post_weight + begin, c);
+#pragma unroll
+                        for (int q = 0; q < VEC; ++q) k[q] = k[q] * w[q];
+                    }
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) {
+                        const int e = i * VEC + q;
+                        const float fh = FULL ? (fv[q] - mean_f) * st.y : fv[q] * st.y, ke = k[q] * e_[e], kf = k[q] * fh;
+                        s_kef = fmaf(ke, fh, s_kef);
+                        s_kfy = fmaf(kf, hat[e], s_kfy);
+                        if (FULL) {
+                            s_ke = s_ke + ke;
+                            s_k = s_k + k[q];
+                            s_kf = s_kf + kf;
+                            s_ky = fmaf(k[q], hat[e], s_ky);
+                        }
+                    }
                 }
-                float gv[VEC];
+            } else {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) gv[k] = one_gate;
-                if (g.gate_mode == kGateRow) {
-                    float q[VEC];
-                    if (a.in[kInGate].p) read_staged<E, VEC>(q, in + kInGate * STAGE, THREADS, i);
-                    else load_part<T, VEC>(q, gate + begin, c);
+                for (int q = 0; q < VEC; ++q) { hat[i * VEC + q] = 0.0f; e_[i * VEC + q] = 0.0f; }
+            }
+        }
+        if (POST || pre) {
+            float v[SUMS];
+            v[0] = s_ay;
+            if constexpr (SUMS == 2) v[1] = s_a;
+            if constexpr (SUMS >= 4) { v[1] = s_kef; v[2] = s_kfy; v[3] = s_a; }
+            if constexpr (SUMS == 8) { v[4] = s_ke; v[5] = s_k; v[6] = s_kf; v[7] = s_ky; }
+            team_fold<FoldSum, THREADS, T>(v, sh, turn, cs);
+            s_ay = v[0];
+            if constexpr (SUMS == 2) s_a = v[1];
+            if constexpr (SUMS >= 4) { s_kef = v[1]; s_kfy = v[2]; s_a = v[3]; }
+            if constexpr (SUMS == 8) { s_ke = v[4]; s_k = v[5]; s_kf = v[6]; s_ky = v[7]; }
+        }
+        // dx = e - b0 - yhat * b1;  df = rstd_f * (k dx - c0 - fhat * c1)
+        const float b0 = FULL && g.pre_kind == CTB_NORM_LAYER ? st.w * (s_a * inv) : 0.0f, b1 = st.w * (s_ay * inv);
+        const float c0 = FULL && g.post_kind == CTB_NORM_LAYER ? (s_ke - (b0 * s_k + b1 * s_ky)) * inv : 0.0f;
+        const float c1 = (s_kef - (b0 * s_kf + b1 * s_kfy)) * inv;
+        float scalar_sum = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) gv[k] = q[k] * g.scale;
+        for (int i = 0; i < E / VEC; ++i) {
+            const int c = col_of<T, VEC>(i, tid);
+            const float* at = in + i * THREADS * VEC;
+            const int64_t out = out_at + i * T * VEC;
+            if (c < width) {
+                float dx[VEC], fv[VEC], w[VEC], gv[VEC];
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) {
+                    const int e = i * VEC + q;
+                    dx[q] = pre ? e_[e] - fmaf(hat[e], b1, b0) : e_[e];
+                    fv[q] = 0.0f;
+                    w[q] = 1.0f;
+                    gv[q] = one_gate;
+                }
+                if (FAST || a.out.x) store_part<VEC>(a.out.x, out, dx);
+                if (has_f) read_own<VEC>(fv, at + kInF * SLOT);
+                if (post) {
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) fv[q] = FULL ? (fv[q] - mean_f) * st.y : fv[q] * st.y;
+                    if (post_weight) load_part<T, VEC>(w, g.post_weight + begin, c);
+                }
+                if (row_gate) {
+                    if (staged_gate) read_own<VEC>(gv, at + kInGate * SLOT);
+                    else load_part<T, VEC>(gv, gate, c);
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) gv[q] = gv[q] * g.scale;
                 }
                 if (want_n) {
-                    float b[VEC], n[VEC];
+                    float n[VEC];
+                    if (FULL && post && g.post_bias) {
+                        float b[VEC];
+                        load_part<T, VEC>(b, g.post_bias + begin, c);
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) b[k] = 0.0f;
-                    if (POST && g.post_bias) load_part<T, VEC>(b, g.post_bias + begin, c);
+                        for (int q = 0; q < VEC; ++q) n[q] = fmaf(fv[q], w[q], b[q]) * (g.scale * dx[q]);
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) n[k] = fmaf(fv[k], w[k], b[k]) * (g.scale * part[k]);
-                    if (g.gate_mode == kGateScalar) {
+                        for (int q = 0; q < VEC; ++q) n[q] = (post ? fv[q] * w[q] : fv[q]) * (g.scale * dx[q]);
+                    }
+                    if (scalar_gate) {
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) s[2] = s[2] + n[k];
+                        for (int q = 0; q < VEC; ++q) scalar_sum = scalar_sum + n[q];
                     } else if (shared_gate) {
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) gate_sum[GATE ? i * VEC + k : 0] += n[k];
+                        for (int q = 0; q < VEC; ++q) gate_sum[GATE ? i * VEC + q : 0] += n[q];
                     } else {
-                        store_part<VEC>(a.out.gate + row * g.cols + begin, c, n);
+                        store_part<VEC>(a.out.gate, out, n);
                     }
                 }
+                float df[VEC];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const int e = i * VEC + k;
-                    const float dn = part[k] * gv[k];
+                for (int q = 0; q < VEC; ++q) {
+                    const int e = i * VEC + q;
+                    const float dn = dx[q] * gv[q];
                     if (POST) {
-                        post_w[e] = fmaf(dn, fv[k], post_w[e]);
-                        if (BIAS) post_b[e] = post_b[e] + dn;
+                        post_w[e] = fmaf(dn, fv[q], post_w[e]);
+                        if (FULL) post_b[e] = post_b[e] + dn;
                     }
-                    dx[e] = dn * w[k];                   // from here on: c = dn * w_post
-                    hat[e] = fv[k];
-                    if (POST) {
-                        s[0] = s[0] + dx[e];
-                        s[1] = fmaf(dx[e], fv[k], s[1]);
-                    }
+                    df[q] = post ? st.y * (dn * w[q] - fmaf(fv[q], c1, c0)) : dn;
                 }
+                if (FAST || a.out.f) store_part<VEC>(a.out.f, out, df);
             }
         }
-        if ((POST && g.post_kind != CTB_NORM_NONE) || scalar_gate) team_fold<FoldSum, THREADS, T>(s, sh, turn, cs);
-        if (a.out.f) {
-            const float c1 = POST && g.post_kind == CTB_NORM_LAYER ? s[0] * inv : 0.0f, c2 = s[1] * inv;
-#pragma unroll
-            for (int i = 0; i < E / VEC; ++i) {
-                const int c = col_of<T, VEC>(i, tid);
-                if (c < width) {
-                    float part[VEC];
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) {
-                        const int e = i * VEC + k;
-                        part[k] = POST && g.post_kind != CTB_NORM_NONE ? st.y * (dx[e] - c1 - hat[e] * c2) : dx[e];
-                    }
-                    store_part<VEC>(a.out.f + row * g.cols + begin, c, part);
-                }
-            }
+        if (scalar_gate) {
+            float one[1] = {scalar_sum};
+            team_fold<FoldSum, THREADS, T>(one, sh_gate, gate_turn, cs);
+            scalar_gate_sum = scalar_gate_sum + one[0];
         }
         // a gate that rows share: its sum so far goes out when the next row belongs to another gate row
-        if (scalar_gate || shared_gate) {
-            scalar_gate_sum = scalar_gate_sum + s[2];
-            if (row + 1 == hi || (row + 1) / g.gate_rows != group) {
-                if (shared_gate) {
+        if (--left == 0 || row + 1 == hi) {
+            if (shared_gate && !a.one_gate_row) {
 #pragma unroll
-                    for (int i = 0; i < E / VEC; ++i) {
-                        const int c = col_of<T, VEC>(i, tid);
-                        float part[VEC];
+                for (int i = 0; i < E / VEC; ++i) {
+                    const int c = col_of<T, VEC>(i, tid);
+                    float part[VEC];
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) {
-                            part[k] = gate_sum[GATE ? i * VEC + k : 0];
-                            gate_sum[GATE ? i * VEC + k : 0] = 0.0f;
-                        }
-                        if (c < width) store_part<VEC>(a.gate_part + (team + group) * g.cols + begin, c, part);
+                    for (int q = 0; q < VEC; ++q) {
+                        part[q] = gate_sum[GATE ? i * VEC + q : 0];
+                        gate_sum[GATE ? i * VEC + q : 0] = 0.0f;
                     }
-                } else if (tid == 0 && rank == 0) {
-                    a.gate_part[team + group] = scalar_gate_sum;
+                    if (c < width) store_part<VEC>(a.gate_part + (team + group) * g.cols + begin, c, part);
                 }
-                scalar_gate_sum = 0.0f;
+            } else if (scalar_gate && tid == 0 && rank == 0) {
+                a.gate_part[team + group] = scalar_gate_sum;
             }
+            scalar_gate_sum = 0.0f;
+            ++group;
+            left = g.gate_rows;
         }
     }
-    // column sums of the team
+    // column sums: the teams of a CTA add theirs in team order (through the ring, which is done with)
     auto put = [&](int at, const float* sum) {
-        float* part_row = a.part + ((int64_t)at * a.teams + team) * g.cols + begin;
+        if (TEAMS > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e) staged[e * THREADS + threadIdx.x] = sum[e];
+            __syncthreads();
+        }
+        if (threadIdx.x >= T) return;
+        float* part_row = a.part + ((int64_t)at * a.parts + blockIdx.x / cs) * g.cols + begin;
 #pragma unroll
         for (int i = 0; i < E / VEC; ++i) {
             const int c = col_of<T, VEC>(i, tid);
             float part[VEC];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) part[k] = sum[i * VEC + k];
+            for (int q = 0; q < VEC; ++q) {
+                part[q] = sum[i * VEC + q];
+#pragma unroll
+                for (int t = 1; t < TEAMS; ++t) part[q] = part[q] + staged[(i * VEC + q) * THREADS + t * T + tid];
+            }
             if (c < width) store_part<VEC>(part_row, c, part);
         }
     };
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (a.out.pre_weight) put(0, pre_w);
-    if (BIAS && a.out.pre_bias) put(1, pre_b);
+    if (FULL && a.out.pre_bias) put(1, pre_b);
     if (POST && a.out.post_weight) put(2, post_w);
-    if (POST && BIAS && a.out.post_bias) put(3, post_b);
+    if (POST && FULL && a.out.post_bias) put(3, post_b);
+    if (GATE && a.one_gate_row) put(4, gate_sum);
 }
 
-// out[c] = sum over partial rows [first, last] of part[row][c], added in row order within eight runs that
-// are joined in order, in fp64.  Jobs: the weight vectors, then one for every gate group.
+// out[c] = sum over partial rows [first, last] of part[row][c], in fp64: runs of consecutive rows, joined in
+// order.  Jobs: the vectors, then one for every gate group.
 struct FoldJobs {
-    const float* part[4];
-    float* out[4];
+    const float* part[5];
+    float* out[5];
     int32_t vectors;
-    int64_t teams, cols;
+    int64_t parts, teams, cols;
     const float* gate_part;
     float* gate;
     int64_t groups, gate_width, gate_rows, rows;
     int64_t vector_blocks, tiles, gate_tiles;
 };
 
-constexpr int kFoldCols = 32, kFoldRuns = 8;
+constexpr int kFoldThreads = 512, kFoldCols = 32, kFoldBatch = 8;
 
-__global__ void __launch_bounds__(kFoldCols * kFoldRuns)
+__global__ void __launch_bounds__(kFoldThreads)
 residual_norm_fold_kernel(const __grid_constant__ FoldJobs j) {
-    __shared__ double sums[kFoldRuns][kFoldCols];
+    __shared__ double sums[kFoldThreads];
     const float* part;
     float* out;
-    int64_t first = 0, last = j.teams - 1, width = j.cols, tile;
+    int64_t first = 0, last = j.parts - 1, width = j.cols, tile;
     const int64_t b = blockIdx.x;
     if (b < j.vector_blocks) {
         const int v = (int)(b / j.tiles);
@@ -485,29 +602,36 @@ residual_norm_fold_kernel(const __grid_constant__ FoldJobs j) {
         part = j.gate_part;
         out = j.gate + group * width;
     }
-    const int64_t c = tile * kFoldCols + threadIdx.x;
-    const int64_t run = (last - first + kFoldRuns) / kFoldRuns;
+    const int across = width == 1 ? 1 : kFoldCols, runs = kFoldThreads / across;
+    const int64_t c = tile * kFoldCols + threadIdx.x % across;
+    const int which = threadIdx.x / across;
+    const int64_t run = (last - first + runs) / runs;
+    const int64_t lo = first + which * run, hi = min(last + 1, lo + run);
     double sum = 0.0;
-    if (c < width)
-        for (int64_t r = first + threadIdx.y * run; r < first + (threadIdx.y + 1) * run && r <= last; ++r) sum = sum + (double)part[r * width + c];
-    sums[threadIdx.y][threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.y == 0 && c < width) {
+    if (c < width) {
+        for (int64_t r = lo; r < hi; r += kFoldBatch) {
+            float v[kFoldBatch];
 #pragma unroll
-        for (int i = 1; i < kFoldRuns; ++i) sum = sum + sums[i][threadIdx.x];
-        out[c] = (float)sum;
+            for (int u = 0; u < kFoldBatch; ++u) v[u] = r + u < hi ? part[(r + u) * width + c] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < kFoldBatch; ++u) sum = sum + (double)v[u];
+        }
     }
+    sums[threadIdx.x] = sum;
+    for (int half = runs / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (which < half) sums[threadIdx.x] = sums[threadIdx.x] + sums[threadIdx.x + half * across];
+    }
+    if (which == 0 && c < width) out[c] = (float)sums[threadIdx.x];
 }
 
 // ---- host -----------------------------------------------------------------------------------------------
 bool rows_aligned(const RowsIn& r) { return !r.p || (is_aligned(r.p, 16) && r.stride % 4 == 0); }
 
-// CTAs of a cluster for `cols` columns when one CTA holds `per_cta`.
+// CTAs of a cluster for `cols` columns when one CTA holds `per_cta` (slices are multiples of four columns).
 int cluster_for(int64_t cols, int64_t per_cta) {
-    int cs = 1;
-    while ((int64_t)cs * per_cta < cols) cs *= 2;
-    // slices are rounded up to four columns
-    if (cs > 1 && ((cols + cs - 1) / cs + 3) / 4 * 4 > per_cta) cs *= 2;
+    int cs = (int)ceil_div(cols, per_cta);
+    if (cs > 1 && (ceil_div(cols, (int64_t)cs) + 3) / 4 * 4 > per_cta) ++cs;
     return cs;
 }
 
@@ -518,47 +642,90 @@ int forward_as(const ResidualNormGeom& g, RowsIn x, RowsIn f, float* y, float* h
                            g, x, f, y, h, stats, cs);
 }
 
-template <int THREADS, int T, int E, int VEC, bool POST, bool BIAS, bool GATE>
-int backward_as(const ResidualBwd& a, int cs, cudaStream_t st) {
-    return launch_clusters("residual_norm", residual_norm_backward_kernel<THREADS, T, E, VEC, POST, BIAS, GATE>, ceil_div(a.teams, (int64_t)(THREADS / T)) * cs,
-                           THREADS, (size_t)2 * kInCount * E * THREADS * sizeof(float), cs, st, a, cs);
+// How a row is dealt out in the backward pass: a team of `team` threads with `share` columns each, `threads` to a
+// CTA, `cs` CTAs to a row.  One CTA of about 500 threads per SM: that many hold the column sums of their rows in
+// registers.  Up to 2048 columns it has several teams, so that one works while another waits in its fold;
+// a wider row keeps the SM busy by itself (the next ones are on their way into shared memory).  Twice the columns
+// per thread halve what a thread does once per row; with LayerNorms or biases the sums of 16 columns
+// would not fit the registers.
+struct BwdShape {
+    int threads, team, share, cs;
+};
+BwdShape bwd_shape(int64_t cols, bool wide) {
+    for (const BwdShape& s : {BwdShape{512, 32, 8, 1}, BwdShape{512, 64, 8, 1}, BwdShape{480, 96, 8, 1}, BwdShape{512, 128, 8, 1}, BwdShape{384, 192, 8, 1}, BwdShape{512, 256, 8, 1}})
+        if (cols <= s.team * s.share) return s;
+    if (wide) return {320, 320, 16, cluster_for(cols, 320 * 16)};
+    return {512, 512, 8, cluster_for(cols, 512 * 8)};
 }
-
-constexpr int kBwdShare = 8;                             // columns per thread
-
-template <int THREADS, int T>
-int backward_select(const ResidualBwd& a, bool vec, bool post, bool bias, bool gate, int cs, cudaStream_t st) {
-    // rows that cannot be read in 16-byte vectors: one instantiation with every sum
-    if (!vec) return backward_as<THREADS, T, kBwdShare, 1, true, true, true>(a, cs, st);
-    if (post) {
-        if (bias) return gate ? backward_as<THREADS, T, kBwdShare, 4, true, true, true>(a, cs, st) : backward_as<THREADS, T, kBwdShare, 4, true, true, false>(a, cs, st);
-        return gate ? backward_as<THREADS, T, kBwdShare, 4, true, false, true>(a, cs, st) : backward_as<THREADS, T, kBwdShare, 4, true, false, false>(a, cs, st);
-    }
-    if (bias) return gate ? backward_as<THREADS, T, kBwdShare, 4, false, true, true>(a, cs, st) : backward_as<THREADS, T, kBwdShare, 4, false, true, false>(a, cs, st);
-    return gate ? backward_as<THREADS, T, kBwdShare, 4, false, false, true>(a, cs, st) : backward_as<THREADS, T, kBwdShare, 4, false, false, false>(a, cs, st);
-}
-
-int bwd_team_threads(int64_t cols) { return cols <= 32 * kBwdShare ? 32 : cols <= 128 * kBwdShare ? 128 : cols <= 256 * kBwdShare ? 256 : 512; }
-// Teams that walk the rows: as many as the machine holds at once (512 threads per SM), at most one per row.
-int64_t bwd_teams(int64_t rows, int64_t cols, int sm_count) {
-    const int t = bwd_team_threads(cols);
-    int64_t teams = (int64_t)sm_count * (512 / t) / cluster_for(cols, (int64_t)t * kBwdShare);
-    if (teams > rows) teams = rows;
-    return teams < 1 ? 1 : teams;
+// Teams that walk the rows, at most one per row: `ctas` CTAs (clusters) run at once.
+int64_t bwd_teams(int64_t rows, const BwdShape& s, int64_t ctas) {
+    const int64_t teams = ctas * (s.threads / s.team);
+    return teams > rows ? rows : (teams < 1 ? 1 : teams);
 }
 constexpr int kMaxSms = 256;                             // what the size query, which names no device, allows for
+
+struct BwdCall {
+    ResidualBwd a;
+    BwdShape shape;
+    bool vec, fast, post, full;
+    int gate;                           // of BwdFlags
+    int sm_count;
+    void* workspace;
+    cudaStream_t st;
+};
+
+template <int THREADS, int T, int E, int VEC, typename F>
+int backward_as(BwdCall& c) {
+    auto kernel = residual_norm_backward_kernel<THREADS, T, E, VEC, F>;
+    ResidualBwd& a = c.a;
+    const int cs = c.shape.cs;
+    const size_t stage = (size_t)F::SLOTS * E * THREADS * sizeof(float), room = (size_t)216 * 1024;
+    a.stages = stage * 4 <= room ? 4 : (stage * 3 <= room ? 3 : 2);
+    int ctas = c.sm_count < kMaxSms ? c.sm_count : kMaxSms;
+    if (cs > 1) {                       // a second wave of a few clusters would double the time
+        int most = 0;
+        if (int rc = resident_clusters((const void*)kernel, THREADS, stage * a.stages, cs, &most)) return rc;
+        ctas = most < ctas / cs ? most : ctas / cs;
+    }
+    a.teams = bwd_teams(a.g.rows, c.shape, ctas);
+    a.parts = ceil_div(a.teams, (int64_t)(THREADS / T));
+    a.part = (float*)c.workspace;
+    a.gate_part = a.part + 5 * a.parts * a.g.cols;
+    return launch_clusters("residual_norm_backward", kernel, a.parts * cs, THREADS, stage * a.stages, cs, c.st, a, cs);
+}
+
+template <int THREADS, int T, int E, bool POST, bool FULL>
+int backward_gate(BwdCall& c) {
+    if (c.gate == 0) return backward_as<THREADS, T, E, 4, BwdFlags<true, POST, FULL, 0>>(c);
+    if (c.gate == 1) return backward_as<THREADS, T, E, 4, BwdFlags<true, POST, FULL, 1>>(c);
+    return backward_as<THREADS, T, E, 4, BwdFlags<true, POST, FULL, 2>>(c);
+}
+template <int THREADS, int T>
+int backward_narrow(BwdCall& c) {
+    // rows that cannot be read in 16-byte vectors, and calls without some operand or result
+    if (!c.vec) return backward_as<THREADS, T, 8, 1, BwdFlags<false, true, true, 1>>(c);
+    if (!c.fast) return backward_as<THREADS, T, 8, 4, BwdFlags<false, true, true, 1>>(c);
+    if (c.post) return c.full ? backward_gate<THREADS, T, 8, true, true>(c) : backward_gate<THREADS, T, 8, true, false>(c);
+    return c.full ? backward_gate<THREADS, T, 8, false, true>(c) : backward_gate<THREADS, T, 8, false, false>(c);
+}
 
 }  // namespace
 
 size_t residual_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_groups, int64_t gate_width) {
-    const int64_t teams = bwd_teams(rows, cols, kMaxSms);
-    return ((size_t)(4 * teams) * (size_t)cols + (size_t)(gate_groups > 0 ? teams + gate_groups : 0) * (size_t)gate_width) * sizeof(float);
+    int64_t teams = 0, parts = 0;
+    for (const BwdShape& shape : {bwd_shape(cols, true), bwd_shape(cols, false)}) {
+        const int64_t t = bwd_teams(rows, shape, kMaxSms), p = ceil_div(t, (int64_t)(shape.threads / shape.team));
+        teams = t > teams ? t : teams;
+        parts = p > parts ? p : parts;
+    }
+    return ((size_t)(5 * parts) * (size_t)cols + (size_t)(gate_groups > 0 ? teams + gate_groups : 0) * (size_t)gate_width) * sizeof(float);
 }
 
 int launch_residual_norm(const ResidualNormGeom& geom, RowsIn x, RowsIn f, float* y, float* h, float* stats, cudaStream_t st) {
     if (geom.rows == 0 || geom.cols == 0) return CTB_OK;
     ResidualNormGeom g = geom;
     g.inv_cols = 1.0 / (double)g.cols;
+    g.by_gate_rows = make_fastdiv((uint32_t)g.gate_rows);
     const bool vec = g.cols % 4 == 0 && rows_aligned(x) && rows_aligned(f) && (!y || is_aligned(y, 16)) && (!h || is_aligned(h, 16)) &&
                      is_aligned(g.post_weight, 16) && is_aligned(g.post_bias, 16) && is_aligned(g.pre_weight, 16) && is_aligned(g.pre_bias, 16) &&
                      (g.gate_mode != kGateRow || rows_aligned(g.gate));
@@ -582,9 +749,11 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     if (g.rows == 0 || g.cols == 0) return CTB_OK;
     DeviceInfo di;
     if (int rc = current_device_info(&di)) return rc;
-    ResidualBwd a{};
+    BwdCall call{};
+    ResidualBwd& a = call.a;
     a.g = g;
     a.g.inv_cols = 1.0 / (double)g.cols;
+    a.g.by_gate_rows = make_fastdiv((uint32_t)g.gate_rows);
     const bool want_gate = out.gate && g.gate_mode != kGateNone;
     const bool post = g.post_kind != CTB_NORM_NONE;
     const bool shared_gate = want_gate && g.gate_mode == kGateRow && g.gate_rows > 1;
@@ -595,34 +764,51 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     a.stats = stats;
     a.out = out;
     a.shared_gate = shared_gate;
-    a.teams = bwd_teams(g.rows, g.cols, di.sm_count < kMaxSms ? di.sm_count : kMaxSms);
-    a.part = (float*)workspace;
-    a.gate_part = a.part + 4 * a.teams * g.cols;
+    a.one_gate_row = shared_gate && groups == 1;
     bool vec = g.cols % 4 == 0 && (!out.x || is_aligned(out.x, 16)) && (!out.f || is_aligned(out.f, 16)) && (!out.gate || is_aligned(out.gate, 16)) &&
                is_aligned(g.post_weight, 16) && is_aligned(g.post_bias, 16) && is_aligned(g.pre_weight, 16) &&
                (g.gate_mode != kGateRow || rows_aligned(g.gate));
     for (const RowsIn& r : a.in) vec = vec && rows_aligned(r);
-    const int t = bwd_team_threads(g.cols), cs = cluster_for(g.cols, (int64_t)t * kBwdShare);
-    const bool bias = out.pre_bias || out.post_bias;
+    call.vec = vec;
+    call.post = post;
+    call.fast = g.pre_kind != CTB_NORM_NONE && g.pre_weight && out.pre_weight && grad_y.p && f.p && out.x && out.f &&
+                (!post || (g.post_weight && out.post_weight)) && (g.gate_mode == kGateNone || (g.gate_mode == kGateRow && out.gate));
+    call.full = g.pre_kind == CTB_NORM_LAYER || g.post_kind == CTB_NORM_LAYER || out.pre_bias || out.post_bias || g.post_bias;
+    call.gate = g.gate_mode == kGateNone ? 0 : (shared_gate ? 1 : 2);
+    call.shape = bwd_shape(g.cols, vec && call.fast && !call.full);
+    call.sm_count = di.sm_count;
+    call.workspace = workspace;
+    call.st = st;
     int rc;
-    if (t == 32) rc = backward_select<256, 32>(a, vec, post, bias, shared_gate, cs, st);
-    else if (t == 128) rc = backward_select<256, 128>(a, vec, post, bias, shared_gate, cs, st);
-    else if (t == 256) rc = backward_select<256, 256>(a, vec, post, bias, shared_gate, cs, st);
-    else rc = backward_select<512, 512>(a, vec, post, bias, shared_gate, cs, st);
+    switch (call.shape.team) {
+    case 32: rc = backward_narrow<512, 32>(call); break;
+    case 64: rc = backward_narrow<512, 64>(call); break;
+    case 96: rc = backward_narrow<480, 96>(call); break;
+    case 128: rc = backward_narrow<512, 128>(call); break;
+    case 192: rc = backward_narrow<384, 192>(call); break;
+    case 256: rc = backward_narrow<512, 256>(call); break;
+    case 320: rc = post ? backward_gate<320, 320, 16, true, false>(call) : backward_gate<320, 320, 16, false, false>(call); break;
+    default: rc = backward_narrow<512, 512>(call);
+    }
     if (rc) return rc;
 
     FoldJobs j{};
     float* const sums[4] = {out.pre_weight, out.pre_bias, out.post_weight, out.post_bias};
     for (int v = 0; v < 4; ++v)
         if (sums[v]) {
-            j.part[j.vectors] = a.part + (int64_t)v * a.teams * g.cols;
+            j.part[j.vectors] = a.part + (int64_t)v * a.parts * g.cols;
             j.out[j.vectors++] = sums[v];
         }
+    if (a.one_gate_row) {
+        j.part[j.vectors] = a.part + 4 * a.parts * g.cols;
+        j.out[j.vectors++] = out.gate;
+    }
+    j.parts = a.parts;
     j.teams = a.teams;
     j.cols = g.cols;
     j.tiles = ceil_div(g.cols, kFoldCols);
     j.vector_blocks = j.vectors * j.tiles;
-    const bool fold_gate = want_gate && (g.gate_mode == kGateScalar || g.gate_rows > 1);
+    const bool fold_gate = want_gate && !a.one_gate_row && (g.gate_mode == kGateScalar || g.gate_rows > 1);
     if (fold_gate) {
         j.gate_part = a.gate_part;
         j.gate = out.gate;
@@ -635,7 +821,7 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     const int64_t blocks = j.vector_blocks + (fold_gate ? groups * j.gate_tiles : 0);
     if (blocks == 0) return CTB_OK;
     if (blocks > 0x7FFFFFFFll) return set_error(CTB_ERR_LIMIT, "residual_norm_backward: too many gate rows for one launch");
-    residual_norm_fold_kernel<<<(unsigned)blocks, dim3(kFoldCols, kFoldRuns), 0, st>>>(j);
+    residual_norm_fold_kernel<<<(unsigned)blocks, kFoldThreads, 0, st>>>(j);
     return cuda_error(cudaGetLastError(), "residual_norm_backward launch");
 }
 

@@ -15,7 +15,7 @@ struct RowsIn {
 enum { kGateNone = 0, kGateRow = 1, kGateScalar = 2 };
 
 struct ResidualNormGeom {
-    int64_t rows;
+    int64_t rows;                       // < 2^31
     int64_t cols;                       // <= kResidualNormMaxCols
     int32_t post_kind, pre_kind;        // CTB_NORM_*
     float post_eps, pre_eps, scale;
@@ -23,7 +23,8 @@ struct ResidualNormGeom {
     int32_t gate_mode;
     int64_t gate_rows;                  // rows that share a gate row / value
     RowsIn gate;                        // stride: between one gate row / value and the next
-    double inv_cols;                    // set by the launchers
+    double inv_cols;                    // these two are set by the launchers
+    FastDiv by_gate_rows;
 };
 constexpr int64_t kResidualNormMaxCols = 32768;
 

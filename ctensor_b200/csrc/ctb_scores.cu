@@ -67,18 +67,39 @@ __device__ __forceinline__ const float* score_row(const ScoreRows& r, const Scor
 // c0 .. c0 + 3, of which some may lie outside the row.
 __device__ __forceinline__ int score_phase(const float* row) { return (int)(((uintptr_t)row >> 2) & 3); }
 
+// The document numbers of a sequence's keys.  `fours`: contiguous, and the row's fours are 16-byte aligned.
+struct ScoreDocs {
+    const int32_t* p;
+    int64_t si;
+    bool fours;
+};
+template <bool DOCS>
+__device__ __forceinline__ ScoreDocs score_docs(const ScoreArgs& a, const ScorePlace& w, int phase) {
+    ScoreDocs d{nullptr, 0, false};
+    if (DOCS) {
+        d.p = a.g.key_docs.p + w.b * a.g.key_docs.sb;
+        d.si = a.g.key_docs.si;
+        d.fours = d.si == 1 && (int)(((uintptr_t)d.p >> 2) & 3) == phase;
+    }
+    return d;
+}
+
 // The admitted ones of the columns c0 .. c0 + 3, as bits.
 template <bool DOCS>
-__device__ __forceinline__ uint32_t score_admitted(const ScoreArgs& a, const ScorePlace& w, int c0) {
+__device__ __forceinline__ uint32_t score_admitted(const ScoreDocs& docs, const ScorePlace& w, int c0) {
     uint32_t bits = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) bits |= (uint32_t)(c0 + k >= 0 && c0 + k < w.live) << k;
     if (DOCS && bits) {
-        const int32_t* docs = a.g.key_docs.p + w.b * a.g.key_docs.sb;
+        if (docs.fours && bits == 15u) {
+            const int4 d = *reinterpret_cast<const int4*>(docs.p + c0);
+            bits = (uint32_t)(d.x == w.doc) | (uint32_t)(d.y == w.doc) << 1 | (uint32_t)(d.z == w.doc) << 2 | (uint32_t)(d.w == w.doc) << 3;
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if ((bits >> k) & 1u)
-                if (docs[(int64_t)(c0 + k) * a.g.key_docs.si] != w.doc) bits &= ~(1u << k);
+            for (int k = 0; k < 4; ++k)
+                if ((bits >> k) & 1u)
+                    if (docs.p[(int64_t)(c0 + k) * docs.si] != w.doc) bits &= ~(1u << k);
+        }
     }
     return bits;
 }
@@ -107,6 +128,17 @@ __device__ __forceinline__ void score_store(float* row, int c0, int keys, const 
     }
 }
 
+// Zeros into the fours without an admitted key, ahead of the loads: these stores need not wait for them.
+template <int T, int NV>
+__device__ __forceinline__ void score_zeros(float* out, int phase, int keys, int tid, uint32_t bits) {
+    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1                                         // unrolled, its addresses double the kernel's registers
+    for (int v = 0; v < NV; ++v) {
+        const int c0 = (v * T + tid) * 4 - phase;
+        if (!((bits >> (4 * v)) & 15u) && c0 < keys) score_store(out, c0, keys, zero);
+    }
+}
+
 // t of one column.  The bias is taken from the key nearest to the query, which changes no probability
 // (a softmax does not see a constant) and keeps t small where the query is far from every key.
 template <bool CAP>
@@ -130,11 +162,13 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
     const float* s = score_row(a.s, w);
     const int phase = score_phase(out);
     const bool aligned = score_phase(s) == phase;
+    const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     int turn = 0;
     float t[NV][4];
     uint32_t bits = 0;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(a, w, (v * T + tid) * 4 - phase) << (4 * v);
+    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, (v * T + tid) * 4 - phase) << (4 * v);
+    score_zeros<T, NV>(out, phase, keys, tid, bits);
 #pragma unroll
     for (int v = 0; v < NV; ++v) score_load(t[v], s, (v * T + tid) * 4 - phase, (bits >> (4 * v)) & 15u, aligned);
     float m[1] = {-INFINITY};
@@ -168,7 +202,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int c0 = (v * T + tid) * 4 - phase;
-        if (c0 < keys) {
+        if ((bits >> (4 * v)) & 15u) {
             float p[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) p[k] = (bits >> (4 * v + k)) & 1u ? t[v][k] * inv : 0.0f;
@@ -192,11 +226,13 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
     const int phase = score_phase(out);
     const bool p_aligned = score_phase(pr) == phase, g_aligned = score_phase(gr) == phase, s_aligned = CAP && score_phase(sr) == phase;
+    const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     int turn = 0;
     float p[NV][4], dp[NV][4], s[CAP ? NV : 1][4];
     uint32_t bits = 0;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(a, w, (v * T + tid) * 4 - phase) << (4 * v);
+    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, (v * T + tid) * 4 - phase) << (4 * v);
+    score_zeros<T, NV>(out, phase, keys, tid, bits);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int c0 = (v * T + tid) * 4 - phase;
@@ -216,7 +252,7 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int c0 = (v * T + tid) * 4 - phase;
-        if (c0 < keys) {
+        if ((bits >> (4 * v)) & 15u) {
             float r[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -262,6 +298,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     const float* s = score_row(a.s, w);
     const int phase = score_phase(out);
     const bool aligned = score_phase(s) == phase;
+    const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
     int turn = 0;
@@ -273,7 +310,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
-            bits[u] = at < live_end ? score_admitted<DOCS>(a, w, (int)(at * 4) - phase) : 0u;
+            bits[u] = at < live_end ? score_admitted<DOCS>(docs, w, (int)(at * 4) - phase) : 0u;
         }
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
@@ -310,7 +347,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
-            bits[u] = at < live_end ? score_admitted<DOCS>(a, w, (int)(at * 4) - phase) : 0u;
+            bits[u] = at < live_end ? score_admitted<DOCS>(docs, w, (int)(at * 4) - phase) : 0u;
         }
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
@@ -340,6 +377,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
     const int phase = score_phase(out);
     const bool p_aligned = score_phase(pr) == phase, g_aligned = score_phase(gr) == phase, s_aligned = CAP && score_phase(sr) == phase;
+    const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
     int turn = 0;
@@ -350,7 +388,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
             const int c0 = (int)(at * 4) - phase;
-            const uint32_t bits = at < live_end ? score_admitted<DOCS>(a, w, c0) : 0u;
+            const uint32_t bits = at < live_end ? score_admitted<DOCS>(docs, w, c0) : 0u;
             score_load(p[u], pr, c0, bits, p_aligned);
             score_load(dp[u], gr, c0, bits, g_aligned);
         }
@@ -369,7 +407,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
             const int c0 = (int)(at * 4) - phase;
-            bits[u] = at < live_end ? score_admitted<DOCS>(a, w, c0) : 0u;
+            bits[u] = at < live_end ? score_admitted<DOCS>(docs, w, c0) : 0u;
             score_load(p[u], pr, c0, bits[u], p_aligned);
             score_load(dp[u], gr, c0, bits[u], g_aligned);
             if (CAP) score_load(s[u], sr, c0, bits[u], s_aligned);
@@ -466,7 +504,8 @@ int launch_scores(ScoreArgs& a, bool backward, cudaStream_t st) {
     if (n <= 128) return rows_as<256, 32, 1>(a, backward, cap, docs, st);
     if (n <= 256) return rows_as<256, 32, 2>(a, backward, cap, docs, st);
     if (n <= 512) return rows_as<256, 32, 4>(a, backward, cap, docs, st);
-    if (n <= 1024) return rows_as<256, 32, 8>(a, backward, cap, docs, st);
+    if (n <= 1024) return backward ? rows_as<256, 64, 4>(a, backward, cap, docs, st) : rows_as<256, 32, 8>(a, backward, cap, docs, st);
+
     if (n <= 2048) return rows_as<256, 128, 4>(a, backward, cap, docs, st);
     if (n <= 4096) return rows_as<256, 256, 4>(a, backward, cap, docs, st);
     if (n <= 8192) return rows_as<512, 512, 4>(a, backward, cap, docs, st);

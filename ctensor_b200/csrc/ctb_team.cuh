@@ -27,41 +27,63 @@ __device__ __forceinline__ void store_peer(uint32_t at, double v) { asm volatile
 
 struct FoldSum {
     template <typename S> static __device__ __forceinline__ S of(S a, S b) { return a + b; }
+    static __device__ __forceinline__ float none() { return 0.0f; }
 };
 struct FoldMax {      // like fmaxf, ignores a NaN
     static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+    static __device__ __forceinline__ float none() { return -INFINITY; }
 };
 
 // Two sets of slots used in turn: a slot is written again only after every reader has passed the barrier
-// of the fold in between.  (One object serves folds of different kinds as long as all of them use `turn`.)
+// of the fold in between.
 template <int THREADS, int N, typename S>
 struct TeamSlots {
     S warps[2][THREADS / 32][N];
     S peers[2][kMaxCluster][N];
 };
 
-// Folds N values over a team of T threads of a CTA of THREADS, and over the `cs` CTAs of a cluster when
-// cs > 1 (a team is then a whole CTA).  Every thread of the team calls it.
+// v[n] = fold over i < count of p[i * N + n], in every lane: lane l reads the entries l, l + 32, ... (all of
+// the same n = l % N), the lanes of equal n join theirs, and lane n passes the result on.
+template <typename OP, int N, typename S>
+__device__ __forceinline__ void lane_fold(S (&v)[N], const S* p, int count) {
+    const int lane = threadIdx.x & 31;
+    S x = (S)OP::none();
+    for (int i = lane; i < count * N; i += 32) x = OP::of(x, p[i]);
+#pragma unroll
+    for (int off = N; off < 32; off <<= 1) x = OP::of(x, __shfl_xor_sync(0xffffffffu, x, off));
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, x, n);
+}
+
+// Folds N (a power of two) values over a team of T threads of a CTA of THREADS, and over the `cs` CTAs of
+// a cluster when cs > 1 (a team is then a whole CTA).  Every thread of the team calls it and gets the same
+// bits.  Within a warp the values are folded in halves — a lane passes on half of its values, then half of
+// the rest — so that eight sums cost 9 shuffles instead of 40; lane l then holds value l / (32 / N).
 template <typename OP, int THREADS, int T, int N, typename S>
 __device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& sh, int& turn, int cs) {
+    const int lane = threadIdx.x & 31;
+    int off = 16;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+    for (int have = N; have > 1; have >>= 1, off >>= 1) {
+        const bool upper = lane & off;
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) v[n] = OP::of(v[n], __shfl_xor_sync(0xffffffffu, v[n], off));
-    if (T == 32) return;
+        for (int n = 0; n < have / 2; ++n) {
+            const S give = upper ? v[n] : v[n + have / 2], keep = upper ? v[n + have / 2] : v[n];
+            v[n] = OP::of(keep, __shfl_xor_sync(0xffffffffu, give, off));
+        }
+    }
+#pragma unroll
+    for (int rest = 16 / N; rest > 0; rest >>= 1) v[0] = OP::of(v[0], __shfl_xor_sync(0xffffffffu, v[0], rest));
+    if (T == 32) {
+        const S mine = v[0];
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, mine, n * (32 / N));
+        return;
+    }
     const int warp = threadIdx.x >> 5, team = threadIdx.x / T;
-    if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) sh.warps[turn][warp][n] = v[n];
-    }
+    if (lane % (32 / N) == 0) sh.warps[turn][warp][lane / (32 / N)] = v[0];
     asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(T) : "memory");
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        S r = sh.warps[turn][team * (T / 32)][n];
-#pragma unroll
-        for (int i = 1; i < T / 32; ++i) r = OP::of(r, sh.warps[turn][team * (T / 32) + i][n]);
-        v[n] = r;
-    }
+    lane_fold<OP, N>(v, &sh.warps[turn][team * (T / 32)][0], T / 32);
     if (cs > 1) {
         if ((int)threadIdx.x < cs) {
             const uint32_t at = peer_shared(&sh.peers[turn][cluster_rank()][0], threadIdx.x);
@@ -70,15 +92,13 @@ __device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& s
         }
         __syncwarp();
         cluster_barrier();
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            S r = sh.peers[turn][0][n];
-            for (int i = 1; i < cs; ++i) r = OP::of(r, sh.peers[turn][i][n]);
-            v[n] = r;
-        }
+        lane_fold<OP, N>(v, &sh.peers[turn][0][0], cs);
     }
     turn ^= 1;
 }
+
+// How many clusters of `cs` CTAs of this kernel the current device runs at once.
+int resident_clusters(const void* kernel, int threads, size_t smem, int cs, int* count);
 
 // One-dimensional launch, in clusters of `cs` CTAs when cs > 1.
 template <typename... Params, typename... Args>
