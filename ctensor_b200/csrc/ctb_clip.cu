@@ -12,6 +12,7 @@
 // Bound by HBM: 4 bytes per Float32 element for the norm and 8 more where the gradients have to be
 // scaled.  Squares and sums are fp64: a square of an fp32 value neither overflows nor vanishes there.
 #include "ctb_clip.cuh"
+#include "ctb_team.cuh"
 
 namespace ctb {
 
@@ -21,7 +22,7 @@ constexpr int kClipThreads = 256;
 constexpr int kClipLoads = 4;                            // 32-byte loads in flight per thread
 constexpr int kClipVecBytes = 32;
 constexpr int kClipChunkBytes = kClipThreads * kClipLoads * kClipVecBytes;      // 32 KiB
-constexpr int kClipBlocksPerSm = 4;
+constexpr int kClipBlocksPerSm = 6;
 constexpr int kClipMaxBlocks = 1024;                     // partials of one launch
 constexpr int kClipSmallTable = 128, kClipLargeTable = 1024;
 
@@ -82,7 +83,7 @@ template <int N> __device__ __forceinline__ int clip_tensor_of(const ClipTable<N
 }
 
 template <int KIND, typename T, int N>
-__global__ void __launch_bounds__(kClipThreads)
+__global__ void __launch_bounds__(kClipThreads, kClipBlocksPerSm)
 clip_norm_kernel(const __grid_constant__ ClipTable<N> t, double* __restrict__ partials) {
     constexpr int VEC = ClipVec<T>::kElems;
     using V = Vec<T, VEC>;
@@ -125,6 +126,7 @@ clip_norm_kernel(const __grid_constant__ ClipTable<N> t, double* __restrict__ pa
             }
         }
     }
+    let_next_start();
     double sum = acc[0];
 #pragma unroll
     for (int k = 1; k < VEC; ++k) sum = clip_fold<KIND>(sum, acc[k]);
@@ -148,6 +150,7 @@ template <int KIND>
 __global__ void __launch_bounds__(kClipThreads)
 clip_finish_kernel(const double* __restrict__ partials, int count, void* norm, int norm_dtype) {
     __shared__ double smem[kClipThreads / 32];
+    wait_for_previous();
     const double total = clip_total<KIND>(partials, count, smem);
     if (threadIdx.x == 0) clip_store_norm(total, norm, norm_dtype);
 }
@@ -161,6 +164,7 @@ clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const double* __restri
     constexpr int CHUNK = kClipChunkBytes / (int)sizeof(T);
     using V = Vec<T, VEC>;
     __shared__ double smem[kClipThreads / 32];
+    wait_for_previous();
     const double total = clip_total<KIND>(partials, count, smem);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) clip_store_norm(total, norm, norm_dtype);
     const bool clipped = total > max_norm && total < INFINITY;
@@ -259,8 +263,10 @@ int clip_launch_table(int phase, const ClipTensor* list, int64_t count, ClipCall
         clip_norm_kernel<KIND, T, N><<<grid, kClipThreads, 0, call.st>>>(table, call.partials + call.total_partials);
         call.total_partials += (int)grid;
     } else {
-        clip_scale_kernel<KIND, T, N><<<grid, kClipThreads, 0, call.st>>>(table, call.partials, call.total_partials, call.max_norm, call.norm, call.norm_dtype);
+        // (a second scaling launch may start early too: it waits for the first, which waited for the norm)
+        const int rc = launch_early(clip_scale_kernel<KIND, T, N>, grid, kClipThreads, call.st, table, call.partials, call.total_partials, call.max_norm, call.norm, call.norm_dtype);
         call.norm = nullptr;                                // written once
+        return rc;
     }
     return cuda_error(cudaGetLastError(), "clip_grad_norm launch");
 }
@@ -286,8 +292,7 @@ int clip_run(const ClipTensor* t32, int64_t n32, const ClipTensor* t64, int64_t 
         if ((rc = clip_phase<KIND, double>(1, t64, n64, call))) return rc;
     }
     if (call.norm) {                                        // no scaling launch wrote it
-        clip_finish_kernel<KIND><<<1, kClipThreads, 0, call.st>>>(call.partials, call.total_partials, call.norm, call.norm_dtype);
-        return cuda_error(cudaGetLastError(), "grad_norm launch");
+        return launch_early(clip_finish_kernel<KIND>, 1, kClipThreads, call.st, call.partials, call.total_partials, call.norm, call.norm_dtype);
     }
     return CTB_OK;
 }

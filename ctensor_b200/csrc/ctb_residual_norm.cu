@@ -347,6 +347,16 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
         const float4 st = next_st;
         fetch(ahead_at);                                 // into the place of the row before this one, which is done with
         if (row + 1 < hi) next_st = *++stats;
+        float w_pre[E];                                  // ahead of the wait for the row
+#pragma unroll
+        for (int i = 0; i < E / VEC; ++i) {
+            float w[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) w[q] = 1.0f;
+            if (pre_weight && col_of<T, VEC>(i, tid) < width) load_part<T, VEC>(w, g.pre_weight + begin, col_of<T, VEC>(i, tid));
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) w_pre[i * VEC + q] = w[q];
+        }
         if (a.stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
         else if (a.stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
         else asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -374,15 +384,12 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                     read_own<VEC>(yv, at + kInY * SLOT);
                     read_own<VEC>(dh, at + kInDh * SLOT);
 #pragma unroll
-                    for (int q = 0; q < VEC; ++q) w[q] = 1.0f;
-                    if (pre_weight) load_part<T, VEC>(w, g.pre_weight + begin, c);
-#pragma unroll
                     for (int q = 0; q < VEC; ++q) {
                         const int e = i * VEC + q;
                         hat[e] = FULL ? (yv[q] - mean_y) * st.w : yv[q] * st.w;
                         pre_w[e] = fmaf(dh[q], hat[e], pre_w[e]);
                         if (FULL) pre_b[e] = pre_b[e] + dh[q];
-                        const float av = dh[q] * w[q];
+                        const float av = dh[q] * w_pre[e];
                         if (FULL) s_a = s_a + av;
                         s_ay = fmaf(av, hat[e], s_ay);
                         e_[e] = fmaf(st.w, av, dy[q]);
@@ -557,6 +564,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
         }
     };
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    let_next_start();
     if (a.out.pre_weight) put(0, pre_w);
     if (FULL && a.out.pre_bias) put(1, pre_b);
     if (POST && a.out.post_weight) put(2, post_w);
@@ -608,6 +616,7 @@ residual_norm_fold_kernel(const __grid_constant__ FoldJobs j) {
     const int64_t run = (last - first + runs) / runs;
     const int64_t lo = first + which * run, hi = min(last + 1, lo + run);
     double sum = 0.0;
+    wait_for_previous();
     if (c < width) {
         for (int64_t r = lo; r < hi; r += kFoldBatch) {
             float v[kFoldBatch];
@@ -654,7 +663,7 @@ struct BwdShape {
 BwdShape bwd_shape(int64_t cols, bool wide) {
     for (const BwdShape& s : {BwdShape{512, 32, 8, 1}, BwdShape{512, 64, 8, 1}, BwdShape{480, 96, 8, 1}, BwdShape{512, 128, 8, 1}, BwdShape{384, 192, 8, 1}, BwdShape{512, 256, 8, 1}})
         if (cols <= s.team * s.share) return s;
-    if (wide) return {320, 320, 16, cluster_for(cols, 320 * 16)};
+    if (wide) return {640, 640, 8, cluster_for(cols, 640 * 8)};
     return {512, 512, 8, cluster_for(cols, 512 * 8)};
 }
 // Teams that walk the rows, at most one per row: `ctas` CTAs (clusters) run at once.
@@ -736,7 +745,8 @@ int launch_residual_norm(const ResidualNormGeom& geom, RowsIn x, RowsIn f, float
     }
     if (g.cols <= 256) return forward_as<256, 32, 8, 4>(g, x, f, y, h, stats, st);
     if (g.cols <= 512) return forward_as<256, 32, 16, 4>(g, x, f, y, h, stats, st);
-    if (g.cols <= 1024) return forward_as<256, 32, 32, 4>(g, x, f, y, h, stats, st);
+    if (g.cols <= 768) return forward_as<288, 96, 8, 4>(g, x, f, y, h, stats, st);
+    if (g.cols <= 1024) return forward_as<256, 128, 8, 4>(g, x, f, y, h, stats, st);
     if (g.cols <= 2048) return forward_as<256, 128, 16, 4>(g, x, f, y, h, stats, st);
     if (g.cols <= 4096) return forward_as<256, 256, 16, 4>(g, x, f, y, h, stats, st);
     return forward_as<512, 512, 16, 4>(g, x, f, y, h, stats, st);
@@ -787,7 +797,7 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     case 128: rc = backward_narrow<512, 128>(call); break;
     case 192: rc = backward_narrow<384, 192>(call); break;
     case 256: rc = backward_narrow<512, 256>(call); break;
-    case 320: rc = post ? backward_gate<320, 320, 16, true, false>(call) : backward_gate<320, 320, 16, false, false>(call); break;
+    case 640: rc = post ? backward_gate<640, 640, 8, true, false>(call) : backward_gate<640, 640, 8, false, false>(call); break;
     default: rc = backward_narrow<512, 512>(call);
     }
     if (rc) return rc;
@@ -821,8 +831,7 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     const int64_t blocks = j.vector_blocks + (fold_gate ? groups * j.gate_tiles : 0);
     if (blocks == 0) return CTB_OK;
     if (blocks > 0x7FFFFFFFll) return set_error(CTB_ERR_LIMIT, "residual_norm_backward: too many gate rows for one launch");
-    residual_norm_fold_kernel<<<(unsigned)blocks, kFoldThreads, 0, st>>>(j);
-    return cuda_error(cudaGetLastError(), "residual_norm_backward launch");
+    return launch_early(residual_norm_fold_kernel, (unsigned)blocks, kFoldThreads, st, j);
 }
 
 }  // namespace ctb

@@ -448,6 +448,7 @@ score_slope_fold_kernel(const double* __restrict__ part, int64_t batch, int64_t 
     __shared__ TeamSlots<256, 1, double> sh;
     const int64_t h = blockIdx.x;
     double sum[1] = {0.0};
+    wait_for_previous();
     for (int64_t b = 0; b < batch; ++b)
         for (int64_t i = threadIdx.x; i < queries; i += 256) sum[0] = sum[0] + part[(b * heads + h) * queries + i];
     int turn = 0;
@@ -537,8 +538,7 @@ int launch_score_softmax_backward(const ScoreGeom& g, ScoreRows grad, ScoreRows 
         CTB_CUDA_TRY(cudaMemsetAsync(grad_slopes, 0, (size_t)g.heads * sizeof(float), st));
         return CTB_OK;
     }
-    score_slope_fold_kernel<<<(unsigned)g.heads, 256, 0, st>>>(partials, g.batch, g.heads, g.queries, grad_slopes);
-    return cuda_error(cudaGetLastError(), "score_softmax_backward launch");
+    return launch_early(score_slope_fold_kernel, (unsigned)g.heads, 256, st, partials, g.batch, g.heads, g.queries, grad_slopes);
 }
 
 }  // namespace ctb

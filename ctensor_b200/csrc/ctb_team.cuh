@@ -100,6 +100,27 @@ __device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& s
 // How many clusters of `cs` CTAs of this kernel the current device runs at once.
 int resident_clusters(const void* kernel, int threads, size_t smem, int cs, int* count);
 
+// A kernel that was launched with `early` may start before the one ahead of it in the stream has ended; it
+// calls wait_for_previous() before it touches what that one writes.  The one ahead calls let_next_start() when
+// it has little left to do.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+int launch_early(void (*kernel)(Params...), unsigned blocks, int threads, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CTB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
+    return CTB_OK;
+}
+
 // One-dimensional launch, in clusters of `cs` CTAs when cs > 1.
 template <typename... Params, typename... Args>
 int launch_clusters(const char* who, void (*kernel)(Params...), int64_t blocks, int threads, size_t smem, int cs, cudaStream_t st, Args... args) {
