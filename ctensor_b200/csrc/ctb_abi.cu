@@ -1410,7 +1410,7 @@ int score_operand(const ctb_view* v, const char* null_msg, const char* who, cons
     if (like && !same_shape(v, like)) return set_error(CTB_ERR_SHAPE, "%s: shapes differ", who);
     if (v->shape[3] > 1 && v->stride[3] != 1) return set_error(CTB_ERR_SHAPE, "%s: the keys must be contiguous", who);
     if ((rc = check_element_alignment(v, who))) return rc;
-    *out = {(const float*)elem_ptr(v), v->stride[0], v->stride[1], v->stride[2]};
+    *out = {(const float*)elem_ptr(v), v->stride[0], v->stride[1], v->stride[2], -1};
     return CTB_OK;
 }
 
@@ -1667,7 +1667,7 @@ int ctb_score_softmax_backward(const ctb_view* grad, const ctb_view* probs, cons
                                void* stream) {
     const char* who = "score_softmax_backward";
     int rc;
-    ScoreRows pr, dp, s{nullptr, 0, 0, 0};
+    ScoreRows pr, dp, s{nullptr, 0, 0, 0, -1};
     ScoreGeom g;
     if ((rc = score_operand(probs, "score_softmax: null input", who, nullptr, &pr))) return rc;
     if ((rc = score_operand(grad, "backward: null gradient", who, probs, &dp))) return rc;

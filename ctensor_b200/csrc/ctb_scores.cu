@@ -29,42 +29,50 @@ struct ScoreArgs {
 
 // Where a row is and what its query may look at.
 struct ScorePlace {
-    int64_t b, h, i;
+    uint32_t row, b, h, i;
     int live;                           // keys [0, live) may be admitted
     int centre;                         // the key position nearest to the query's within [0, live)
     float beyond;                       // |pos - centre|
     float slope;
     int doc;
 };
-__device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, int64_t row) {
+__device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, uint32_t row) {
     const ScoreGeom& g = a.g;
+    const int keys = (int)g.keys;
     ScorePlace w;
-    const uint32_t bh = fast_div((uint32_t)row, a.by_queries);
-    w.i = (uint32_t)row - bh * a.by_queries.d;
+    const uint32_t bh = fast_div(row, a.by_queries);
+    w.row = row;
+    w.i = row - bh * a.by_queries.d;
     w.b = fast_div(bh, a.by_heads);
-    w.h = bh - (uint32_t)w.b * a.by_heads.d;
-    const int64_t pos = (g.query_start.p ? (int64_t)g.query_start.p[w.b * g.query_start.sb] : g.keys - g.queries) + w.i;
-    int64_t live = g.keys;
-    if (g.key_lengths.p) live = min(live, (int64_t)g.key_lengths.p[w.b * g.key_lengths.sb]);
+    w.h = bh - w.b * a.by_heads.d;
+    int64_t pos = (g.query_start.p ? (int64_t)g.query_start.p[w.b * g.query_start.sb] : g.keys - g.queries) + w.i;
+    w.live = keys;
+    if (g.key_lengths.p) w.live = min(keys, g.key_lengths.p[w.b * g.key_lengths.sb]);
     if (g.causal) {
-        int64_t reach = pos + 1;
-        if (g.prefix.p) reach = max(reach, (int64_t)g.prefix.p[w.b * g.prefix.sb]);
-        live = min(live, reach);
+        int reach = (int)max(min(pos + 1, (int64_t)keys), (int64_t)0);
+        if (g.prefix.p) reach = max(reach, g.prefix.p[w.b * g.prefix.sb]);
+        w.live = min(w.live, reach);
     }
-    live = max(live, (int64_t)0);
-    const int64_t centre = max(min(pos, live - 1), (int64_t)0);
-    w.live = (int)live;
-    w.centre = (int)centre;
-    w.beyond = (float)(pos > centre ? pos - centre : centre - pos);
-    w.slope = g.slopes ? g.slopes[w.h * g.slope_stride] : 0.0f;
+    w.live = max(w.live, 0);
+    w.centre = 0;
+    w.beyond = w.slope = 0.0f;
+    if (g.slopes) {
+        w.centre = (int)max(min(pos, (int64_t)w.live - 1), (int64_t)0);
+        w.beyond = (float)(pos > w.centre ? pos - w.centre : w.centre - pos);
+        w.slope = g.slopes[w.h * g.slope_stride];
+    }
     w.doc = g.query_docs.p ? g.query_docs.p[w.b * g.query_docs.sb + w.i * g.query_docs.si] : 0;
     return w;
 }
-__device__ __forceinline__ const float* score_row(const ScoreRows& r, const ScorePlace& w) { return r.p + w.b * r.sb + w.h * r.sh + w.i * r.sq; }
+__device__ __forceinline__ const float* score_row(const ScoreRows& r, const ScorePlace& w) {
+    if (r.even >= 0) return r.p + (int64_t)w.row * r.even;
+    return r.p + w.b * r.sb + w.h * r.sh + w.i * r.sq;
+}
 
 // Rows start at any multiple of four bytes.  Columns are dealt out in fours counted from the output row's
 // address rounded down to 16 bytes, so whole fours of the output are aligned; a four holds the columns
-// c0 .. c0 + 3, of which some may lie outside the row.
+// c0 .. c0 + 3, of which some may lie outside the row.  ALIGNED: every row of every operand starts on 16 bytes
+// and has whole fours only (a four with an admitted column may then be read whole).
 __device__ __forceinline__ int score_phase(const float* row) { return (int)(((uintptr_t)row >> 2) & 3); }
 
 // The document numbers of a sequence's keys.  `fours`: contiguous, and the row's fours are 16-byte aligned.
@@ -87,9 +95,8 @@ __device__ __forceinline__ ScoreDocs score_docs(const ScoreArgs& a, const ScoreP
 // The admitted ones of the columns c0 .. c0 + 3, as bits.
 template <bool DOCS>
 __device__ __forceinline__ uint32_t score_admitted(const ScoreDocs& docs, const ScorePlace& w, int c0) {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) bits |= (uint32_t)(c0 + k >= 0 && c0 + k < w.live) << k;
+    const int hi = min(max(w.live - c0, 0), 4), lo = min(max(-c0, 0), 4);
+    uint32_t bits = (15u >> (4 - hi)) & (15u << lo);
     if (DOCS && bits) {
         if (docs.fours && bits == 15u) {
             const int4 d = *reinterpret_cast<const int4*>(docs.p + c0);
@@ -115,12 +122,15 @@ __device__ __forceinline__ void score_load(float (&v)[4], const float* row, int 
         for (int k = 0; k < 4; ++k) v[k] = (bits >> k) & 1u ? row[c0 + k] : 0.0f;
     }
 }
+__device__ __forceinline__ void score_store_four(float* at, const float (&v)[4]) {
+    Vec<float, 4> q;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q.v[k] = v[k];
+    stg_stream(reinterpret_cast<Vec<float, 4>*>(at), q);
+}
 __device__ __forceinline__ void score_store(float* row, int c0, int keys, const float (&v)[4]) {
     if (c0 >= 0 && c0 + 4 <= keys) {
-        Vec<float, 4> q;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q.v[k] = v[k];
-        stg_stream(reinterpret_cast<Vec<float, 4>*>(row + c0), q);
+        score_store_four(row + c0, v);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -128,27 +138,89 @@ __device__ __forceinline__ void score_store(float* row, int c0, int keys, const 
     }
 }
 
-// Zeros into the fours without an admitted key, ahead of the loads: these stores need not wait for them.
-template <int T, int NV>
-__device__ __forceinline__ void score_zeros(float* out, int phase, int keys, int tid, uint32_t bits) {
-    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1                                         // unrolled, its addresses double the kernel's registers
-    for (int v = 0; v < NV; ++v) {
-        const int c0 = (v * T + tid) * 4 - phase;
-        if (!((bits >> (4 * v)) & 15u) && c0 < keys) score_store(out, c0, keys, zero);
+// e^x = 2^(x log2 e).  x is a difference of logits (were the logits themselves kept in units of log 2, a row of
+// the type's lowest values would overflow).  The instruction's relative error is below 2^-22, results below
+// 2^-126 are 0.
+__device__ __forceinline__ float score_exp(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
+// t of a four's columns.  The bias is taken from the key nearest to the query, which changes no probability
+// (a softmax does not see a constant) and keeps t small where the query is far from every key.
+template <bool CAP>
+__device__ __forceinline__ void score_logits(const ScoreGeom& g, const ScorePlace& w, float (&t)[4], int c0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = CAP ? g.cap * tanhf(t[k] * g.over_cap) : t[k] * g.scale;
+    if (g.slopes) {
+        const float from = (float)(c0 - w.centre);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = fmaf(-w.slope, fabsf(from + (float)k), t[k]);
+    }
+}
+template <bool CAP>
+__device__ __forceinline__ void score_slow(const ScoreGeom& g, float (&r)[4], const float* s) {     // r *= scale * (1 - tanh^2)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        r[k] = r[k] * g.scale;
+        if (CAP) {
+            const float th = tanhf(s[k] * g.over_cap);
+            r[k] = r[k] * fmaf(-th, th, 1.0f);
+        }
     }
 }
 
-// t of one column.  The bias is taken from the key nearest to the query, which changes no probability
-// (a softmax does not see a constant) and keeps t small where the query is far from every key.
-template <bool CAP>
-__device__ __forceinline__ float score_logit(const ScoreGeom& g, const ScorePlace& w, float s, int col) {
-    float t = CAP ? g.cap * tanhf(s * g.over_cap) : s * g.scale;
-    if (g.slopes) t = fmaf(-w.slope, (float)abs(col - w.centre), t);
-    return t;
-}
+// A thread's fours of a row: four v has the columns (v * T + tid) * 4 - phase and on.  Which columns are
+// admitted is a comparison with `live` where rows are aligned and no documents are given, else kept as bits.
+template <int T, int NV, bool DOCS, bool ALIGNED>
+struct ScoreShare {
+    static constexpr bool kBits = DOCS || !ALIGNED;
+    int first;                          // column of the first four
+    int rest;                           // admissible columns from there on
+    uint32_t bits;
+    __device__ __forceinline__ void init(const ScoreDocs& docs, const ScorePlace& w, int tid, int phase) {
+        first = tid * 4 - phase;
+        rest = w.live - first;
+        bits = 0;
+        if (kBits) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, column(v)) << (4 * v);
+        }
+    }
+    __device__ __forceinline__ int column(int v) const { return first + v * T * 4; }
+    __device__ __forceinline__ bool any(int v) const { return kBits ? ((bits >> (4 * v)) & 15u) != 0 : rest > v * T * 4; }
+    __device__ __forceinline__ bool has(int v, int k) const { return kBits ? ((bits >> (4 * v + k)) & 1u) != 0 : rest > v * T * 4 + k; }
+    // values of the fours that have an admitted column; others keep what they held
+    __device__ __forceinline__ void load(float (&x)[NV][4], const float* row, bool aligned) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (ALIGNED) {
+                if (any(v)) {
+                    const Vec<float, 4> q = ldg_stream(reinterpret_cast<const Vec<float, 4>*>(row + column(v)));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[v][k] = q.v[k];
+                }
+            } else {
+                score_load(x[v], row, column(v), (bits >> (4 * v)) & 15u, aligned);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* out, int v, int keys, const float (&x)[4]) const {
+        if (ALIGNED) score_store_four(out + column(v), x);
+        else score_store(out, column(v), keys, x);
+    }
+    // Zeros into the fours without an admitted key, ahead of the loads: these stores need not wait for them.
+    __device__ __forceinline__ void zeros(float* out, int keys) const {
+        const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1                                         // unrolled, its addresses double the kernel's registers
+        for (int v = 0; v < NV; ++v) {
+            const int c0 = column(v);
+            if (!any(v) && c0 < keys) store(out, v, keys, zero);
+        }
+    }
+};
 
-template <int THREADS, int T, int NV, bool CAP, bool DOCS>
+template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS)
 score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
     static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
@@ -156,29 +228,25 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
     const int tid = threadIdx.x % T;
     const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
     if (row >= a.rows) return;                           // whole teams leave together
-    const ScorePlace w = score_place(a, row);
+    const ScorePlace w = score_place(a, (uint32_t)row);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float* s = score_row(a.s, w);
-    const int phase = score_phase(out);
-    const bool aligned = score_phase(s) == phase;
-    const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
+    const int phase = ALIGNED ? 0 : score_phase(out);
+    ScoreShare<T, NV, DOCS, ALIGNED> mine;
+    mine.init(score_docs<DOCS>(a, w, phase), w, tid, phase);
+    mine.zeros(out, keys);
     int turn = 0;
     float t[NV][4];
-    uint32_t bits = 0;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, (v * T + tid) * 4 - phase) << (4 * v);
-    score_zeros<T, NV>(out, phase, keys, tid, bits);
-#pragma unroll
-    for (int v = 0; v < NV; ++v) score_load(t[v], s, (v * T + tid) * 4 - phase, (bits >> (4 * v)) & 15u, aligned);
+    mine.load(t, s, score_phase(s) == phase);
     float m[1] = {-INFINITY};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const uint32_t four = (bits >> (4 * v)) & 15u;
-        if (four) {
+        if (mine.any(v)) {
+            score_logits<CAP>(a.g, w, t[v], mine.column(v));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                t[v][k] = (four >> k) & 1u ? score_logit<CAP>(a.g, w, t[v][k], (v * T + tid) * 4 - phase + k) : -INFINITY;
+                t[v][k] = mine.has(v, k) ? t[v][k] : -INFINITY;
                 m[0] = fmaxf(m[0], t[v][k]);
             }
         }
@@ -188,10 +256,10 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        if ((bits >> (4 * v)) & 15u) {
+        if (mine.any(v)) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                t[v][k] = expf(t[v][k] - top);
+                t[v][k] = score_exp(t[v][k] - top);
                 part[k] = part[k] + t[v][k];
             }
         }
@@ -199,19 +267,23 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
     float z[1] = {(part[0] + part[1]) + (part[2] + part[3])};
     team_fold<FoldSum, THREADS, T>(z, sh, turn, 1);
     const float inv = z[0] == 0.0f ? 0.0f : __frcp_rn(z[0]);
+    const bool usual = z[0] < INFINITY;                  // else NaN, which must not reach the masked columns
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c0 = (v * T + tid) * 4 - phase;
-        if ((bits >> (4 * v)) & 15u) {
+        if (mine.any(v)) {
             float p[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) p[k] = (bits >> (4 * v + k)) & 1u ? t[v][k] * inv : 0.0f;
-            score_store(out, c0, keys, p);
+            for (int k = 0; k < 4; ++k) p[k] = t[v][k] * inv;
+            if (!usual) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) p[k] = mine.has(v, k) ? p[k] : 0.0f;
+            }
+            mine.store(out, v, keys, p);
         }
     }
 }
 
-template <int THREADS, int T, int NV, bool CAP, bool DOCS>
+template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS)
 score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
     static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
@@ -220,52 +292,54 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
     const int tid = threadIdx.x % T;
     const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
     if (row >= a.rows) return;
-    const ScorePlace w = score_place(a, row);
+    const ScorePlace w = score_place(a, (uint32_t)row);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
-    const int phase = score_phase(out);
-    const bool p_aligned = score_phase(pr) == phase, g_aligned = score_phase(gr) == phase, s_aligned = CAP && score_phase(sr) == phase;
-    const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
+    const int phase = ALIGNED ? 0 : score_phase(out);
+    ScoreShare<T, NV, DOCS, ALIGNED> mine;
+    mine.init(score_docs<DOCS>(a, w, phase), w, tid, phase);
+    mine.zeros(out, keys);
     int turn = 0;
     float p[NV][4], dp[NV][4], s[CAP ? NV : 1][4];
-    uint32_t bits = 0;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, (v * T + tid) * 4 - phase) << (4 * v);
-    score_zeros<T, NV>(out, phase, keys, tid, bits);
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        const int c0 = (v * T + tid) * 4 - phase;
-        const uint32_t four = (bits >> (4 * v)) & 15u;
-        score_load(p[v], pr, c0, four, p_aligned);
-        score_load(dp[v], gr, c0, four, g_aligned);
-        if (CAP) score_load(s[v], sr, c0, four, s_aligned);
-    }
+    mine.load(p, pr, score_phase(pr) == phase);
+    mine.load(dp, gr, score_phase(gr) == phase);
+    if constexpr (CAP) mine.load(s, sr, score_phase(sr) == phase);
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+        if (mine.any(v)) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) part[k] = fmaf(p[v][k], dp[v][k], part[k]);
+            for (int k = 0; k < 4; ++k) {
+                if (ALIGNED) {                           // whole fours were read: masked columns hold anything
+                    p[v][k] = mine.has(v, k) ? p[v][k] : 0.0f;
+                    dp[v][k] = mine.has(v, k) ? dp[v][k] : 0.0f;
+                    if constexpr (CAP) s[v][k] = mine.has(v, k) ? s[v][k] : 0.0f;
+                }
+                part[k] = fmaf(p[v][k], dp[v][k], part[k]);
+            }
+        }
+    }
     float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
     team_fold<FoldSum, THREADS, T>(d, sh, turn, 1);
+    const bool usual = fabsf(d[0]) < INFINITY;           // else 0 * (0 - D) is NaN in the masked columns
     float slope_sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const int c0 = (v * T + tid) * 4 - phase;
-        if ((bits >> (4 * v)) & 15u) {
+        if (mine.any(v)) {
             float r[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float dt = p[v][k] * (dp[v][k] - d[0]);
-                if (a.slope_part && ((bits >> (4 * v + k)) & 1u)) slope_sum = fmaf((float)abs(c0 + k - w.centre) + w.beyond, dt, slope_sum);
-                r[k] = dt * a.g.scale;
-                if (CAP) {
-                    const float th = tanhf(s[v][k] * a.g.over_cap);
-                    r[k] = r[k] * fmaf(-th, th, 1.0f);
-                }
-                if (!((bits >> (4 * v + k)) & 1u)) r[k] = 0.0f;
+                r[k] = p[v][k] * (dp[v][k] - d[0]);
+                if (!usual && !mine.has(v, k)) r[k] = 0.0f;
             }
-            score_store(out, c0, keys, r);
+            if (a.slope_part) {
+                const float from = (float)(mine.column(v) - w.centre);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) slope_sum = fmaf(fabsf(from + (float)k) + w.beyond, r[k], slope_sum);
+            }
+            score_slow<CAP>(a.g, r, s[CAP ? v : 0]);
+            mine.store(out, v, keys, r);
         }
     }
     if (a.slope_part) {
@@ -292,7 +366,7 @@ __global__ void __launch_bounds__(kSweepThreads)
 score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     const int64_t row = blockIdx.x / cs;
-    const ScorePlace w = score_place(a, row);
+    const ScorePlace w = score_place(a, (uint32_t)row);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float* s = score_row(a.s, w);
@@ -316,13 +390,16 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
         for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
         float top = m;
 #pragma unroll
-        for (int u = 0; u < kSweepBatch; ++u)
+        for (int u = 0; u < kSweepBatch; ++u) {
+            if (!bits[u]) continue;
+            score_logits<CAP>(a.g, w, t[u], (int)((f + (int64_t)u * kSweepThreads) * 4) - phase);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                t[u][k] = (bits[u] >> k) & 1u ? score_logit<CAP>(a.g, w, t[u][k], (int)((f + (int64_t)u * kSweepThreads) * 4) - phase + k) : -INFINITY;
+                t[u][k] = (bits[u] >> k) & 1u ? t[u][k] : -INFINITY;
                 top = fmaxf(top, t[u][k]);
             }
-        if (m != -INFINITY) z = z * expf(m - top);
+        }
+        if (m != -INFINITY) z = z * score_exp(m - top);
         m = top;
         const float from = m == -INFINITY ? 0.0f : m;
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -330,14 +407,14 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
         for (int u = 0; u < kSweepBatch; ++u)
             if (bits[u]) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) part[k] = part[k] + expf(t[u][k] - from);
+                for (int k = 0; k < 4; ++k) part[k] = part[k] + score_exp(t[u][k] - from);
             }
         z = z + ((part[0] + part[1]) + (part[2] + part[3]));
     }
     float top[1] = {m};
     team_fold<FoldMax, kSweepThreads, kSweepThreads>(top, sh, turn, cs);
     const float from = top[0] == -INFINITY ? 0.0f : top[0];
-    float sum[1] = {m == -INFINITY ? z : z * expf(m - from)};
+    float sum[1] = {m == -INFINITY ? z : z * score_exp(m - from)};
     team_fold<FoldSum, kSweepThreads, kSweepThreads>(sum, sh, turn, cs);
     const float inv = sum[0] == 0.0f ? 0.0f : __frcp_rn(sum[0]);
     // second sweep
@@ -357,9 +434,12 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
             if (at >= span.hi) break;
             const int c0 = (int)(at * 4) - phase;
             float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (bits[u]) {
+                score_logits<CAP>(a.g, w, t[u], c0);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if ((bits[u] >> k) & 1u) p[k] = expf(score_logit<CAP>(a.g, w, t[u][k], c0 + k) - from) * inv;
+                for (int k = 0; k < 4; ++k)
+                    if ((bits[u] >> k) & 1u) p[k] = score_exp(t[u][k] - from) * inv;
+            }
             score_store(out, c0, keys, p);
         }
     }
@@ -371,7 +451,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     __shared__ TeamSlots<kSweepThreads, 1, double> sh_slope;
     const int64_t row = blockIdx.x / cs;
-    const ScorePlace w = score_place(a, row);
+    const ScorePlace w = score_place(a, (uint32_t)row);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
@@ -418,18 +498,16 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
             const int64_t at = f + (int64_t)u * kSweepThreads;
             if (at >= span.hi) break;
             const int c0 = (int)(at * 4) - phase;
-            float r[4];
+            float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (bits[u]) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool in = (bits[u] >> k) & 1u;
-                const float dt = p[u][k] * (dp[u][k] - d[0]);
-                if (a.slope_part && in) slope_part = fmaf((float)abs(c0 + k - w.centre) + w.beyond, dt, slope_part);
-                r[k] = dt * a.g.scale;
-                if (CAP) {
-                    const float th = tanhf(s[u][k] * a.g.over_cap);
-                    r[k] = r[k] * fmaf(-th, th, 1.0f);
+                for (int k = 0; k < 4; ++k) r[k] = (bits[u] >> k) & 1u ? p[u][k] * (dp[u][k] - d[0]) : 0.0f;
+                if (a.slope_part) {
+                    const float from = (float)(c0 - w.centre);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) slope_part = fmaf(fabsf(from + (float)k) + w.beyond, r[k], slope_part);
                 }
-                if (!in) r[k] = 0.0f;
+                score_slow<CAP>(a.g, r, s[u]);
             }
             score_store(out, c0, keys, r);
         }
@@ -457,82 +535,107 @@ score_slope_fold_kernel(const double* __restrict__ part, int64_t batch, int64_t 
 }
 
 // ---- host -----------------------------------------------------------------------------------------------
+struct ScoreCall {
+    ScoreArgs a;
+    bool backward, cap, docs, aligned;
+    int sm_count;
+    cudaStream_t st;
+};
+constexpr const char* kScoreName = "score_softmax";
+
+template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
+int rows_with(const ScoreCall& c) {
+    const int64_t blocks = ceil_div(c.a.rows, (int64_t)(THREADS / T));
+    if (!c.backward) return launch_clusters(kScoreName, score_softmax_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, 1, c.st, c.a);
+    // two or three operands are held: half the fours per thread of the forward pass
+    if constexpr (NV == 8) {
+        constexpr int WIDE = 2 * T > THREADS ? 2 * T : THREADS;
+        return launch_clusters(kScoreName, score_softmax_backward_kernel<WIDE, 2 * T, 4, CAP, DOCS, ALIGNED>, ceil_div(c.a.rows, (int64_t)(WIDE / (2 * T))), WIDE, 0, 1, c.st, c.a);
+    } else return launch_clusters(kScoreName, score_softmax_backward_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, 1, c.st, c.a);
+}
 template <int THREADS, int T, int NV>
-int rows_as(const ScoreArgs& a, bool backward, bool cap, bool docs, cudaStream_t st) {
-    const int64_t blocks = ceil_div(a.rows, (int64_t)(THREADS / T));
-    const char* who = "score_softmax";
-    if (backward) {
-        if (cap) return docs ? launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, true, true>, blocks, THREADS, 0, 1, st, a)
-                             : launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, true, false>, blocks, THREADS, 0, 1, st, a);
-        return docs ? launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, false, true>, blocks, THREADS, 0, 1, st, a)
-                    : launch_clusters(who, score_softmax_backward_kernel<THREADS, T, NV, false, false>, blocks, THREADS, 0, 1, st, a);
+int rows_as(const ScoreCall& c) {
+    if (c.cap) {
+        if (c.docs) return c.aligned ? rows_with<THREADS, T, NV, true, true, true>(c) : rows_with<THREADS, T, NV, true, true, false>(c);
+        return c.aligned ? rows_with<THREADS, T, NV, true, false, true>(c) : rows_with<THREADS, T, NV, true, false, false>(c);
     }
-    if (cap) return docs ? launch_clusters(who, score_softmax_kernel<THREADS, T, NV, true, true>, blocks, THREADS, 0, 1, st, a)
-                         : launch_clusters(who, score_softmax_kernel<THREADS, T, NV, true, false>, blocks, THREADS, 0, 1, st, a);
-    return docs ? launch_clusters(who, score_softmax_kernel<THREADS, T, NV, false, true>, blocks, THREADS, 0, 1, st, a)
-                : launch_clusters(who, score_softmax_kernel<THREADS, T, NV, false, false>, blocks, THREADS, 0, 1, st, a);
+    if (c.docs) return c.aligned ? rows_with<THREADS, T, NV, false, true, true>(c) : rows_with<THREADS, T, NV, false, true, false>(c);
+    return c.aligned ? rows_with<THREADS, T, NV, false, false, true>(c) : rows_with<THREADS, T, NV, false, false, false>(c);
 }
 
-int sweep(const ScoreArgs& a, bool backward, bool cap, bool docs, int sm_count, cudaStream_t st) {
+template <bool CAP, bool DOCS>
+int sweep_with(const ScoreCall& c, int cs) {
+    if (c.backward) return launch_clusters(kScoreName, score_softmax_backward_sweep_kernel<CAP, DOCS>, c.a.rows * cs, kSweepThreads, 0, cs, c.st, c.a, cs);
+    return launch_clusters(kScoreName, score_softmax_sweep_kernel<CAP, DOCS>, c.a.rows * cs, kSweepThreads, 0, cs, c.st, c.a, cs);
+}
+int sweep(const ScoreCall& c) {
     // as many CTAs per row as it takes to occupy the machine, while each has at least 4096 keys
     int cs = 1;
-    while (cs < kMaxCluster && a.rows * cs < 2 * sm_count && a.g.keys / (2 * cs) >= 4096) cs *= 2;
-    const int64_t blocks = a.rows * cs;
-    const char* who = "score_softmax";
-    if (backward) {
-        if (cap) return docs ? launch_clusters(who, score_softmax_backward_sweep_kernel<true, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
-                             : launch_clusters(who, score_softmax_backward_sweep_kernel<true, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
-        return docs ? launch_clusters(who, score_softmax_backward_sweep_kernel<false, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
-                    : launch_clusters(who, score_softmax_backward_sweep_kernel<false, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
-    }
-    if (cap) return docs ? launch_clusters(who, score_softmax_sweep_kernel<true, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
-                         : launch_clusters(who, score_softmax_sweep_kernel<true, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
-    return docs ? launch_clusters(who, score_softmax_sweep_kernel<false, true>, blocks, kSweepThreads, 0, cs, st, a, cs)
-                : launch_clusters(who, score_softmax_sweep_kernel<false, false>, blocks, kSweepThreads, 0, cs, st, a, cs);
+    while (cs < kMaxCluster && c.a.rows * cs < 2 * c.sm_count && c.a.g.keys / (2 * cs) >= 4096) cs *= 2;
+    if (c.cap) return c.docs ? sweep_with<true, true>(c, cs) : sweep_with<true, false>(c, cs);
+    return c.docs ? sweep_with<false, true>(c, cs) : sweep_with<false, false>(c, cs);
 }
 
-int launch_scores(ScoreArgs& a, bool backward, cudaStream_t st) {
+// Whether all rows of the operand start on 16 bytes; fills in the distance of consecutive rows if there is one.
+bool settle_rows(const ScoreGeom& g, ScoreRows* r) {
+    if (!r->p) return true;
+    const int64_t q = g.queries > 1 ? r->sq : 0, h = g.heads > 1 ? r->sh : 0, b = g.batch > 1 ? r->sb : 0;
+    r->even = -1;
+    const int64_t even = g.queries > 1 ? q : (g.heads > 1 ? h : b);
+    if ((g.heads <= 1 || h == even * g.queries) && (g.batch <= 1 || b == even * g.queries * g.heads)) r->even = even;
+    return is_aligned(r->p, 16) && q % 4 == 0 && h % 4 == 0 && b % 4 == 0;
+}
+
+int launch_scores(ScoreCall& c) {
+    ScoreArgs& a = c.a;
     a.rows = a.g.batch * a.g.heads * a.g.queries;
     if (a.rows == 0 || a.g.keys == 0) return CTB_OK;
     if (a.rows > 0x7FFFFFFFll || a.g.keys > (1ll << 30)) return set_error(CTB_ERR_LIMIT, "score_softmax: more than 2^31 - 1 rows or 2^30 keys");
     DeviceInfo di;
     if (int rc = current_device_info(&di)) return rc;
+    c.sm_count = di.sm_count;
     a.by_queries = make_fastdiv((uint32_t)a.g.queries);
     a.by_heads = make_fastdiv((uint32_t)a.g.heads);
-    const bool cap = a.g.cap > 0.0f, docs = a.g.key_docs.p != nullptr;
+    c.cap = a.g.cap > 0.0f;
+    c.docs = a.g.key_docs.p != nullptr;
+    const bool rows_aligned = settle_rows(a.g, &a.s) & settle_rows(a.g, &a.p) & settle_rows(a.g, &a.dp);
+    c.aligned = rows_aligned && a.g.keys % 4 == 0 && is_aligned(a.out, 16);
     // columns to deal out: up to three more than the keys where rows do not start on 16 bytes
     const int64_t n = a.g.keys % 4 == 0 && is_aligned(a.out, 16) ? a.g.keys : a.g.keys + 3;
-    if (n <= 128) return rows_as<256, 32, 1>(a, backward, cap, docs, st);
-    if (n <= 256) return rows_as<256, 32, 2>(a, backward, cap, docs, st);
-    if (n <= 512) return rows_as<256, 32, 4>(a, backward, cap, docs, st);
-    if (n <= 1024) return backward ? rows_as<256, 64, 4>(a, backward, cap, docs, st) : rows_as<256, 32, 8>(a, backward, cap, docs, st);
-
-    if (n <= 2048) return rows_as<256, 128, 4>(a, backward, cap, docs, st);
-    if (n <= 4096) return rows_as<256, 256, 4>(a, backward, cap, docs, st);
-    if (n <= 8192) return rows_as<512, 512, 4>(a, backward, cap, docs, st);
-    return sweep(a, backward, cap, docs, di.sm_count, st);
+    if (n <= 128) return rows_as<256, 32, 1>(c);
+    if (n <= 256) return rows_as<256, 32, 2>(c);
+    if (n <= 512) return rows_as<256, 32, 4>(c);
+    if (n <= 1024) return rows_as<256, 32, 8>(c);
+    if (n <= 2048) return rows_as<256, 64, 8>(c);
+    if (n <= 4096) return rows_as<256, 128, 8>(c);
+    if (n <= 8192) return rows_as<256, 256, 8>(c);
+    return sweep(c);
 }
 
 }  // namespace
 
 int launch_score_softmax(const ScoreGeom& g, ScoreRows scores, float* out, cudaStream_t st) {
-    ScoreArgs a{};
-    a.g = g;
-    a.s = scores;
-    a.out = out;
-    return launch_scores(a, false, st);
+    ScoreCall c{};
+    c.a.g = g;
+    c.a.s = scores;
+    c.a.out = out;
+    c.st = st;
+    return launch_scores(c);
 }
 
 int launch_score_softmax_backward(const ScoreGeom& g, ScoreRows grad, ScoreRows probs, ScoreRows scores, float* grad_scores,
                                   float* grad_slopes, double* partials, cudaStream_t st) {
-    ScoreArgs a{};
+    ScoreCall c{};
+    ScoreArgs& a = c.a;
     a.g = g;
     a.s = scores;
     a.p = probs;
     a.dp = grad;
     a.out = grad_scores;
     a.slope_part = grad_slopes ? partials : nullptr;
-    if (int rc = launch_scores(a, true, st)) return rc;
+    c.backward = true;
+    c.st = st;
+    if (int rc = launch_scores(c)) return rc;
     if (!grad_slopes || g.heads == 0) return CTB_OK;
     if (a.rows == 0 || g.keys == 0) {                    // sums over nothing
         CTB_CUDA_TRY(cudaMemsetAsync(grad_slopes, 0, (size_t)g.heads * sizeof(float), st));

@@ -8,6 +8,7 @@ namespace ctb {
 struct ScoreRows {
     const float* p;
     int64_t sb, sh, sq;
+    int64_t even;                       // distance of consecutive rows in (batch, head, query) order, -1: none; set by the launchers
 };
 // An Int32 rule table with a stride per dim; p == NULL: the rule is absent.
 struct ScoreTable {

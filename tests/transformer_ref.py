@@ -59,8 +59,9 @@ def score_softmax(s, rules):
 
 def score_bound(s, p, rules):
     """|error| of a probability.  t: at most four roundings and a tanh within 2 steps (4 U) of a value no larger
-    than T = |t| + bias; subtracting the maximum one more; so each exponential is off by 2 * 9 U * T relative,
-    expf by 4 U, the sum (chains of at most 64 terms, then a tree of at most 13) by 77 U, reciprocal and
+    than T = |t| + bias, so t and the maximum are off by 8 U T each; their difference, of at most 2 T, is rounded
+    (2 U T) and multiplied by log2(e), a rounded constant (4 U T): each exponential is off by 22 U T relative,
+    the instruction for it by 2^-22 = 4 U, the sum (chains of at most 64 terms, then a tree of at most 13) by 77 U, reciprocal and
     product by 2 U."""
     ok = admitted(s.shape, rules, s.device)
     bare = {k: v for k, v in rules.items() if k != "slopes"}
@@ -75,7 +76,7 @@ def score_bound(s, p, rules):
         extra = s.shape[-1] if rules.get("key_docs") is not None else 0
         T = T + rules["slopes"].double().abs()[None, :, None, None] * (d + extra)
     top = T.amax(-1, keepdim=True)
-    return p * U * (18.0 * top + 83.0) + 1e-37
+    return p * U * (22.0 * top + 83.0) + 1e-37
 
 
 def score_gradients(s, p, dp, rules):
