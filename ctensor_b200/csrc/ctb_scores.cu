@@ -27,6 +27,18 @@ struct ScoreArgs {
     FastDiv by_queries, by_heads;
 };
 
+// The row of a team.  Teams smaller than a warp keep their warp company when there is no row left for them (they then
+// see and write nothing).
+struct ScoreRow {
+    uint32_t row;
+    bool present;
+};
+template <int THREADS, int T>
+__device__ __forceinline__ ScoreRow score_row_of(const ScoreArgs& a, int cs) {
+    const int64_t row = (int64_t)(T == THREADS ? blockIdx.x / (unsigned)cs : blockIdx.x) * (THREADS / T) + threadIdx.x / T;
+    const bool present = row < a.rows;
+    return {present ? (uint32_t)row : (uint32_t)(a.rows - 1), present};
+}
 // Where a row is and what its query may look at.
 struct ScorePlace {
     uint32_t row, b, h, i;
@@ -36,13 +48,13 @@ struct ScorePlace {
     float slope;
     int doc;
 };
-__device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, uint32_t row) {
+__device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, ScoreRow r) {
     const ScoreGeom& g = a.g;
     const int keys = (int)g.keys;
     ScorePlace w;
-    const uint32_t bh = fast_div(row, a.by_queries);
-    w.row = row;
-    w.i = row - bh * a.by_queries.d;
+    const uint32_t bh = fast_div(r.row, a.by_queries);
+    w.row = r.row;
+    w.i = r.row - bh * a.by_queries.d;
     w.b = fast_div(bh, a.by_heads);
     w.h = bh - w.b * a.by_heads.d;
     int64_t pos = (g.query_start.p ? (int64_t)g.query_start.p[w.b * g.query_start.sb] : g.keys - g.queries) + w.i;
@@ -67,6 +79,22 @@ __device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, uint32_t r
 __device__ __forceinline__ const float* score_row(const ScoreRows& r, const ScorePlace& w) {
     if (r.even >= 0) return r.p + (int64_t)w.row * r.even;
     return r.p + w.b * r.sb + w.h * r.sh + w.i * r.sq;
+}
+
+// What of a row a CTA of its cluster has: the fours from `from` on, up to the column `end`.
+struct ScoreSpan {
+    int from, end;
+    __device__ __forceinline__ ScorePlace sees(ScorePlace w) const {
+        w.live = min(w.live, end);
+        return w;
+    }
+};
+template <int T>
+__device__ __forceinline__ ScoreSpan score_span(const ScoreArgs& a, const ScoreRow& r, int keys, int phase, int cs) {
+    if (T < 32 && !r.present) return {0, 0};
+    if (cs == 1) return {0, keys};
+    const int fours = (keys + phase + 3) / 4, share = (fours + cs - 1) / cs, from = share * (int)cluster_rank();
+    return {from, min(keys, max((from + share) * 4 - phase, 0))};
 }
 
 // Rows start at any multiple of four bytes.  Columns are dealt out in fours counted from the output row's
@@ -178,11 +206,23 @@ struct ScoreShare {
     int first;                          // column of the first four
     int rest;                           // admissible columns from there on
     uint32_t bits;
-    __device__ __forceinline__ void init(const ScoreDocs& docs, const ScorePlace& w, int tid, int phase) {
-        first = tid * 4 - phase;
+    // `from`: the first four of this CTA's slice of the row
+    __device__ __forceinline__ void init(const ScoreDocs& docs, const ScorePlace& w, int from, int tid, int phase) {
+        first = (from + tid) * 4 - phase;
         rest = w.live - first;
         bits = 0;
-        if (kBits) {
+        if (DOCS && ALIGNED && docs.fours) {             // fours of document numbers may be read whole
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int left = rest - v * T * 4;
+                if (left > 0) {
+                    const int4 d = *reinterpret_cast<const int4*>(docs.p + column(v));
+                    uint32_t four = (d.x == w.doc ? 1u : 0u) + (d.y == w.doc ? 2u : 0u) + (d.z == w.doc ? 4u : 0u) + (d.w == w.doc ? 8u : 0u);
+                    if (left < 4) four &= (1u << left) - 1u;
+                    bits |= four << (4 * v);
+                }
+            }
+        } else if (kBits) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, column(v)) << (4 * v);
         }
@@ -205,37 +245,40 @@ struct ScoreShare {
             }
         }
     }
-    __device__ __forceinline__ void store(float* out, int v, int keys, const float (&x)[4]) const {
+    __device__ __forceinline__ void store(float* out, int v, int end, const float (&x)[4]) const {
         if (ALIGNED) score_store_four(out + column(v), x);
-        else score_store(out, column(v), keys, x);
+        else score_store(out, column(v), end, x);
     }
     // Zeros into the fours without an admitted key, ahead of the loads: these stores need not wait for them.
-    __device__ __forceinline__ void zeros(float* out, int keys) const {
+    __device__ __forceinline__ void zeros(float* out, int end) const {
         const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1                                         // unrolled, its addresses double the kernel's registers
         for (int v = 0; v < NV; ++v) {
             const int c0 = column(v);
-            if (!any(v) && c0 < keys) store(out, v, keys, zero);
+            if (!any(v) && c0 < end) store(out, v, end, zero);
         }
     }
 };
 
 template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS)
-score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
+__global__ void __launch_bounds__(THREADS, (ALIGNED ? 1280 : 1024) / THREADS)
+score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
+    const int cs = T == 512 ? ctas : 1;                  // only whole CTAs of 512 threads come in clusters
     static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
     __shared__ TeamSlots<THREADS, 1, float> sh;
     const int tid = threadIdx.x % T;
-    const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
-    if (row >= a.rows) return;                           // whole teams leave together
-    const ScorePlace w = score_place(a, (uint32_t)row);
+    const ScoreRow place = score_row_of<THREADS, T>(a, cs);
+    if (T >= 32 && !place.present) return;               // whole teams leave together; never in a cluster
+    const int64_t row = place.row;
+    const ScorePlace w = score_place(a, place);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float* s = score_row(a.s, w);
     const int phase = ALIGNED ? 0 : score_phase(out);
     ScoreShare<T, NV, DOCS, ALIGNED> mine;
-    mine.init(score_docs<DOCS>(a, w, phase), w, tid, phase);
-    mine.zeros(out, keys);
+    const ScoreSpan span = score_span<T>(a, place, keys, phase, cs);
+    mine.init(score_docs<DOCS>(a, w, phase), span.sees(w), span.from, tid, phase);
+    mine.zeros(out, span.end);
     int turn = 0;
     float t[NV][4];
     mine.load(t, s, score_phase(s) == phase);
@@ -251,7 +294,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
             }
         }
     }
-    team_fold<FoldMax, THREADS, T>(m, sh, turn, 1);
+    team_fold<FoldMax, THREADS, T>(m, sh, turn, cs);
     const float top = m[0] == -INFINITY ? 0.0f : m[0];
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -265,7 +308,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
         }
     }
     float z[1] = {(part[0] + part[1]) + (part[2] + part[3])};
-    team_fold<FoldSum, THREADS, T>(z, sh, turn, 1);
+    team_fold<FoldSum, THREADS, T>(z, sh, turn, cs);
     const float inv = z[0] == 0.0f ? 0.0f : __frcp_rn(z[0]);
     const bool usual = z[0] < INFINITY;                  // else NaN, which must not reach the masked columns
 #pragma unroll
@@ -278,28 +321,31 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) p[k] = mine.has(v, k) ? p[k] : 0.0f;
             }
-            mine.store(out, v, keys, p);
+            mine.store(out, v, span.end, p);
         }
     }
 }
 
 template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS)
-score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
+score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
+    const int cs = T == 512 ? ctas : 1;                  // only whole CTAs of 512 threads come in clusters
     static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
     __shared__ TeamSlots<THREADS, 1, float> sh;
     __shared__ TeamSlots<THREADS, 1, double> sh_slope;
     const int tid = threadIdx.x % T;
-    const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
-    if (row >= a.rows) return;
-    const ScorePlace w = score_place(a, (uint32_t)row);
+    const ScoreRow place = score_row_of<THREADS, T>(a, cs);
+    if (T >= 32 && !place.present) return;
+    const int64_t row = place.row;
+    const ScorePlace w = score_place(a, place);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
     const int phase = ALIGNED ? 0 : score_phase(out);
     ScoreShare<T, NV, DOCS, ALIGNED> mine;
-    mine.init(score_docs<DOCS>(a, w, phase), w, tid, phase);
-    mine.zeros(out, keys);
+    const ScoreSpan span = score_span<T>(a, place, keys, phase, cs);
+    mine.init(score_docs<DOCS>(a, w, phase), span.sees(w), span.from, tid, phase);
+    mine.zeros(out, span.end);
     int turn = 0;
     float p[NV][4], dp[NV][4], s[CAP ? NV : 1][4];
     mine.load(p, pr, score_phase(pr) == phase);
@@ -321,7 +367,7 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
         }
     }
     float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
-    team_fold<FoldSum, THREADS, T>(d, sh, turn, 1);
+    team_fold<FoldSum, THREADS, T>(d, sh, turn, cs);
     const bool usual = fabsf(d[0]) < INFINITY;           // else 0 * (0 - D) is NaN in the masked columns
     float slope_sum = 0.0f;
 #pragma unroll
@@ -339,13 +385,13 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a) {
                 for (int k = 0; k < 4; ++k) slope_sum = fmaf(fabsf(from + (float)k) + w.beyond, r[k], slope_sum);
             }
             score_slow<CAP>(a.g, r, s[CAP ? v : 0]);
-            mine.store(out, v, keys, r);
+            mine.store(out, v, span.end, r);
         }
     }
     if (a.slope_part) {
         double sum[1] = {(double)slope_sum};
-        team_fold<FoldSum, THREADS, T>(sum, sh_slope, turn, 1);
-        if (tid == 0) a.slope_part[row] = sum[0];
+        team_fold<FoldSum, THREADS, T>(sum, sh_slope, turn, cs);
+        if (tid == 0 && place.present && (cs == 1 || cluster_rank() == 0)) a.slope_part[row] = sum[0];
     }
 }
 
@@ -366,7 +412,7 @@ __global__ void __launch_bounds__(kSweepThreads)
 score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     const int64_t row = blockIdx.x / cs;
-    const ScorePlace w = score_place(a, (uint32_t)row);
+    const ScorePlace w = score_place(a, {(uint32_t)row, true});
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float* s = score_row(a.s, w);
@@ -451,7 +497,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     __shared__ TeamSlots<kSweepThreads, 1, double> sh_slope;
     const int64_t row = blockIdx.x / cs;
-    const ScorePlace w = score_place(a, (uint32_t)row);
+    const ScorePlace w = score_place(a, {(uint32_t)row, true});
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
@@ -538,6 +584,7 @@ score_slope_fold_kernel(const double* __restrict__ part, int64_t batch, int64_t 
 struct ScoreCall {
     ScoreArgs a;
     bool backward, cap, docs, aligned;
+    int cs;                             // CTAs per row
     int sm_count;
     cudaStream_t st;
 };
@@ -545,13 +592,9 @@ constexpr const char* kScoreName = "score_softmax";
 
 template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
 int rows_with(const ScoreCall& c) {
-    const int64_t blocks = ceil_div(c.a.rows, (int64_t)(THREADS / T));
-    if (!c.backward) return launch_clusters(kScoreName, score_softmax_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, 1, c.st, c.a);
-    // two or three operands are held: half the fours per thread of the forward pass
-    if constexpr (NV == 8) {
-        constexpr int WIDE = 2 * T > THREADS ? 2 * T : THREADS;
-        return launch_clusters(kScoreName, score_softmax_backward_kernel<WIDE, 2 * T, 4, CAP, DOCS, ALIGNED>, ceil_div(c.a.rows, (int64_t)(WIDE / (2 * T))), WIDE, 0, 1, c.st, c.a);
-    } else return launch_clusters(kScoreName, score_softmax_backward_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, 1, c.st, c.a);
+    const int64_t blocks = ceil_div(c.a.rows, (int64_t)(THREADS / T)) * c.cs;
+    if (!c.backward) return launch_clusters(kScoreName, score_softmax_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, c.cs, c.st, c.a, c.cs);
+    return launch_clusters(kScoreName, score_softmax_backward_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, c.cs, c.st, c.a, c.cs);
 }
 template <int THREADS, int T, int NV>
 int rows_as(const ScoreCall& c) {
@@ -568,10 +611,13 @@ int sweep_with(const ScoreCall& c, int cs) {
     if (c.backward) return launch_clusters(kScoreName, score_softmax_backward_sweep_kernel<CAP, DOCS>, c.a.rows * cs, kSweepThreads, 0, cs, c.st, c.a, cs);
     return launch_clusters(kScoreName, score_softmax_sweep_kernel<CAP, DOCS>, c.a.rows * cs, kSweepThreads, 0, cs, c.st, c.a, cs);
 }
+// CTAs per row: until what the resident CTAs (two per SM) read twice takes half of L2's 126 MB, for rows longer
+// than that would be read from HBM twice (12 heads, gradients of 64 queries x 100000 keys: 1 CTA 229 us, 4 188, 8 219;
+// 512 x 16384: 1 CTA 217, 2 246); or, with few rows, until the machine is occupied while each CTA has 4096 keys.
 int sweep(const ScoreCall& c) {
-    // as many CTAs per row as it takes to occupy the machine, while each has at least 4096 keys
+    const int64_t row_bytes = c.a.g.keys * 4 * (c.backward ? (c.cap ? 3 : 2) : 1);
     int cs = 1;
-    while (cs < kMaxCluster && c.a.rows * cs < 2 * c.sm_count && c.a.g.keys / (2 * cs) >= 4096) cs *= 2;
+    while (cs < kMaxCluster && (row_bytes / cs * 2 * c.sm_count > (int64_t(64) << 20) || (c.a.rows * cs < 2 * c.sm_count && c.a.g.keys / (2 * cs) >= 4096))) cs *= 2;
     if (c.cap) return c.docs ? sweep_with<true, true>(c, cs) : sweep_with<true, false>(c, cs);
     return c.docs ? sweep_with<false, true>(c, cs) : sweep_with<false, false>(c, cs);
 }
@@ -602,13 +648,27 @@ int launch_scores(ScoreCall& c) {
     c.aligned = rows_aligned && a.g.keys % 4 == 0 && is_aligned(a.out, 16);
     // columns to deal out: up to three more than the keys where rows do not start on 16 bytes
     const int64_t n = a.g.keys % 4 == 0 && is_aligned(a.out, 16) ? a.g.keys : a.g.keys + 3;
-    if (n <= 128) return rows_as<256, 32, 1>(c);
-    if (n <= 256) return rows_as<256, 32, 2>(c);
+    // Up to 512 columns a team takes 16 bytes a lane and as few lanes as hold the row four to a lane (rows of 64
+    // keys with a warp each spent most instructions on finding their place: 21.8 us where this takes the figure
+    // in the design notes); wider forward rows eight fours a lane, backward rows, with two or three operands, four.
+    c.cs = 1;
+    if (n <= 32) return rows_as<256, 8, 1>(c);
+    if (n <= 64) return rows_as<256, 8, 2>(c);
+    if (n <= 128) return rows_as<256, 8, 4>(c);
+    if (n <= 256) return rows_as<256, 16, 4>(c);
     if (n <= 512) return rows_as<256, 32, 4>(c);
-    if (n <= 1024) return rows_as<256, 32, 8>(c);
-    if (n <= 2048) return rows_as<256, 64, 8>(c);
-    if (n <= 4096) return rows_as<256, 128, 8>(c);
-    if (n <= 8192) return rows_as<256, 256, 8>(c);
+    if (n <= 1024) return c.backward ? rows_as<256, 64, 4>(c) : rows_as<256, 32, 8>(c);
+    if (n <= 2048) return c.backward ? rows_as<256, 128, 4>(c) : rows_as<256, 64, 8>(c);
+    // Few long rows: a cluster of CTAs holds each, as many as it takes to occupy the machine while each has 2048
+    // columns.  (With rows enough, clusters cost more than they bring: forward, 6144 rows of 16384 keys, 1 CTA
+    // 143 us, 2 268, 4 490; gradients 217 swept by one CTA, 361 held by four.)
+    const int64_t most = c.backward ? 8192 : 16384;      // columns in the registers of one CTA
+    while (c.cs < kMaxCluster && a.rows * c.cs * 2 <= c.sm_count && n / (c.cs * 2) >= 2048) c.cs *= 2;
+    if (c.cs > 1 && n <= most * c.cs) return c.backward ? rows_as<512, 512, 4>(c) : rows_as<512, 512, 8>(c);
+    c.cs = 1;
+    if (n <= 4096) return c.backward ? rows_as<256, 256, 4>(c) : rows_as<256, 128, 8>(c);
+    if (n <= 8192 && !c.backward) return rows_as<256, 256, 8>(c);
+    if (n <= most) return c.backward ? rows_as<512, 512, 4>(c) : rows_as<512, 512, 8>(c);
     return sweep(c);
 }
 

@@ -61,6 +61,13 @@ __device__ __forceinline__ void lane_fold(S (&v)[N], const S* p, int count) {
 // the rest — so that eight sums cost 9 shuffles instead of 40; lane l then holds value l / (32 / N).
 template <typename OP, int THREADS, int T, int N, typename S>
 __device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& sh, int& turn, int cs) {
+    if constexpr (T < 32) {                              // several teams in a warp, all of whose lanes take part
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int off = T / 2; off > 0; off >>= 1) v[n] = OP::of(v[n], __shfl_xor_sync(0xffffffffu, v[n], off));
+        return;
+    }
     const int lane = threadIdx.x & 31;
     int off = 16;
 #pragma unroll
