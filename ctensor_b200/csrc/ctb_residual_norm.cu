@@ -272,7 +272,7 @@ struct BwdFlags {
 };
 
 template <int THREADS, int T, int E, int VEC, typename F>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1)
 residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
     extern __shared__ __align__(16) float staged[];      // [stages][SLOTS][E][THREADS]
     constexpr bool FAST = F::FAST, POST = F::POST, FULL = F::FULL, GATE = F::GATE == 1 || !FAST;
@@ -311,6 +311,27 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
     const bool shared_gate = FAST ? F::GATE == 1 : a.shared_gate != 0;
     const bool scalar_gate = !FAST && g.gate_mode == kGateScalar && a.out.gate;
 
+    // Weights, and a gate row that rows share, stay in registers where those suffice (not beside the sums of two biases):
+    // with most of the SM's memory given to the ring, L1 is too small to serve them every row.
+    constexpr bool HOLD = FAST && (!FULL || !POST);
+    float w_pre[HOLD ? E : 1], w_post[HOLD && POST ? E : 1], w_gate[HOLD && F::GATE == 1 ? E : 1];
+    auto hold = [&](float* v, const float* row) {
+#pragma unroll
+        for (int i = 0; i < E / VEC; ++i) {
+            const int c = col_of<T, VEC>(i, tid);
+            float w[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) w[q] = 0.0f;
+            if (c < width) load_part<T, VEC>(w, row + begin, c);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) v[i * VEC + q] = w[q];
+        }
+    };
+    if constexpr (HOLD) {
+        hold(w_pre, g.pre_weight);
+        if constexpr (POST) hold(w_post, g.post_weight);
+    }
+
     // the thread's place in each operand's next row to fetch, and in its own stage slots
     const float* next[kInCount];
 #pragma unroll
@@ -347,15 +368,20 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
         const float4 st = next_st;
         fetch(ahead_at);                                 // into the place of the row before this one, which is done with
         if (row + 1 < hi) next_st = *++stats;
-        float w_pre[E];                                  // ahead of the wait for the row
+        float w_row[HOLD ? 1 : E];                       // ahead of the wait for the row
+        if constexpr (!HOLD) {
 #pragma unroll
-        for (int i = 0; i < E / VEC; ++i) {
-            float w[VEC];
+            for (int i = 0; i < E / VEC; ++i) {
+                float w[VEC];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) w[q] = 1.0f;
-            if (pre_weight && col_of<T, VEC>(i, tid) < width) load_part<T, VEC>(w, g.pre_weight + begin, col_of<T, VEC>(i, tid));
+                for (int q = 0; q < VEC; ++q) w[q] = 1.0f;
+                if (pre_weight && col_of<T, VEC>(i, tid) < width) load_part<T, VEC>(w, g.pre_weight + begin, col_of<T, VEC>(i, tid));
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) w_pre[i * VEC + q] = w[q];
+                for (int q = 0; q < VEC; ++q) w_row[i * VEC + q] = w[q];
+            }
+        }
+        if constexpr (HOLD && F::GATE == 1) {
+            if (left == g.gate_rows || row == lo) hold(w_gate, g.gate.p + group * g.gate.stride);
         }
         if (a.stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
         else if (a.stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
@@ -389,7 +415,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                         hat[e] = FULL ? (yv[q] - mean_y) * st.w : yv[q] * st.w;
                         pre_w[e] = fmaf(dh[q], hat[e], pre_w[e]);
                         if (FULL) pre_b[e] = pre_b[e] + dh[q];
-                        const float av = dh[q] * w_pre[e];
+                        const float av = dh[q] * (HOLD ? w_pre[HOLD ? e : 0] : w_row[HOLD ? 0 : e]);
                         if (FULL) s_a = s_a + av;
                         s_ay = fmaf(av, hat[e], s_ay);
                         e_[e] = fmaf(st.w, av, dy[q]);
@@ -404,13 +430,24 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                     for (int q = 0; q < VEC; ++q) k[q] = one_gate;
                     if (row_gate) {
                         float gv[VEC];
-                        if (staged_gate) read_own<VEC>(gv, at + kInGate * SLOT);
-                        else load_part<T, VEC>(gv, gate, c);
+                        if (staged_gate) {
+                            read_own<VEC>(gv, at + kInGate * SLOT);
+                        } else if constexpr (HOLD && F::GATE == 1) {
+#pragma unroll
+                            for (int q = 0; q < VEC; ++q) gv[q] = w_gate[i * VEC + q];
+                        } else {
+                            load_part<T, VEC>(gv, gate, c);
+                        }
 #pragma unroll
                         for (int q = 0; q < VEC; ++q) k[q] = gv[q] * g.scale;
                     }
                     if (post_weight) {
-                        load_part<T, VEC>(w, g.post_weight + begin, c);
+                        if constexpr (HOLD && POST) {
+#pragma unroll
+                            for (int q = 0; q < VEC; ++q) w[q] = w_post[i * VEC + q];
+                        } else {
+                            load_part<T, VEC>(w, g.post_weight + begin, c);
+                        }
 #pragma unroll
                         for (int q = 0; q < VEC; ++q) k[q] = k[q] * w[q];
                     }
@@ -470,11 +507,22 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                 if (post) {
 #pragma unroll
                     for (int q = 0; q < VEC; ++q) fv[q] = FULL ? (fv[q] - mean_f) * st.y : fv[q] * st.y;
-                    if (post_weight) load_part<T, VEC>(w, g.post_weight + begin, c);
+                    if constexpr (HOLD && POST) {
+#pragma unroll
+                        for (int q = 0; q < VEC; ++q) w[q] = w_post[i * VEC + q];
+                    } else if (post_weight) {
+                        load_part<T, VEC>(w, g.post_weight + begin, c);
+                    }
                 }
                 if (row_gate) {
-                    if (staged_gate) read_own<VEC>(gv, at + kInGate * SLOT);
-                    else load_part<T, VEC>(gv, gate, c);
+                    if (staged_gate) {
+                        read_own<VEC>(gv, at + kInGate * SLOT);
+                    } else if constexpr (HOLD && F::GATE == 1) {
+#pragma unroll
+                        for (int q = 0; q < VEC; ++q) gv[q] = w_gate[i * VEC + q];
+                    } else {
+                        load_part<T, VEC>(gv, gate, c);
+                    }
 #pragma unroll
                     for (int q = 0; q < VEC; ++q) gv[q] = gv[q] * g.scale;
                 }
@@ -651,20 +699,30 @@ int forward_as(const ResidualNormGeom& g, RowsIn x, RowsIn f, float* y, float* h
                            g, x, f, y, h, stats, cs);
 }
 
-// How a row is dealt out in the backward pass: a team of `team` threads with `share` columns each, `threads` to a
-// CTA, `cs` CTAs to a row.  One CTA of about 500 threads per SM: that many hold the column sums of their rows in
-// registers.  Up to 2048 columns it has several teams, so that one works while another waits in its fold;
-// a wider row keeps the SM busy by itself (the next ones are on their way into shared memory).  Twice the columns
-// per thread halve what a thread does once per row; with LayerNorms or biases the sums of 16 columns
-// would not fit the registers.
+// How a row is dealt out in the backward pass: a team of `team` threads with kBwdShare columns each, `threads` to
+// a CTA, `cs` CTAs to a row, `ctas` of them on an SM.  The column sums of a row's team live in registers, so
+// about 500 to 640 threads fit an SM.  Up to 2048 columns a CTA has several teams, so that one works while another
+// waits in its fold; a wider row keeps the SM busy by itself (the next ones are on their way into shared
+// memory) as long as one CTA holds it.  Beyond that, clusters of small CTAs, two on an SM for the same reason:
+// 4096 rows of 8192 columns with RMS norms took 206 us with one cluster per SM pair.
+constexpr int kBwdShare = 8;
 struct BwdShape {
-    int threads, team, share, cs;
+    int threads, team, cs, ctas;
 };
-BwdShape bwd_shape(int64_t cols, bool wide) {
-    for (const BwdShape& s : {BwdShape{512, 32, 8, 1}, BwdShape{512, 64, 8, 1}, BwdShape{480, 96, 8, 1}, BwdShape{512, 128, 8, 1}, BwdShape{384, 192, 8, 1}, BwdShape{512, 256, 8, 1}})
-        if (cols <= s.team * s.share) return s;
-    if (wide) return {640, 640, 8, cluster_for(cols, 640 * 8)};
-    return {512, 512, 8, cluster_for(cols, 512 * 8)};
+// Specialised: RMS norms without biases; a LayerNorm or a bias before the next block; both norms, one of them such.
+// Rows that go element by element.  Everything else.
+enum BwdKind { kBwdLean, kBwdFullPre, kBwdFull, kBwdScalar, kBwdAny };
+BwdShape bwd_shape(int64_t cols, BwdKind kind) {
+    for (const BwdShape& s : {BwdShape{512, 32, 1, 1}, BwdShape{512, 64, 1, 1}, BwdShape{480, 96, 1, 1}, BwdShape{512, 128, 1, 1}, BwdShape{384, 192, 1, 1}, BwdShape{512, 256, 1, 1}})
+        if (cols <= s.team * kBwdShare && (kind != kBwdScalar || s.team == 32 || s.team == 128)) return s;
+    // (the sums of a LayerNorm and its bias leave a thread 128 registers where the CTA can be that small)
+    if (cols <= 512 * kBwdShare && kind != kBwdLean) return {512, 512, 1, 1};
+    const bool small = kind == kBwdLean || kind == kBwdFullPre;
+    const int alone = small ? 640 : 512, in_cluster = small ? 320 : 256;
+    if (cols <= alone * kBwdShare) return {alone, alone, 1, 1};
+    const int cs = cluster_for(cols, in_cluster * kBwdShare);
+    if ((small || kind == kBwdFull) && cs <= kMaxCluster) return {in_cluster, in_cluster, cs, 2};
+    return {alone, alone, cluster_for(cols, alone * kBwdShare), 1};
 }
 // Teams that walk the rows, at most one per row: `ctas` CTAs (clusters) run at once.
 int64_t bwd_teams(int64_t rows, const BwdShape& s, int64_t ctas) {
@@ -688,9 +746,9 @@ int backward_as(BwdCall& c) {
     auto kernel = residual_norm_backward_kernel<THREADS, T, E, VEC, F>;
     ResidualBwd& a = c.a;
     const int cs = c.shape.cs;
-    const size_t stage = (size_t)F::SLOTS * E * THREADS * sizeof(float), room = (size_t)216 * 1024;
+    const size_t stage = (size_t)F::SLOTS * E * THREADS * sizeof(float), room = (size_t)(212 * 1024) / c.shape.ctas;
     a.stages = stage * 4 <= room ? 4 : (stage * 3 <= room ? 3 : 2);
-    int ctas = c.sm_count < kMaxSms ? c.sm_count : kMaxSms;
+    int ctas = (c.sm_count < kMaxSms ? c.sm_count : kMaxSms) * c.shape.ctas;
     if (cs > 1) {                       // a second wave of a few clusters would double the time
         int most = 0;
         if (int rc = resident_clusters((const void*)kernel, THREADS, stage * a.stages, cs, &most)) return rc;
@@ -703,27 +761,40 @@ int backward_as(BwdCall& c) {
     return launch_clusters("residual_norm_backward", kernel, a.parts * cs, THREADS, stage * a.stages, cs, c.st, a, cs);
 }
 
-template <int THREADS, int T, int E, bool POST, bool FULL>
+template <int THREADS, int T, bool POST, bool FULL, int VEC = 4>
 int backward_gate(BwdCall& c) {
-    if (c.gate == 0) return backward_as<THREADS, T, E, 4, BwdFlags<true, POST, FULL, 0>>(c);
-    if (c.gate == 1) return backward_as<THREADS, T, E, 4, BwdFlags<true, POST, FULL, 1>>(c);
-    return backward_as<THREADS, T, E, 4, BwdFlags<true, POST, FULL, 2>>(c);
+    if (c.gate == 0) return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 0>>(c);
+    if (c.gate == 1) return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 1>>(c);
+    return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 2>>(c);
+}
+template <int THREADS, int T, bool FULL, int VEC = 4>
+int backward_fast(BwdCall& c) {
+    return c.post ? backward_gate<THREADS, T, true, FULL, VEC>(c) : backward_gate<THREADS, T, false, FULL, VEC>(c);
+}
+template <int THREADS>
+int backward_lean(BwdCall& c) {
+    if (c.full) return backward_gate<THREADS, THREADS, false, true>(c);
+    return backward_fast<THREADS, THREADS, false>(c);
 }
 template <int THREADS, int T>
 int backward_narrow(BwdCall& c) {
-    // rows that cannot be read in 16-byte vectors, and calls without some operand or result
-    if (!c.vec) return backward_as<THREADS, T, 8, 1, BwdFlags<false, true, true, 1>>(c);
-    if (!c.fast) return backward_as<THREADS, T, 8, 4, BwdFlags<false, true, true, 1>>(c);
-    if (c.post) return c.full ? backward_gate<THREADS, T, 8, true, true>(c) : backward_gate<THREADS, T, 8, true, false>(c);
-    return c.full ? backward_gate<THREADS, T, 8, false, true>(c) : backward_gate<THREADS, T, 8, false, false>(c);
+    if (!c.fast) {
+        if (c.vec) return backward_as<THREADS, T, kBwdShare, 4, BwdFlags<false, true, true, 1>>(c);
+        return backward_as<THREADS, T, kBwdShare, 1, BwdFlags<false, true, true, 1>>(c);
+    }
+    if (!c.vec) {
+        if constexpr (T == 32 || T == 128 || T == 512) return backward_fast<THREADS, T, true, 1>(c);
+    }
+    return c.full ? backward_fast<THREADS, T, true>(c) : backward_fast<THREADS, T, false>(c);
 }
 
 }  // namespace
 
 size_t residual_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_groups, int64_t gate_width) {
     int64_t teams = 0, parts = 0;
-    for (const BwdShape& shape : {bwd_shape(cols, true), bwd_shape(cols, false)}) {
-        const int64_t t = bwd_teams(rows, shape, kMaxSms), p = ceil_div(t, (int64_t)(shape.threads / shape.team));
+    for (BwdKind kind : {kBwdLean, kBwdFullPre, kBwdFull, kBwdScalar, kBwdAny}) {
+        const BwdShape shape = bwd_shape(cols, kind);
+        const int64_t t = bwd_teams(rows, shape, (int64_t)kMaxSms * shape.ctas / shape.cs), p = ceil_div(t, (int64_t)(shape.threads / shape.team));
         teams = t > teams ? t : teams;
         parts = p > parts ? p : parts;
     }
@@ -785,7 +856,7 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
                 (!post || (g.post_weight && out.post_weight)) && (g.gate_mode == kGateNone || (g.gate_mode == kGateRow && out.gate));
     call.full = g.pre_kind == CTB_NORM_LAYER || g.post_kind == CTB_NORM_LAYER || out.pre_bias || out.post_bias || g.post_bias;
     call.gate = g.gate_mode == kGateNone ? 0 : (shared_gate ? 1 : 2);
-    call.shape = bwd_shape(g.cols, vec && call.fast && !call.full);
+    call.shape = bwd_shape(g.cols, !call.fast ? kBwdAny : (!vec ? kBwdScalar : (!call.full ? kBwdLean : (post ? kBwdFull : kBwdFullPre))));
     call.sm_count = di.sm_count;
     call.workspace = workspace;
     call.st = st;
@@ -796,8 +867,9 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     case 96: rc = backward_narrow<480, 96>(call); break;
     case 128: rc = backward_narrow<512, 128>(call); break;
     case 192: rc = backward_narrow<384, 192>(call); break;
-    case 256: rc = backward_narrow<512, 256>(call); break;
-    case 640: rc = post ? backward_gate<640, 640, 8, true, false>(call) : backward_gate<640, 640, 8, false, false>(call); break;
+    case 256: rc = call.shape.threads == 512 ? backward_narrow<512, 256>(call) : backward_gate<256, 256, true, true>(call); break;
+    case 320: rc = backward_lean<320>(call); break;
+    case 640: rc = backward_lean<640>(call); break;
     default: rc = backward_narrow<512, 512>(call);
     }
     if (rc) return rc;

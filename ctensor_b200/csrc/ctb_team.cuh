@@ -38,8 +38,7 @@ struct FoldMax {      // like fmaxf, ignores a NaN
 // of the fold in between.
 template <int THREADS, int N, typename S>
 struct TeamSlots {
-    S warps[2][THREADS / 32][N];
-    S peers[2][kMaxCluster][N];
+    S warps[2][kMaxCluster * (THREADS / 32)][N];         // entries of this CTA's warps, or of all warps of the cluster
 };
 
 // v[n] = fold over i < count of p[i * N + n], in every lane: lane l reads the entries l, l + 32, ... (all of
@@ -88,18 +87,18 @@ __device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& s
         return;
     }
     const int warp = threadIdx.x >> 5, team = threadIdx.x / T;
-    if (lane % (32 / N) == 0) sh.warps[turn][warp][lane / (32 / N)] = v[0];
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(T) : "memory");
-    lane_fold<OP, N>(v, &sh.warps[turn][team * (T / 32)][0], T / 32);
-    if (cs > 1) {
-        if ((int)threadIdx.x < cs) {
-            const uint32_t at = peer_shared(&sh.peers[turn][cluster_rank()][0], threadIdx.x);
-#pragma unroll
-            for (int n = 0; n < N; ++n) store_peer(at + n * (uint32_t)sizeof(S), v[n]);
-        }
+    if (T == THREADS && cs > 1) {
+        // every warp leaves its values with every CTA: one barrier for warps and CTAs together
+        const uint32_t rank = cluster_rank();
+        const S mine = __shfl_sync(0xffffffffu, v[0], (lane % N) * (32 / N));
+        for (int peer = lane / N; peer < cs; peer += 32 / N) store_peer(peer_shared(&sh.warps[turn][rank * (THREADS / 32) + warp][lane % N], peer), mine);
         __syncwarp();
         cluster_barrier();
-        lane_fold<OP, N>(v, &sh.peers[turn][0][0], cs);
+        lane_fold<OP, N>(v, &sh.warps[turn][0][0], cs * (THREADS / 32));
+    } else {
+        if (lane % (32 / N) == 0) sh.warps[turn][warp][lane / (32 / N)] = v[0];
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(T) : "memory");
+        lane_fold<OP, N>(v, &sh.warps[turn][team * (T / 32)][0], T / 32);
     }
     turn ^= 1;
 }
