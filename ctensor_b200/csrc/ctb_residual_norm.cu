@@ -120,7 +120,7 @@ __device__ __forceinline__ void row_statistics(const float (&v)[E], int kind, fl
 // Wide rows keep x in shared memory (each thread its own columns) until it is needed: 40 registers instead of
 // 59, so three CTAs of 512 threads share an SM and one row's folds hide behind the loads of two others.
 template <int THREADS, int T, int E, int VEC> constexpr bool kStageX = T == THREADS && E == 16 && VEC == 4;
-template <int THREADS, int T, int E, int VEC> constexpr int kForwardCtas = kStageX<THREADS, T, E, VEC> ? 1536 / THREADS : T == THREADS ? 1 : E == 32 ? 2 : 4;
+template <int THREADS, int T, int E, int VEC> constexpr int kForwardCtas = kStageX<THREADS, T, E, VEC> ? 1536 / THREADS : T == THREADS ? 2 : 4;
 
 template <int THREADS, int T, int E, int VEC>
 __global__ void __launch_bounds__(THREADS, (kForwardCtas<THREADS, T, E, VEC>))
@@ -227,6 +227,98 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
         }
     }
     if (stats && tid == 0 && rank == 0) *reinterpret_cast<float4*>(stats + row * 4) = st;
+}
+
+// RMS norms on both sides need one fold per row instead of two: with u = scale * gate * w_post * f and
+// X = x + scale * gate * b_post the stream is y = X + rstd_f * u, so
+//     sum(y^2) = sum(X^2) + 2 rstd_f sum(X u) + rstd_f^2 sum(u^2)
+// and all four sums (fp64) are known after one pass over x and f.  For rows of up to 2048 columns: [16384, 1536]
+// 69 us against 74; wider rows, which hold more of it per thread, lose ([4096, 4096] 60 against 52).
+template <int THREADS, int T, int E, int VEC>
+__global__ void __launch_bounds__(THREADS, 4)
+residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ y, float* __restrict__ h, float* __restrict__ stats) {
+    __shared__ TeamSlots<THREADS, 4, double> sh;
+    const int tid = threadIdx.x % T;
+    const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
+    if (row >= g.rows) return;                           // whole teams leave together
+    const int width = (int)g.cols;
+    int turn = 0;
+    float xv[E], u[E];
+    load_share<T, E, VEC>(xv, x.p + row * x.stride, width, tid);
+    load_share<T, E, VEC>(u, f.p + row * f.stride, width, tid);
+    const float* gate = g.gate.p + (int64_t)fast_div((uint32_t)row, g.by_gate_rows) * g.gate.stride;
+    const float one_gate = g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};                  // f^2, X^2, X u, u^2
+#pragma unroll
+    for (int i = 0; i < E / VEC; ++i) {
+        const int c = col_of<T, VEC>(i, tid);
+        if (c < width) {
+            float k[VEC], X[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) k[q] = one_gate;
+            if (g.gate_mode == kGateRow) {
+                load_part<T, VEC>(k, gate, c);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) k[q] = k[q] * g.scale;
+            }
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) X[q] = xv[i * VEC + q];
+            if (g.post_bias) {
+                float b[VEC];
+                load_part<T, VEC>(b, g.post_bias, c);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) xv[i * VEC + q] = X[q] = fmaf(k[q], b[q], X[q]);
+            }
+            if (g.post_weight) {
+                float w[VEC];
+                load_part<T, VEC>(w, g.post_weight, c);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) k[q] = k[q] * w[q];
+            }
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) {
+                const double fd = u[i * VEC + q], Xd = X[q];
+                u[i * VEC + q] = u[i * VEC + q] * k[q];
+                const double ud = u[i * VEC + q];
+                s[0] = fma(fd, fd, s[0]);
+                s[1] = fma(Xd, Xd, s[1]);
+                s[2] = fma(Xd, ud, s[2]);
+                s[3] = fma(ud, ud, s[3]);
+            }
+        }
+    }
+    team_fold<FoldSum, THREADS, T>(s, sh, turn, 1);
+    const float rf = __frsqrt_rn((float)(s[0] * g.inv_cols + (double)g.post_eps));
+    const double r = rf;
+    double sy = fma(r, fma(r, s[3], 2.0 * s[2]), s[1]);
+    if (sy < 0.0) sy = 0.0;
+    const float ry = __frsqrt_rn((float)(sy * g.inv_cols + (double)g.pre_eps));
+#pragma unroll
+    for (int i = 0; i < E / VEC; ++i) {
+        const int c = col_of<T, VEC>(i, tid);
+        if (c < width) {
+            float out[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) out[q] = fmaf(rf, u[i * VEC + q], xv[i * VEC + q]);
+            store_part<VEC>(y + row * g.cols, c, out);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) out[q] = out[q] * ry;
+            if (g.pre_weight) {
+                float w[VEC];
+                load_part<T, VEC>(w, g.pre_weight, c);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) out[q] = out[q] * w[q];
+            }
+            if (g.pre_bias) {
+                float w[VEC];
+                load_part<T, VEC>(w, g.pre_bias, c);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) out[q] = out[q] + w[q];
+            }
+            store_part<VEC>(h + row * g.cols, c, out);
+        }
+    }
+    if (stats && tid == 0) *reinterpret_cast<float4*>(stats + row * 4) = make_float4(0.0f, rf, 0.0f, ry);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------
@@ -692,11 +784,24 @@ int cluster_for(int64_t cols, int64_t per_cta) {
     return cs;
 }
 
+struct ForwardCall {
+    ResidualNormGeom g;
+    RowsIn x, f;
+    float *y, *h, *stats;
+    cudaStream_t st;
+};
 template <int THREADS, int T, int E, int VEC>
-int forward_as(const ResidualNormGeom& g, RowsIn x, RowsIn f, float* y, float* h, float* stats, cudaStream_t st) {
-    const int cs = T == THREADS ? cluster_for(g.cols, (int64_t)T * E) : 1;
-    return launch_clusters("residual_norm", residual_norm_kernel<THREADS, T, E, VEC>, ceil_div(g.rows, (int64_t)(THREADS / T)) * cs, THREADS, 0, cs, st,
-                           g, x, f, y, h, stats, cs);
+int forward_as(const ForwardCall& c) {
+    const char* who = "residual_norm";
+    const int64_t ctas = ceil_div(c.g.rows, (int64_t)(THREADS / T));
+    if constexpr (T < THREADS) {
+        if (c.f.p && c.g.post_kind == CTB_NORM_RMS && c.g.pre_kind == CTB_NORM_RMS)
+            return launch_clusters(who, residual_rms_kernel<THREADS, T, E, VEC>, ctas, THREADS, 0, 1, c.st, c.g, c.x, c.f, c.y, c.h, c.stats);
+        return launch_clusters(who, residual_norm_kernel<THREADS, T, E, VEC>, ctas, THREADS, 0, 1, c.st, c.g, c.x, c.f, c.y, c.h, c.stats, 1);
+    } else {
+        const int cs = cluster_for(c.g.cols, (int64_t)T * E);
+        return launch_clusters(who, residual_norm_kernel<THREADS, T, E, VEC>, ctas * cs, THREADS, 0, cs, c.st, c.g, c.x, c.f, c.y, c.h, c.stats, cs);
+    }
 }
 
 // How a row is dealt out in the backward pass: a team of `team` threads with kBwdShare columns each, `threads` to
@@ -809,18 +914,19 @@ int launch_residual_norm(const ResidualNormGeom& geom, RowsIn x, RowsIn f, float
     const bool vec = g.cols % 4 == 0 && rows_aligned(x) && rows_aligned(f) && (!y || is_aligned(y, 16)) && (!h || is_aligned(h, 16)) &&
                      is_aligned(g.post_weight, 16) && is_aligned(g.post_bias, 16) && is_aligned(g.pre_weight, 16) && is_aligned(g.pre_bias, 16) &&
                      (g.gate_mode != kGateRow || rows_aligned(g.gate));
+    const ForwardCall c{g, x, f, y, h, stats, st};
     if (!vec) {
-        if (g.cols <= 256) return forward_as<256, 32, 8, 1>(g, x, f, y, h, stats, st);
-        if (g.cols <= 2048) return forward_as<256, 128, 16, 1>(g, x, f, y, h, stats, st);
-        return forward_as<512, 512, 16, 1>(g, x, f, y, h, stats, st);
+        if (g.cols <= 256) return forward_as<256, 32, 8, 1>(c);
+        if (g.cols <= 2048) return forward_as<256, 128, 16, 1>(c);
+        return forward_as<512, 512, 16, 1>(c);
     }
-    if (g.cols <= 256) return forward_as<256, 32, 8, 4>(g, x, f, y, h, stats, st);
-    if (g.cols <= 512) return forward_as<256, 32, 16, 4>(g, x, f, y, h, stats, st);
-    if (g.cols <= 768) return forward_as<288, 96, 8, 4>(g, x, f, y, h, stats, st);
-    if (g.cols <= 1024) return forward_as<256, 128, 8, 4>(g, x, f, y, h, stats, st);
-    if (g.cols <= 2048) return forward_as<256, 128, 16, 4>(g, x, f, y, h, stats, st);
-    if (g.cols <= 4096) return forward_as<256, 256, 16, 4>(g, x, f, y, h, stats, st);
-    return forward_as<512, 512, 16, 4>(g, x, f, y, h, stats, st);
+    if (g.cols <= 256) return forward_as<256, 32, 8, 4>(c);
+    if (g.cols <= 512) return forward_as<256, 32, 16, 4>(c);
+    if (g.cols <= 768) return forward_as<288, 96, 8, 4>(c);
+    if (g.cols <= 1024) return forward_as<256, 128, 8, 4>(c);
+    if (g.cols <= 2048) return forward_as<256, 128, 16, 4>(c);
+    if (g.cols <= 4096) return forward_as<256, 256, 16, 4>(c);
+    return forward_as<512, 512, 16, 4>(c);
 }
 
 int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y, const float* stats, RowsIn grad_y, RowsIn grad_h,
