@@ -3,9 +3,13 @@
 // here: shapes are inferred, the output tensor is allocated, the C entry point is called, and
 // — because callers dereference storage on the CPU (src/neuralnet/loss.cpp:25,
 // src/core/autograd.cpp:97-155 of the reference) — the call waits for the kernel.
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <map>
+#include <memory>
 #include <mutex>
+#include <set>
 
 #include "include/ctb_host.h"
 #include "include/ops_dispatch.h"
@@ -241,6 +245,24 @@ int32_t* bad_label_flag(int index) {
     return (int32_t*)flags[index].get();
 }
 std::vector<size_t> broadcast_of(const Tensor& a, const Tensor& b) { return broadcast_shape(a, b); }
+// One double per device and host thread that a norm is written to (managed: the host reads it).
+double* norm_cell(int index) {
+    static thread_local std::vector<std::shared_ptr<void>> cells;
+    if ((int)cells.size() <= index) cells.resize(index + 1);
+    if (!cells[index]) {
+        void* p = nullptr;
+        check(ctb_alloc_managed(&p, sizeof(double), /*zero=*/1));
+        cells[index] = std::shared_ptr<void>(p, [](void*) {});           // lives as long as the thread's context
+    }
+    return (double*)cells[index].get();
+}
+ctb_view scalar_view(double* p) {
+    ctb_view v;
+    std::memset(&v, 0, sizeof v);
+    v.base = p;
+    v.dtype = CTB_F64;
+    return v;
+}
 }  // namespace
 
 Tensor cross_entropy(const Tensor& logits, const Tensor& labels, bool mean) {
@@ -340,6 +362,149 @@ void zero_grad(Tensor& param) {
     for (int d = 0; d < vz.ndim; ++d) vz.stride[d] = 0;
     check(ctb_copy_into(&vz, &vg, nullptr));
     after_op();
+}
+
+double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, double p) {
+    std::map<int, std::vector<ctb_view>> by_device;
+    std::set<const void*> seen;
+    for (const Tensor* param : params) {
+        if (!param || !has_grad(*param)) continue;
+        Tensor g;
+        g.impl = param->impl->grad;
+        if (g.numel() == 0 || !seen.insert(g.impl->data->data.get()).second) continue;
+        by_device[device_index_of(g.device())].push_back(view_of(g, "clip_grad_norm"));
+    }
+    if (by_device.empty()) by_device[g_device];
+    // one call per GPU; the norm comes back through managed memory
+    auto call = [&](int index, const std::vector<ctb_view>& views, double limit, bool scale) {
+        use_device(index);
+        double* out = norm_cell(index);
+        const ctb_view vn = scalar_view(out);
+        std::vector<const ctb_view*> list;
+        for (const ctb_view& v : views) list.push_back(&v);
+        if (scale) check(ctb_clip_grad_norm(list.data(), (int)list.size(), limit, p, nullptr, &vn, nullptr, 0, nullptr));
+        else check(ctb_grad_norm(list.data(), (int)list.size(), p, &vn, nullptr, 0, nullptr));
+        check(ctb_sync(nullptr));
+        return *out;
+    };
+    if (by_device.size() == 1) return call(by_device.begin()->first, by_device.begin()->second, max_norm, true);
+    if (!(max_norm >= 0.0)) throw std::runtime_error("clip_grad_norm: max_norm must not be negative or NaN");
+    double total = 0.0;
+    std::map<int, double> part;
+    for (const auto& d : by_device) {
+        const double n = part[d.first] = call(d.first, d.second, 0.0, false);
+        if (p == 2.0) total += n * n;
+        else if (p == 1.0) total += n;
+        else total = (std::isnan(total) || total >= n) ? total : n;
+    }
+    if (p == 2.0) total = std::sqrt(total);
+    if (total > max_norm && std::isfinite(total))
+        for (const auto& d : by_device) call(d.first, d.second, part[d.first] * (max_norm / total), true);
+    return total;
+}
+
+// ---- a transformer block's steps between its matrix products ----------------------------------------------
+namespace {
+// The optional tensors of one call as pointers to C views (null: absent), all on the device of the first.
+class OptionalViews {
+public:
+    OptionalViews(const Tensor& first, const char* who) : first_(first), who_(who) {}
+    const ctb_view* operator()(const Tensor& t) {
+        if (!t.impl) return nullptr;
+        if (t.device() != first_.device()) throw std::runtime_error(std::string(who_) + ": tensors must be on same device");
+        views_.push_back(std::make_unique<ctb_view>(view_of(t, who_)));
+        return views_.back().get();
+    }
+
+private:
+    const Tensor& first_;
+    const char* who_;
+    std::vector<std::unique_ptr<ctb_view>> views_;
+};
+ctb_score_rules c_rules(const ScoreRules& r, OptionalViews& view) {
+    ctb_score_rules c;
+    std::memset(&c, 0, sizeof c);
+    c.scale = r.scale;
+    c.cap = r.cap;
+    c.causal = r.causal ? 1 : 0;
+    c.query_start = view(r.query_start);
+    c.key_lengths = view(r.key_lengths);
+    c.prefix = view(r.prefix);
+    c.query_docs = view(r.query_docs);
+    c.key_docs = view(r.key_docs);
+    c.slopes = view(r.slopes);
+    return c;
+}
+ctb_residual_norm_params c_params(const ResidualNorm& p, OptionalViews& view) {
+    ctb_residual_norm_params c;
+    c.post_kind = (int32_t)p.post;
+    c.pre_kind = (int32_t)p.pre;
+    c.post_eps = p.post_eps;
+    c.pre_eps = p.pre_eps;
+    c.scale = p.scale;
+    c.post_weight = view(p.post_weight);
+    c.post_bias = view(p.post_bias);
+    c.pre_weight = view(p.pre_weight);
+    c.pre_bias = view(p.pre_bias);
+    return c;
+}
+// A fresh tensor shaped like `t`, or an absent one.
+Tensor output_like(const Tensor& t) { return t.impl ? new_output(t.shape(), DType::Float32, t.device()) : Tensor(); }
+}  // namespace
+
+Tensor score_softmax(const Tensor& scores, const ScoreRules& rules) {
+    if (!scores.impl) throw std::runtime_error("score_softmax: null input");
+    use_device_of(scores);
+    OptionalViews view(scores, "score_softmax");
+    const ctb_score_rules c = c_rules(rules, view);
+    Tensor out = output_like(scores);
+    check(ctb_score_softmax(view(scores), &c, view(out), nullptr));
+    after_op();
+    return out;
+}
+
+Tensor score_softmax_backward(const Tensor& grad, const Tensor& probs, const ScoreRules& rules, const Tensor& scores, Tensor* grad_slopes) {
+    if (!grad.impl || !probs.impl) throw std::runtime_error("score_softmax_backward: null input");
+    use_device_of(probs);
+    OptionalViews view(probs, "score_softmax_backward");
+    const ctb_score_rules c = c_rules(rules, view);
+    Tensor out = output_like(probs);
+    if (grad_slopes) *grad_slopes = output_like(rules.slopes);
+    check(ctb_score_softmax_backward(view(grad), view(probs), view(scores), &c, view(out), grad_slopes ? view(*grad_slopes) : nullptr, nullptr, 0, nullptr));
+    after_op();
+    return out;
+}
+
+ResidualNormResult residual_norm(const Tensor& x, const Tensor& f, const ResidualNorm& params, const Tensor& gate) {
+    if (!x.impl) throw std::runtime_error("residual_norm: null input");
+    use_device_of(x);
+    OptionalViews view(x, "residual_norm");
+    const ctb_residual_norm_params c = c_params(params, view);
+    ResidualNormResult r;
+    if (f.impl) r.y = output_like(x);
+    if (params.pre != NormKind::None) r.h = output_like(x);
+    std::vector<size_t> rows = x.shape();
+    if (rows.empty()) throw std::runtime_error("residual_norm: needs at least one dim");
+    rows.back() = 4;
+    r.stats = new_output(rows, DType::Float32, x.device());
+    check(ctb_residual_norm(view(x), view(f), view(gate), &c, view(r.y), view(r.h), view(r.stats), nullptr));
+    after_op();
+    if (!f.impl) r.y = x;
+    return r;
+}
+
+ResidualNormGrads residual_norm_backward(const Tensor& f, const ResidualNormResult& forward, const ResidualNorm& params, const Tensor& grad_y,
+                                         const Tensor& grad_h, const Tensor& gate) {
+    if (!forward.y.impl || !forward.stats.impl) throw std::runtime_error("residual_norm_backward: null input");
+    use_device_of(forward.y);
+    OptionalViews view(forward.y, "residual_norm_backward");
+    const ctb_residual_norm_params c = c_params(params, view);
+    ResidualNormGrads g{output_like(forward.y), f.impl ? output_like(forward.y) : Tensor(), output_like(gate), output_like(params.post_weight),
+                        output_like(params.post_bias), output_like(params.pre_weight), output_like(params.pre_bias)};
+    const ctb_residual_norm_grads cg{view(g.x), view(g.f), view(g.gate), view(g.post_weight), view(g.post_bias), view(g.pre_weight), view(g.pre_bias)};
+    check(ctb_residual_norm_backward(view(f), view(forward.y), view(gate), view(forward.stats), &c, view(grad_y), view(grad_h), &cg, nullptr, 0, nullptr));
+    after_op();
+    return g;
 }
 
 void set_backward_entry(std::function<void(Tensor&)> f) { g_backward = std::move(f); }

@@ -8,6 +8,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <set>
 
 #include "include/ctb_gen1.h"
 #include "include/opsmp.h"
@@ -205,6 +206,32 @@ void zero_grad(Tensor& param) {
     for (int d = 0; d < vz.ndim; ++d) vz.stride[d] = 0;
     check(ctb_copy_into(&vz, &vg, nullptr));
     after_op();
+}
+
+double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, double p) {
+    ensure_device();
+    // the norm comes back through managed memory
+    static thread_local double* cell = nullptr;
+    if (!cell) {
+        void* q = nullptr;
+        check(ctb_alloc_managed(&q, sizeof(double), /*zero=*/1));
+        cell = (double*)q;
+    }
+    std::vector<ctb_view> views;
+    std::set<const void*> seen;
+    for (const Tensor* param : params) {
+        if (!param || !has_grad(*param) || param->numel() == 0) continue;
+        if (seen.insert(param->impl->storage->grad.get()).second) views.push_back(grad_view_of(*param));
+    }
+    std::vector<const ctb_view*> list;
+    for (const ctb_view& v : views) list.push_back(&v);
+    ctb_view vn;
+    std::memset(&vn, 0, sizeof vn);
+    vn.base = cell;
+    vn.dtype = CTB_F64;
+    check(ctb_clip_grad_norm(list.data(), (int)list.size(), max_norm, p, nullptr, &vn, nullptr, 0, nullptr));
+    check(ctb_sync(nullptr));
+    return *cell;
 }
 
 void set_backward_entry(std::function<void(Tensor&)> f) { g_backward = std::move(f); }

@@ -67,6 +67,38 @@ Tensor cross_entropy_backward(const Tensor& logits, const Tensor& labels, double
 void div_backward(const Tensor& grad, const Tensor& a, const Tensor& b, Tensor* grad_a, Tensor* grad_b);
 Tensor tanh_backward(const Tensor& grad, const Tensor& t);
 
+// ---- a transformer block's steps between its matrix products --------------------------------------------
+// The C ABI's ctb_score_softmax, ctb_residual_norm and their gradients (include/ctb200.h has the formulas
+// and the layouts).  A Tensor that was never given a value stands for "absent".
+//   score_softmax           attention probabilities of scores [batch, heads, queries, keys]
+//   score_softmax_backward  gradient of the scores (`scores` is needed with a cap) and, if asked for, of the slopes
+//   residual_norm           y = x + scale * gate * N_post(f), h = N_pre(y); without f, y is x
+//   residual_norm_backward  the gradients of everything that went in (absent where there was no such input)
+struct ScoreRules {
+    double scale = 1.0, cap = 0.0;
+    bool causal = false;
+    Tensor query_start, key_lengths, prefix, query_docs, key_docs, slopes;
+};
+Tensor score_softmax(const Tensor& scores, const ScoreRules& rules);
+Tensor score_softmax_backward(const Tensor& grad, const Tensor& probs, const ScoreRules& rules, const Tensor& scores = Tensor(),
+                              Tensor* grad_slopes = nullptr);
+
+enum class NormKind : int { None = 0, Layer = 1, RMS = 2 };
+struct ResidualNorm {
+    NormKind post = NormKind::None, pre = NormKind::Layer;
+    double post_eps = 1e-5, pre_eps = 1e-5, scale = 1.0;
+    Tensor post_weight, post_bias, pre_weight, pre_bias;
+};
+struct ResidualNormResult {
+    Tensor y, h, stats;
+};
+struct ResidualNormGrads {
+    Tensor x, f, gate, post_weight, post_bias, pre_weight, pre_bias;
+};
+ResidualNormResult residual_norm(const Tensor& x, const Tensor& f, const ResidualNorm& params, const Tensor& gate = Tensor());
+ResidualNormGrads residual_norm_backward(const Tensor& f, const ResidualNormResult& forward, const ResidualNorm& params, const Tensor& grad_y,
+                                         const Tensor& grad_h, const Tensor& gate = Tensor());
+
 // ---- optimizer steps: what the host layer's train_utils.h is built on ----------------------------------
 // One fused in-place update of `param` from its gradient buffer on the GPU, with the arithmetic of
 // the reference's optimizer classes (src/neuralnet/train_utils.h:50-494), expression for expression.
@@ -83,6 +115,9 @@ std::shared_ptr<float> optimizer_state(const Tensor& param);
 void optimizer_step(OptimizerKind kind, Tensor& param, float* state1, float* state2, const OptimizerHyper& hyper, int step);
 // Clears the parameter's gradient buffer on the GPU (Optimizer::zero_grad, :37-46).
 void zero_grad(Tensor& param);
+// What Optimizer::clip_grad_norm does with its parameters (null ones and those without a gradient
+// buffer are passed over, a buffer that several share counts once; on several GPUs too).
+double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, double p);
 
 // Hook behind Tensor::backward(); the autograd library installs its backward(root) here.
 void set_backward_entry(std::function<void(Tensor&)> f);

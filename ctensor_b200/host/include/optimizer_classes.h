@@ -15,7 +15,8 @@
 // loader and its dashboard, which are not part of the operator path.
 #pragma once
 // Included by train_utils.h of either host layer, which defines CTB_OPT_NS (ctb_host or ctb_gen1:
-// the namespace with has_grad, storage_key, optimizer_state, optimizer_step and zero_grad) first.
+// the namespace with has_grad, storage_key, optimizer_state, optimizer_step, zero_grad and
+// clip_grad_norm) first.
 #ifndef CTB_OPT_NS
 #error "include train_utils.h, not optimizer_classes.h"
 #endif
@@ -47,6 +48,11 @@ public:
         for (Tensor* p : params)
             if (p) CTB_OPT_NS::zero_grad(*p);
     }
+
+    // Scales all gradients by max_norm / norm when the norm of all of them together, (sum |g|^p)^(1/p) with
+    // p = 1, 2 or infinity, is above max_norm and finite; returns the norm from before.  Call it
+    // between backward() and step().  (The reference has no gradient clipping.)
+    double clip_grad_norm(double max_norm, double p = 2.0) { return CTB_OPT_NS::clip_grad_norm(params, max_norm, p); }
 
 protected:
     using Kind = ctb_opt::Kind;
