@@ -89,6 +89,11 @@ __device__ __forceinline__ void read_own(float (&v)[VEC], const float* p) {
 }
 
 // ---- forward ------------------------------------------------------------------------------------------
+// v^-1/2, also where v is beyond Float32 or subnormal there (rows of 1e20, or of 1e-20 without an eps).
+__device__ __forceinline__ float inverse_root(double v) {
+    if (v > 1e-37 && v < 1e38) return __frsqrt_rn((float)v);
+    return (float)rsqrt(v);
+}
 // mean and rstd of a row from fp64 sums of v and v^2: one sum over the team instead of two, and no
 // cancellation that fp64 would notice until |mean| / sigma is about 1e6.
 template <int THREADS, int T, int E>
@@ -114,7 +119,7 @@ __device__ __forceinline__ void row_statistics(const float (&v)[E], int kind, fl
         var = fma(-m, m, var);
         if (var < 0.0) var = 0.0;
     }
-    *rstd = __frsqrt_rn((float)(var + (double)eps));
+    *rstd = inverse_root(var + (double)eps);
 }
 
 // Wide rows keep x in shared memory (each thread its own columns) until it is needed: 40 registers instead of
@@ -288,11 +293,11 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
         }
     }
     team_fold<FoldSum, THREADS, T>(s, sh, turn, 1);
-    const float rf = __frsqrt_rn((float)(s[0] * g.inv_cols + (double)g.post_eps));
+    const float rf = inverse_root(s[0] * g.inv_cols + (double)g.post_eps);
     const double r = rf;
     double sy = fma(r, fma(r, s[3], 2.0 * s[2]), s[1]);
     if (sy < 0.0) sy = 0.0;
-    const float ry = __frsqrt_rn((float)(sy * g.inv_cols + (double)g.pre_eps));
+    const float ry = inverse_root(sy * g.inv_cols + (double)g.pre_eps);
 #pragma unroll
     for (int i = 0; i < E / VEC; ++i) {
         const int c = col_of<T, VEC>(i, tid);

@@ -307,6 +307,18 @@ def test_residual_norm_large_mean(ct):
     check_norm(ct, x, f, vectors(g, 1, True, True, 1000), vectors(g, 1, True, True, 1000), None, 1.0, dy, dh)
 
 
+@pytest.mark.parametrize("cols", [20, 1000, 4100])
+@pytest.mark.parametrize("kind", [1, 2])
+def test_residual_norm_huge_and_tiny_rows(ct, cols, kind):
+    """Rows whose mean square is beyond Float32 on either side are normed like any other."""
+    g = gen(cols)
+    for size in (1e20, 1e-25):
+        x = randn(g, 3, cols) * size
+        _, h, _ = ct.residual_norm(x, None, ct.ResidualNorm(pre=kind, pre_eps=0.0))
+        want = ref.normed(x.double(), kind, None, None, 0.0)
+        within(h, want, ref.norm_bound(x.double(), kind, None, None, 0.0) + U * want.abs(), f"rows of {size}")
+
+
 def test_residual_norm_empty(ct):
     C = 12
     w = torch.ones(C, device=DEV)
@@ -496,6 +508,30 @@ def test_side_stream_graph_and_two_graphs_at_once(ct):
     assert torch.equal(graphs[0][1][0], ct.score_softmax(b["s"], a["rules"]))
 
 
+def test_clusters_in_a_graph(ct):
+    """Rows that take a cluster of CTAs, first met while capturing, on a stream of their own."""
+    g = gen(3)
+    C = 12300
+    x, f, dy, dh, w = randn(g, 2, 70, C), randn(g, 2, 70, C), randn(g, 2, 70, C), randn(g, 2, 70, C), randn(g, C)
+    norm = ct.ResidualNorm(pre=ct.NORM_RMS, pre_weight=w, post=ct.NORM_RMS, post_weight=w)
+    s, dp = randn(g, 1, 2, 1, 30000), randn(g, 1, 2, 1, 30000)
+    rules = ct.ScoreRules(slopes=torch.rand(2, device=DEV, generator=g))
+
+    def run():
+        y, h, stats = ct.residual_norm(x, f, norm)
+        n = ct.residual_norm_backward(f, y, stats, norm, grad_y=dy, grad_h=dh)
+        p = ct.score_softmax(s, rules)
+        return [y, h, n.x, n.f, n.pre_weight, n.post_weight, p, *ct.score_softmax_backward(dp, p, rules, want_slopes=True)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [t.clone() for t in outs]
+    assert all(torch.equal(a, b) for a, b in zip(got, run()))
+
+
 def test_a_training_step_of_a_block(ct):
     """Attention and a feed-forward product between pre and post norms, cross-entropy, every gradient, the
     clipping and an Adam step, against the same network differentiated in 64 bits."""
@@ -562,6 +598,7 @@ def test_a_training_step_of_a_block(ct):
     yd2 = yd + ref.normed((ref.normed(yd, 2, w["n2"], None, 1e-5) @ w["wu"]).relu(), 2, w["p2"], None, 1e-5)
     ld = torch.nn.functional.cross_entropy((ref.normed(yd2, 2, w["n3"], None, 1e-5) @ w["head"]).reshape(B * T, V), labels.long())
     ld.backward()
+    ld = ld.detach()
     assert abs(float(loss) - float(ld)) < 2e-5 * float(ld)      # the loss's own 1e-5, and fp32 products
     for name, t in grads.items():
         want = w[name].grad
