@@ -351,13 +351,13 @@ struct ResidualBwd {
     int64_t teams;
     int64_t parts;                  // rows of partial column sums: one per CTA (column slice)
     float* part;                    // [pre_weight, pre_bias, post_weight, post_bias, gate][parts][cols]
-    float* gate_part;               // [teams + groups][cols or 1]: slot team + group
+    float* gate_part;               // [teams + groups][cols or 1]: slot team + group; gate rows that lie in one team go out directly
     int32_t one_gate_row;           // all rows share one gate row: its sums go to `part`
 };
 
 // What a launch is specialised for.  A specialised kernel (FAST) has a pre norm with a weight, the gradient of y
 // and, if POST, a post norm with a weight; all of its gradients are wanted, the gate's for GATE != 0: 1 = a row
-// that rows share, 2 = a row for every row.  Otherwise every one of these is looked up at run time, the
+// that rows share, 2 = a row for every row, 3 = single values.  Otherwise every one of these is looked up at run time, the
 // flags then only say that the sums have a place: that took 640 instructions per warp and row where the
 // specialised kernel takes a third of it, and instructions, not bytes, bound narrow rows.
 // FULL: there may be LayerNorms and biases.
@@ -372,7 +372,7 @@ template <int THREADS, int T, int E, int VEC, typename F>
 __global__ void __launch_bounds__(THREADS, THREADS <= 320 ? 2 : 1)
 residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
     extern __shared__ __align__(16) float staged[];      // [stages][SLOTS][E][THREADS]
-    constexpr bool FAST = F::FAST, POST = F::POST, FULL = F::FULL, GATE = F::GATE == 1 || !FAST;
+    constexpr bool FAST = F::FAST, POST = F::POST, FULL = F::FULL, GATE = F::GATE == 1 || !FAST, SCALAR = F::GATE == 3;
     constexpr int SUMS = POST ? (FULL ? 8 : 4) : (FULL ? 2 : 1);
     __shared__ TeamSlots<THREADS, SUMS, float> sh;
     __shared__ TeamSlots<THREADS, 1, float> sh_gate;
@@ -400,17 +400,41 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
         if (GATE) gate_sum[e] = 0.0f;
     }
     float scalar_gate_sum = 0.0f;
+    // single gate values: a row's sum is left in shared memory by every warp (of the cluster) and added up by one
+    // thread after the next row's fold, whose barrier lies in between
+    auto leave = [&](float v, int parity) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) v = v + __shfl_xor_sync(0xffffffffu, v, off);
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0) {
+            float* at = &sh_gate.warps[parity][rank * (THREADS / 32) + warp][0];
+            if (T == THREADS && cs > 1) store_peer(peer_shared(at, 0), v);
+            else *at = v;
+        }
+    };
+    // its sum goes to the gate's gradient when a gate value's last row (in this team) has been added
+    auto collect = [&](int64_t row, int64_t of_group, int parity) {
+        if (tid != 0 || rank != 0) return;
+        const int first = T == THREADS ? 0 : (int)threadIdx.x / 32, count = (T == THREADS ? cs : 1) * (T / 32);
+        for (int i = 0; i < count; ++i) scalar_gate_sum = scalar_gate_sum + sh_gate.warps[parity][first + i][0];
+        const int64_t from = of_group * g.gate_rows, to = from + g.gate_rows;
+        if (row + 1 < hi && row + 1 < to) return;
+        if (from >= lo && to <= hi) a.out.gate[of_group] = scalar_gate_sum;
+        else a.gate_part[team + of_group] = scalar_gate_sum;
+        scalar_gate_sum = 0.0f;
+    };
     const bool pre = FAST || g.pre_kind != CTB_NORM_NONE, post = FAST ? POST : g.post_kind != CTB_NORM_NONE;
     const bool has_dy = FAST || a.in[kInDy].p, has_f = FAST ? POST || F::GATE != 0 : a.in[kInF].p != nullptr;
     const bool pre_weight = FAST || g.pre_weight, post_weight = FAST ? POST : g.post_weight != nullptr;
-    const bool row_gate = FAST ? F::GATE != 0 : g.gate_mode == kGateRow, staged_gate = FAST ? F::GATE == 2 : a.in[kInGate].p != nullptr;
+    const bool row_gate = FAST ? F::GATE == 1 || F::GATE == 2 : g.gate_mode == kGateRow, staged_gate = FAST ? F::GATE == 2 : a.in[kInGate].p != nullptr;
     const bool want_n = FAST ? F::GATE != 0 : g.gate_mode != kGateNone && a.out.gate;
     const bool shared_gate = FAST ? F::GATE == 1 : a.shared_gate != 0;
-    const bool scalar_gate = !FAST && g.gate_mode == kGateScalar && a.out.gate;
+    const bool scalar_gate = FAST ? SCALAR : g.gate_mode == kGateScalar && a.out.gate;
 
-    // Weights, and a gate row that rows share, stay in registers where those suffice (not beside the sums of two biases):
+    // Weights, and a gate row that rows share, stay in registers where those suffice (beside the sums of two biases only
+    // with 170 of them: [16384, 1536] 134 us without, 101 with):
     // with most of the SM's memory given to the ring, L1 is too small to serve them every row.
-    constexpr bool HOLD = FAST && (!FULL || !POST);
+    constexpr bool HOLD = FAST && (!FULL || !POST || THREADS <= 384);
     float w_pre[HOLD ? E : 1], w_post[HOLD && POST ? E : 1], w_gate[HOLD && F::GATE == 1 ? E : 1];
     auto hold = [&](float* v, const float* row) {
 #pragma unroll
@@ -487,7 +511,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
         stage_at = stage_at + STAGE == ring ? 0 : stage_at + STAGE;
         ahead_at = ahead_at + STAGE == ring ? 0 : ahead_at + STAGE;
         const float* gate = g.gate.p + group * g.gate.stride + (row_gate ? begin : 0);
-        const float one_gate = !FAST && g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
+        const float one_gate = (FAST ? SCALAR : g.gate_mode == kGateScalar) ? gate[0] * g.scale : g.scale;
         const float mean_f = FULL ? st.x : 0.0f, mean_y = FULL ? st.z : 0.0f;
 
         float e_[E], hat[E];                             // e = dy + rstd_y * a, and yhat
@@ -574,6 +598,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
             if constexpr (SUMS >= 4) { v[1] = s_kef; v[2] = s_kfy; v[3] = s_a; }
             if constexpr (SUMS == 8) { v[4] = s_ke; v[5] = s_k; v[6] = s_kf; v[7] = s_ky; }
             team_fold<FoldSum, THREADS, T>(v, sh, turn, cs);
+            if (SCALAR && row > lo) collect(row - 1, left == g.gate_rows ? group - 1 : group, (int)(row - 1 - lo) & 1);
             s_ay = v[0];
             if constexpr (SUMS == 2) s_a = v[1];
             if constexpr (SUMS >= 4) { s_kef = v[1]; s_kfy = v[2]; s_a = v[3]; }
@@ -658,14 +683,18 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                 if (FAST || a.out.f) store_part<VEC>(a.out.f, out, df);
             }
         }
-        if (scalar_gate) {
+        if constexpr (SCALAR) {
+            leave(scalar_sum, (int)(row - lo) & 1);
+        } else if (scalar_gate) {
             float one[1] = {scalar_sum};
             team_fold<FoldSum, THREADS, T>(one, sh_gate, gate_turn, cs);
             scalar_gate_sum = scalar_gate_sum + one[0];
         }
         // a gate that rows share: its sum so far goes out when the next row belongs to another gate row
         if (--left == 0 || row + 1 == hi) {
+            const bool whole = group * g.gate_rows >= lo && (group + 1) * g.gate_rows <= hi;
             if (shared_gate && !a.one_gate_row) {
+                float* to = (whole ? a.out.gate + group * g.cols : a.gate_part + (team + group) * g.cols) + begin;
 #pragma unroll
                 for (int i = 0; i < E / VEC; ++i) {
                     const int c = col_of<T, VEC>(i, tid);
@@ -675,15 +704,21 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                         part[q] = gate_sum[GATE ? i * VEC + q : 0];
                         gate_sum[GATE ? i * VEC + q : 0] = 0.0f;
                     }
-                    if (c < width) store_part<VEC>(a.gate_part + (team + group) * g.cols + begin, c, part);
+                    if (c < width) store_part<VEC>(to, c, part);
                 }
-            } else if (scalar_gate && tid == 0 && rank == 0) {
-                a.gate_part[team + group] = scalar_gate_sum;
+            } else if (!SCALAR && scalar_gate && tid == 0 && rank == 0) {
+                *(whole ? a.out.gate + group : a.gate_part + team + group) = scalar_gate_sum;
             }
-            scalar_gate_sum = 0.0f;
+            if (!SCALAR) scalar_gate_sum = 0.0f;
             ++group;
             left = g.gate_rows;
         }
+    }
+    if constexpr (SCALAR) {
+        if (T == THREADS && cs > 1) { __syncwarp(); cluster_barrier(); }
+        else if (T == 32) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / T), "r"(T) : "memory");
+        if (lo < hi) collect(hi - 1, fast_div((uint32_t)(hi - 1), g.by_gate_rows), (int)(hi - 1 - lo) & 1);
     }
     // column sums: the teams of a CTA add theirs in team order (through the ring, which is done with)
     auto put = [&](int at, const float* sum) {
@@ -726,7 +761,9 @@ struct FoldJobs {
     int64_t parts, teams, cols;
     const float* gate_part;
     float* gate;
-    int64_t groups, gate_width, gate_rows, rows;
+    int64_t gate_width, gate_rows, rows;
+    int32_t by_group;                   // gate jobs: one for every gate row, or (more gate rows than teams) for every two
+                                        // neighbouring teams whose rows share one
     int64_t vector_blocks, tiles, gate_tiles;
 };
 
@@ -745,12 +782,19 @@ residual_norm_fold_kernel(const __grid_constant__ FoldJobs j) {
         part = j.part[v];
         out = j.out[v];
     } else {
-        const int64_t group = (b - j.vector_blocks) / j.gate_tiles;
+        // team t has rows [rows * t / teams, rows * (t + 1) / teams)
+        int64_t group = (b - j.vector_blocks) / j.gate_tiles;
         tile = (b - j.vector_blocks) % j.gate_tiles;
-        // the teams whose rows meet the group's: team t has rows [rows * t / teams, rows * (t + 1) / teams)
+        if (!j.by_group) {
+            const int64_t t = group + 1, start = j.rows * t / j.teams;
+            group = start / j.gate_rows;
+            // a gate row begins here, or the one that does not began before the team ahead, whose job it then is
+            if (start % j.gate_rows == 0 || j.rows * (t - 1) / j.teams > group * j.gate_rows) return;
+        }
         const int64_t r0 = group * j.gate_rows, r1 = r0 + j.gate_rows - 1;
         first = ((r0 + 1) * j.teams - 1) / j.rows + group;
         last = ((r1 + 1) * j.teams - 1) / j.rows + group;
+        if (first == last) return;                       // one team's: it wrote the sum itself
         width = j.gate_width;
         part = j.gate_part;
         out = j.gate + group * width;
@@ -811,10 +855,10 @@ int forward_as(const ForwardCall& c) {
 
 // How a row is dealt out in the backward pass: a team of `team` threads with kBwdShare columns each, `threads` to
 // a CTA, `cs` CTAs to a row, `ctas` of them on an SM.  The column sums of a row's team live in registers, so
-// about 500 to 640 threads fit an SM.  Up to 2048 columns a CTA has several teams, so that one works while another
+// 384 to 640 threads fit an SM.  Up to 2048 columns a CTA has several teams, so that one works while another
 // waits in its fold; a wider row keeps the SM busy by itself (the next ones are on their way into shared
 // memory) as long as one CTA holds it.  Beyond that, clusters of small CTAs, two on an SM for the same reason:
-// 4096 rows of 8192 columns with RMS norms took 206 us with one cluster per SM pair.
+// 4096 rows of 8192 columns with RMS norms took 206 us with one cluster per SM pair, 139 with two.
 constexpr int kBwdShare = 8;
 struct BwdShape {
     int threads, team, cs, ctas;
@@ -823,8 +867,12 @@ struct BwdShape {
 // Rows that go element by element.  Everything else.
 enum BwdKind { kBwdLean, kBwdFullPre, kBwdFull, kBwdScalar, kBwdAny };
 BwdShape bwd_shape(int64_t cols, BwdKind kind) {
-    for (const BwdShape& s : {BwdShape{512, 32, 1, 1}, BwdShape{512, 64, 1, 1}, BwdShape{480, 96, 1, 1}, BwdShape{512, 128, 1, 1}, BwdShape{384, 192, 1, 1}, BwdShape{512, 256, 1, 1}})
-        if (cols <= s.team * kBwdShare && (kind != kBwdScalar || s.team == 32 || s.team == 128)) return s;
+    for (int team : {32, 64, 96, 128, 192, 256}) {
+        if (cols > team * kBwdShare || (kind == kBwdScalar && team != 32 && team != 128)) continue;
+        // four sums per column and the weights beside them: 170 registers a thread
+        if (kind == kBwdFull && team <= 192) return {384, team, 1, 1};
+        return {team == 96 ? 480 : (team == 192 ? 384 : 512), team, 1, 1};
+    }
     // (the sums of a LayerNorm and its bias leave a thread 128 registers where the CTA can be that small)
     if (cols <= 512 * kBwdShare && kind != kBwdLean) return {512, 512, 1, 1};
     const bool small = kind == kBwdLean || kind == kBwdFullPre;
@@ -875,7 +923,8 @@ template <int THREADS, int T, bool POST, bool FULL, int VEC = 4>
 int backward_gate(BwdCall& c) {
     if (c.gate == 0) return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 0>>(c);
     if (c.gate == 1) return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 1>>(c);
-    return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 2>>(c);
+    if (c.gate == 2) return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 2>>(c);
+    return backward_as<THREADS, T, kBwdShare, VEC, BwdFlags<true, POST, FULL, 3>>(c);
 }
 template <int THREADS, int T, bool FULL, int VEC = 4>
 int backward_fast(BwdCall& c) {
@@ -888,6 +937,7 @@ int backward_lean(BwdCall& c) {
 }
 template <int THREADS, int T>
 int backward_narrow(BwdCall& c) {
+    constexpr int FULL_THREADS = T <= 192 ? 384 : THREADS;
     if (!c.fast) {
         if (c.vec) return backward_as<THREADS, T, kBwdShare, 4, BwdFlags<false, true, true, 1>>(c);
         return backward_as<THREADS, T, kBwdShare, 1, BwdFlags<false, true, true, 1>>(c);
@@ -895,7 +945,8 @@ int backward_narrow(BwdCall& c) {
     if (!c.vec) {
         if constexpr (T == 32 || T == 128 || T == 512) return backward_fast<THREADS, T, true, 1>(c);
     }
-    return c.full ? backward_fast<THREADS, T, true>(c) : backward_fast<THREADS, T, false>(c);
+    if (!c.full) return backward_fast<THREADS, T, false>(c);
+    return c.post ? backward_gate<FULL_THREADS, T, true, true>(c) : backward_gate<THREADS, T, false, true>(c);
 }
 
 }  // namespace
@@ -964,9 +1015,9 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     call.vec = vec;
     call.post = post;
     call.fast = g.pre_kind != CTB_NORM_NONE && g.pre_weight && out.pre_weight && grad_y.p && f.p && out.x && out.f &&
-                (!post || (g.post_weight && out.post_weight)) && (g.gate_mode == kGateNone || (g.gate_mode == kGateRow && out.gate));
+                (!post || (g.post_weight && out.post_weight)) && (g.gate_mode == kGateNone || out.gate);
     call.full = g.pre_kind == CTB_NORM_LAYER || g.post_kind == CTB_NORM_LAYER || out.pre_bias || out.post_bias || g.post_bias;
-    call.gate = g.gate_mode == kGateNone ? 0 : (shared_gate ? 1 : 2);
+    call.gate = g.gate_mode == kGateNone ? 0 : (g.gate_mode == kGateScalar ? 3 : (shared_gate ? 1 : 2));
     call.shape = bwd_shape(g.cols, !call.fast ? kBwdAny : (!vec ? kBwdScalar : (!call.full ? kBwdLean : (post ? kBwdFull : kBwdFullPre))));
     call.sm_count = di.sm_count;
     call.workspace = workspace;
@@ -1001,17 +1052,17 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     j.cols = g.cols;
     j.tiles = ceil_div(g.cols, kFoldCols);
     j.vector_blocks = j.vectors * j.tiles;
-    const bool fold_gate = want_gate && !a.one_gate_row && (g.gate_mode == kGateScalar || g.gate_rows > 1);
+    const bool fold_gate = want_gate && !a.one_gate_row && g.gate_rows > 1;
     if (fold_gate) {
         j.gate_part = a.gate_part;
         j.gate = out.gate;
-        j.groups = groups;
+        j.by_group = groups < a.teams;
         j.gate_width = gate_width;
         j.gate_rows = g.gate_rows;
         j.rows = g.rows;
         j.gate_tiles = ceil_div(gate_width, kFoldCols);
     }
-    const int64_t blocks = j.vector_blocks + (fold_gate ? groups * j.gate_tiles : 0);
+    const int64_t blocks = j.vector_blocks + (fold_gate ? (j.by_group ? groups : a.teams - 1) * j.gate_tiles : 0);
     if (blocks == 0) return CTB_OK;
     if (blocks > 0x7FFFFFFFll) return set_error(CTB_ERR_LIMIT, "residual_norm_backward: too many gate rows for one launch");
     return launch_early(residual_norm_fold_kernel, (unsigned)blocks, kFoldThreads, st, j);
