@@ -864,20 +864,20 @@ struct BwdShape {
     int threads, team, cs, ctas;
 };
 // Specialised: RMS norms without biases; a LayerNorm or a bias before the next block; both norms, one of them such.
-// Rows that go element by element.  Everything else.
-enum BwdKind { kBwdLean, kBwdFullPre, kBwdFull, kBwdScalar, kBwdAny };
+// The last two for rows that go element by element.  Everything else.
+enum BwdKind { kBwdLean, kBwdFullPre, kBwdFull, kBwdScalarPre, kBwdScalar, kBwdAny };
 BwdShape bwd_shape(int64_t cols, BwdKind kind) {
     for (int team : {32, 64, 96, 128, 192, 256}) {
-        if (cols > team * kBwdShare || (kind == kBwdScalar && team != 32 && team != 128)) continue;
+        if (cols > team * kBwdShare || ((kind == kBwdScalarPre || kind == kBwdScalar) && team != 32 && team != 128)) continue;
         // four sums per column and the weights beside them: 170 registers a thread
-        if (kind == kBwdFull && team <= 192) return {384, team, 1, 1};
+        if ((kind == kBwdFull || kind == kBwdScalar) && team <= 192) return {384, team, 1, 1};
         return {team == 96 ? 480 : (team == 192 ? 384 : 512), team, 1, 1};
     }
     // (the sums of a LayerNorm and its bias leave a thread 128 registers where the CTA can be that small)
     if (cols <= 512 * kBwdShare && kind != kBwdLean) return {512, 512, 1, 1};
     const bool small = kind == kBwdLean || kind == kBwdFullPre;
     const int alone = small ? 640 : 512, in_cluster = small ? 320 : 256;
-    if (cols <= alone * kBwdShare) return {alone, alone, 1, 1};
+    if (cols <= 640 * kBwdShare && (small || kind == kBwdScalarPre)) return {640, 640, 1, 1};
     const int cs = cluster_for(cols, in_cluster * kBwdShare);
     if ((small || kind == kBwdFull) && cs <= kMaxCluster) return {in_cluster, in_cluster, cs, 2};
     return {alone, alone, cluster_for(cols, alone * kBwdShare), 1};
@@ -943,7 +943,7 @@ int backward_narrow(BwdCall& c) {
         return backward_as<THREADS, T, kBwdShare, 1, BwdFlags<false, true, true, 1>>(c);
     }
     if (!c.vec) {
-        if constexpr (T == 32 || T == 128 || T == 512) return backward_fast<THREADS, T, true, 1>(c);
+        if constexpr (T == 32 || T == 128 || T == 512) return c.post ? backward_gate<FULL_THREADS, T, true, true, 1>(c) : backward_gate<THREADS, T, false, true, 1>(c);
     }
     if (!c.full) return backward_fast<THREADS, T, false>(c);
     return c.post ? backward_gate<FULL_THREADS, T, true, true>(c) : backward_gate<THREADS, T, false, true>(c);
@@ -953,7 +953,7 @@ int backward_narrow(BwdCall& c) {
 
 size_t residual_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_groups, int64_t gate_width) {
     int64_t teams = 0, parts = 0;
-    for (BwdKind kind : {kBwdLean, kBwdFullPre, kBwdFull, kBwdScalar, kBwdAny}) {
+    for (BwdKind kind : {kBwdLean, kBwdFullPre, kBwdFull, kBwdScalarPre, kBwdScalar, kBwdAny}) {
         const BwdShape shape = bwd_shape(cols, kind);
         const int64_t t = bwd_teams(rows, shape, (int64_t)kMaxSms * shape.ctas / shape.cs), p = ceil_div(t, (int64_t)(shape.threads / shape.team));
         teams = t > teams ? t : teams;
@@ -1018,7 +1018,7 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
                 (!post || (g.post_weight && out.post_weight)) && (g.gate_mode == kGateNone || out.gate);
     call.full = g.pre_kind == CTB_NORM_LAYER || g.post_kind == CTB_NORM_LAYER || out.pre_bias || out.post_bias || g.post_bias;
     call.gate = g.gate_mode == kGateNone ? 0 : (g.gate_mode == kGateScalar ? 3 : (shared_gate ? 1 : 2));
-    call.shape = bwd_shape(g.cols, !call.fast ? kBwdAny : (!vec ? kBwdScalar : (!call.full ? kBwdLean : (post ? kBwdFull : kBwdFullPre))));
+    call.shape = bwd_shape(g.cols, !call.fast ? kBwdAny : (!vec ? (post ? kBwdScalar : kBwdScalarPre) : (!call.full ? kBwdLean : (post ? kBwdFull : kBwdFullPre))));
     call.sm_count = di.sm_count;
     call.workspace = workspace;
     call.st = st;
@@ -1031,7 +1031,7 @@ int launch_residual_norm_backward(const ResidualNormGeom& g, RowsIn f, RowsIn y,
     case 192: rc = backward_narrow<384, 192>(call); break;
     case 256: rc = call.shape.threads == 512 ? backward_narrow<512, 256>(call) : backward_gate<256, 256, true, true>(call); break;
     case 320: rc = backward_lean<320>(call); break;
-    case 640: rc = backward_lean<640>(call); break;
+    case 640: rc = vec ? backward_lean<640>(call) : backward_gate<640, 640, false, true, 1>(call); break;
     default: rc = backward_narrow<512, 512>(call);
     }
     if (rc) return rc;
