@@ -10,7 +10,9 @@
 // captured graph keeps its own list.
 //
 // Bound by HBM: 4 bytes per Float32 element for the norm and 8 more where the gradients have to be
-// scaled.  Squares and sums are fp64: a square of an fp32 value neither overflows nor vanishes there.
+// scaled (what the first launch read last is still in L2 and is scaled first).  Measured: 1.07 billion
+// gradients in 193 tensors, scaled out of place, 1984 us = 6.49 TB/s over 12 bytes per element; the norm of
+// 202 million alone 141 us = 5.8 TB/s; four small tensors 7.0 us, two launches.  Squares and sums are fp64: a square of an fp32 value neither overflows nor vanishes there.
 #include "ctb_clip.cuh"
 #include "ctb_team.cuh"
 

@@ -6,11 +6,16 @@
 //   dslope = -sum_j |pos - j| * p_j * (dp_j - D)
 //
 // Causal, prefix and length rules admit a run of keys [0, live); only the document rule is decided key by
-// key.  Keys outside are neither read nor evaluated, their results are written as zeros.
+// key.  Fours of keys without an admitted one are neither read nor evaluated, their results are written as
+// zeros ahead of the loads.
 //
 // Bound by HBM: 4 bytes per admitted score in, 4 per element out; backward 8 (12 with a cap) in, 4 out.
-// Rows that fit are held in the registers of a warp or a CTA and read once (ScoreRow kernels); longer rows,
-// and few rows that are long, are swept twice by a cluster of CTAs (second sweep from L2).
+// Rows that fit are held in the registers of part of a warp, a warp or a CTA and read once; longer rows are swept
+// twice by one or more CTAs (second sweep from L2), few long ones held by a cluster.  Measured (bytes that
+// have to move over time, share of the 6.54 TB/s of a copy): [8,12,1024,1024] causal forward 96 us, 6.3 TB/s (0.96),
+// backward 129 us, 6.25 (0.95); capped 102 us (0.91) and 180 us (0.85); packed documents, capped: 91 us (0.75),
+// instructions bound it (three quarters of the issue slots: a row that is nearly all zeros still looks at
+// every document number); [1,12,512,16384] 143 us (0.86); swept rows of 100000: 165 us (0.57), gradients 185 (0.76).
 #include "ctb_scores.cuh"
 #include "ctb_team.cuh"
 
@@ -649,8 +654,8 @@ int launch_scores(ScoreCall& c) {
     // columns to deal out: up to three more than the keys where rows do not start on 16 bytes
     const int64_t n = a.g.keys % 4 == 0 && is_aligned(a.out, 16) ? a.g.keys : a.g.keys + 3;
     // Up to 512 columns a team takes 16 bytes a lane and as few lanes as hold the row four to a lane (rows of 64
-    // keys with a warp each spent most instructions on finding their place: 21.8 us where this takes the figure
-    // in the design notes); wider forward rows eight fours a lane, backward rows, with two or three operands, four.
+    // keys with a warp each spent most instructions on finding their place: 98304 rows 21.8 us, so 8.0);
+    // wider forward rows eight fours a lane, backward rows, with two or three operands, four.
     c.cs = 1;
     if (n <= 32) return rows_as<256, 8, 1>(c);
     if (n <= 64) return rows_as<256, 8, 2>(c);
