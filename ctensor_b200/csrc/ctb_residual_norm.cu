@@ -242,7 +242,8 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
 // RMS norms on both sides need one fold per row instead of two: with u = scale * gate * w_post * f and
 // X = x + scale * gate * b_post the stream is y = X + rstd_f * u, so
 //     sum(y^2) = sum(X^2) + 2 rstd_f sum(X u) + rstd_f^2 sum(u^2)
-// and all four sums (fp64) are known after one pass over x and f.  For rows of up to 2048 columns: [16384, 1536]
+// and all four sums (fp64) are known after one pass over x and f.  Where the block's output cancels the stream to
+// less than a thousandth, those sums would lose what the norm magnifies: such a row takes the second fold.  For rows of up to 2048 columns: [16384, 1536]
 // 69 us against 74; wider rows, which hold more of it per thread, lose ([4096, 4096] 60 against 52).
 template <int THREADS, int T, int E, int VEC>
 __global__ void __launch_bounds__(THREADS, 4)
@@ -301,7 +302,18 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
     const float rf = inverse_root(s[0] * g.inv_cols + (double)g.post_eps);
     const double r = rf;
     double sy = fma(r, fma(r, s[3], 2.0 * s[2]), s[1]);
-    if (sy < 0.0) sy = 0.0;
+    if (sy < 1e-6 * s[1]) {                              // the same in every thread of the team
+        double square = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const double d = col_of<T, VEC>(e / VEC, tid) < width ? fmaf(rf, u[e], xv[e]) : 0.0f;
+            square = fma(d, d, square);
+        }
+        s[0] = square;
+        s[1] = s[2] = s[3] = 0.0;
+        team_fold<FoldSum, THREADS, T>(s, sh, turn, 1);
+        sy = s[0];
+    }
     const float ry = inverse_root(sy * g.inv_cols + (double)g.pre_eps);
 #pragma unroll
     for (int i = 0; i < E / VEC; ++i) {
@@ -364,7 +376,7 @@ struct ResidualBwd {
 // and, if POST, a post norm with a weight; all of its gradients are wanted, the gate's for GATE != 0: 1 = a row
 // that rows share, 2 = a row for every row, 3 = single values.  Otherwise every one of these is looked up at run time, the
 // flags then only say that the sums have a place: that took 640 instructions per warp and row where the
-// specialised kernel takes a third of it, and instructions, not bytes, bound narrow rows.
+// specialised kernel takes 360, and instructions, not bytes, bound narrow rows.
 // FULL: there may be LayerNorms and biases.
 template <bool FAST_, bool POST_, bool FULL_, int GATE_>
 struct BwdFlags {

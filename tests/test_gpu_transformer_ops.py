@@ -307,6 +307,16 @@ def test_residual_norm_large_mean(ct):
     check_norm(ct, x, f, vectors(g, 1, True, True, 1000), vectors(g, 1, True, True, 1000), None, 1.0, dy, dh)
 
 
+@pytest.mark.parametrize("cols", [200, 1000, 1024, 2040, 4096])
+@pytest.mark.parametrize("part", [1.0, 1.0 - 2.0 ** -12])
+def test_residual_norm_of_a_stream_that_cancels(ct, cols, part):
+    """The block takes back all, or nearly all, of the stream: the next norm magnifies what is left."""
+    g = gen(cols)
+    f = randn(g, 6, cols)
+    x = -part * f / torch.sqrt((f.double() ** 2).mean(-1, keepdim=True) + 1e-5).float()
+    check_norm(ct, x, f, (2, None, None), (2, None, None), None, 1.0, randn(g, 6, cols), randn(g, 6, cols))
+
+
 @pytest.mark.parametrize("cols", [20, 1000, 4100])
 @pytest.mark.parametrize("kind", [1, 2])
 def test_residual_norm_huge_and_tiny_rows(ct, cols, kind):
