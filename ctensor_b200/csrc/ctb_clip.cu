@@ -11,8 +11,9 @@
 //
 // Bound by HBM: 4 bytes per Float32 element for the norm and 8 more where the gradients have to be
 // scaled (what the first launch read last is still in L2 and is scaled first).  Measured: 1.07 billion
-// gradients in 193 tensors, scaled out of place, 1984 us = 6.49 TB/s over 12 bytes per element; the norm of
-// 202 million alone 141 us = 5.8 TB/s; four small tensors 7.0 us, two launches.  Squares and sums are fp64: a square of an fp32 value neither overflows nor vanishes there.
+// gradients in 193 tensors, scaled out of place, 1978 us = 6.51 TB/s over 12 bytes per element; the norm of
+// 202 million alone 122 us = 6.6 TB/s; four small tensors 6.3 us, two launches.  Squares and sums are fp64: a
+// square of an fp32 value neither overflows nor vanishes there.
 #include "ctb_clip.cuh"
 #include "ctb_team.cuh"
 
@@ -21,14 +22,17 @@ namespace ctb {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr int kClipLoads = 4;                            // 32-byte loads in flight per thread
+constexpr int kClipLoads = 8;                            // 32-byte loads in flight per thread
 constexpr int kClipVecBytes = 32;
-constexpr int kClipChunkBytes = kClipThreads * kClipLoads * kClipVecBytes;      // 32 KiB
-constexpr int kClipBlocksPerSm = 6;
+constexpr int kClipChunkBytes = kClipThreads * kClipLoads * kClipVecBytes;      // 64 KiB
+// Resident blocks: eight loads a thread and three blocks read 202 million gradients in 122 us, four loads and five or
+// six blocks in 130 and 140 (spilled sums), eight and four in 127.  The scaling pass, which stores as well, is
+// launched with four blocks an SM and its registers left free: bounding them to four spills (2034 us for 1.07 billion).
+constexpr int kNormBlocksPerSm = 3, kScaleBlocksPerSm = 4;
 constexpr int kClipMaxBlocks = 1024;                     // partials of one launch
 constexpr int kClipSmallTable = 128, kClipLargeTable = 1024;
 
-// Tensors of one launch.  Tensor t is cut into chunks of 32 KiB counted from its first element's
+// Tensors of one launch.  Tensor t is cut into chunks of 64 KiB counted from its first element's
 // address rounded down to 32 bytes, so that all vector accesses are aligned wherever it starts;
 // `first[t]` is its first chunk's number, first[count] the number of chunks.
 template <int N>
@@ -85,7 +89,7 @@ template <int N> __device__ __forceinline__ int clip_tensor_of(const ClipTable<N
 }
 
 template <int KIND, typename T, int N>
-__global__ void __launch_bounds__(kClipThreads, kClipBlocksPerSm)
+__global__ void __launch_bounds__(kClipThreads, kNormBlocksPerSm)
 clip_norm_kernel(const __grid_constant__ ClipTable<N> t, double* __restrict__ partials) {
     constexpr int VEC = ClipVec<T>::kElems;
     using V = Vec<T, VEC>;
@@ -239,8 +243,8 @@ int clip_fill(ClipTable<N>* table, const ClipTensor* list, int64_t count) {
 }
 
 // One block per SM slot, never more blocks than chunks (and at least one, which writes its partial).
-unsigned clip_grid(uint32_t chunks, int sm_count) {
-    int64_t g = (int64_t)sm_count * kClipBlocksPerSm;
+unsigned clip_grid(uint32_t chunks, int sm_count, int per_sm) {
+    int64_t g = (int64_t)sm_count * per_sm;
     if (g > kClipMaxBlocks) g = kClipMaxBlocks;
     if (g > chunks) g = chunks;
     return (unsigned)(g < 1 ? 1 : g);
@@ -260,7 +264,7 @@ template <int KIND, typename T, int N>
 int clip_launch_table(int phase, const ClipTensor* list, int64_t count, ClipCall& call) {
     ClipTable<N> table;
     if (int rc = clip_fill<T, N>(&table, list, count)) return rc;
-    const unsigned grid = clip_grid(table.first[count], call.sm_count);
+    const unsigned grid = clip_grid(table.first[count], call.sm_count, phase == 0 ? kNormBlocksPerSm : kScaleBlocksPerSm);
     if (phase == 0) {
         clip_norm_kernel<KIND, T, N><<<grid, kClipThreads, 0, call.st>>>(table, call.partials + call.total_partials);
         call.total_partials += (int)grid;
