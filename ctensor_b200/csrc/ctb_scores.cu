@@ -13,9 +13,9 @@
 // Rows that fit are held in the registers of part of a warp, a warp or a CTA and read once; longer rows are swept
 // twice by one or more CTAs (second sweep from L2), few long ones held by a cluster.  Measured (bytes that
 // have to move over time, share of the 6.54 TB/s of a copy): [8,12,1024,1024] causal forward 96 us, 6.3 TB/s (0.96),
-// backward 129 us, 6.25 (0.95); capped 102 us (0.91) and 180 us (0.85); packed documents, capped: 91 us (0.75),
+// backward 126 us, 6.4 (0.98); capped 100 us (0.93) and 176 us (0.87); five packed documents, capped: 84 us (0.81),
 // instructions bound it (three quarters of the issue slots: a row that is nearly all zeros still looks at
-// every document number); [1,12,512,16384] 143 us (0.86); swept rows of 100000: 165 us (0.57), gradients 185 (0.76).
+// every document number), gradients 130 us; [1,12,512,16384] 143 us (0.86); swept rows of 100000: 165 us (0.57), gradients 185 (0.76).
 #include "ctb_scores.cuh"
 #include "ctb_team.cuh"
 
@@ -205,12 +205,32 @@ __device__ __forceinline__ void score_slow(const ScoreGeom& g, float (&r)[4], co
 
 // A thread's fours of a row: four v has the columns (v * T + tid) * 4 - phase and on.  Which columns are
 // admitted is a comparison with `live` where rows are aligned and no documents are given, else kept as bits.
+// With documents few fours of a row may have an admitted key, anywhere in it: a warp then goes over those v that
+// have one in any of its lanes, the j-th of them held in the j-th registers, instead of over all with a test and a
+// branch each ([8,12,1024,1024] causal, capped, five packed documents: 91 us, so 84, gradients 155 and 130; all
+// keys in one document 97 and 101).
 template <int T, int NV, bool DOCS, bool ALIGNED>
 struct ScoreShare {
     static constexpr bool kBits = DOCS || !ALIGNED;
+    static constexpr bool kSparse = DOCS && NV > 2;
+    struct Four {                                        // of the v in `active`
+        int at;
+        uint32_t bits;
+        __device__ __forceinline__ int column() const { return at; }
+        __device__ __forceinline__ uint32_t four() const { return bits & 15u; }
+        __device__ __forceinline__ bool has(int k) const { return ((bits >> k) & 1u) != 0; }
+    };
+    struct FixedFour {
+        const ScoreShare& of;
+        int v;
+        __device__ __forceinline__ int column() const { return of.column(v); }
+        __device__ __forceinline__ uint32_t four() const { return (of.bits >> (4 * v)) & 15u; }
+        __device__ __forceinline__ bool has(int k) const { return kBits ? ((of.bits >> (4 * v + k)) & 1u) != 0 : of.rest > v * T * 4 + k; }
+    };
     int first;                          // column of the first four
     int rest;                           // admissible columns from there on
     uint32_t bits;
+    uint32_t active;                    // kSparse: the v with an admitted column in this warp
     // `from`: the first four of this CTA's slice of the row
     __device__ __forceinline__ void init(const ScoreDocs& docs, const ScorePlace& w, int from, int tid, int phase) {
         first = (from + tid) * 4 - phase;
@@ -231,36 +251,65 @@ struct ScoreShare {
 #pragma unroll
             for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, column(v)) << (4 * v);
         }
+        if (kSparse) {
+            uint32_t all = __reduce_or_sync(0xFFFFFFFFu, bits);
+            all |= all >> 1;
+            active = (all | all >> 2) & 0x11111111u;     // bit 4 v
+        }
+    }
+    // f(j, four) for the fours worked on, their values being the j-th.
+    template <typename F> __device__ __forceinline__ void each(F&& f) const {
+        if (kSparse) {
+            uint32_t left = active;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                if (!left) break;
+                const int at = __ffs(left) - 1;
+                left &= left - 1;
+                f(j, Four{first + at * T, bits >> at});
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (any(v)) f(v, FixedFour{*this, v});
+        }
     }
     __device__ __forceinline__ int column(int v) const { return first + v * T * 4; }
     __device__ __forceinline__ bool any(int v) const { return kBits ? ((bits >> (4 * v)) & 15u) != 0 : rest > v * T * 4; }
-    __device__ __forceinline__ bool has(int v, int k) const { return kBits ? ((bits >> (4 * v + k)) & 1u) != 0 : rest > v * T * 4 + k; }
-    // values of the fours that have an admitted column; others keep what they held
+    // values of the fours that have an admitted column; others are 0 or keep what they held
     __device__ __forceinline__ void load(float (&x)[NV][4], const float* row, bool aligned) const {
+        if (!kSparse && !ALIGNED) {                         // a branch round each four more costs 7 % on a row of 4097
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
+            for (int v = 0; v < NV; ++v) score_load(x[v], row, column(v), (bits >> (4 * v)) & 15u, aligned);
+            return;
+        }
+        each([&](int j, const auto& o) {
             if (ALIGNED) {
-                if (any(v)) {
-                    const Vec<float, 4> q = ldg_stream(reinterpret_cast<const Vec<float, 4>*>(row + column(v)));
+                if (kSparse) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) x[v][k] = q.v[k];
+                    for (int k = 0; k < 4; ++k) x[j][k] = 0.0f;
+                }
+                if (!kSparse || o.four()) {
+                    const Vec<float, 4> q = ldg_stream(reinterpret_cast<const Vec<float, 4>*>(row + o.column()));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[j][k] = q.v[k];
                 }
             } else {
-                score_load(x[v], row, column(v), (bits >> (4 * v)) & 15u, aligned);
+                score_load(x[j], row, o.column(), o.four(), aligned);
             }
-        }
+        });
     }
-    __device__ __forceinline__ void store(float* out, int v, int end, const float (&x)[4]) const {
-        if (ALIGNED) score_store_four(out + column(v), x);
-        else score_store(out, column(v), end, x);
+    __device__ __forceinline__ void store(float* out, int column, int end, const float (&x)[4]) const {
+        if (!ALIGNED) score_store(out, column, end, x);
+        else if (!kSparse || column < end) score_store_four(out + column, x);
     }
-    // Zeros into the fours without an admitted key, ahead of the loads: these stores need not wait for them.
+    // Zeros into the fours not worked on, ahead of the loads: these stores need not wait for them.
     __device__ __forceinline__ void zeros(float* out, int end) const {
         const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1                                         // unrolled, its addresses double the kernel's registers
         for (int v = 0; v < NV; ++v) {
             const int c0 = column(v);
-            if (!any(v) && c0 < end) store(out, v, end, zero);
+            if (!(kSparse ? (active >> (4 * v)) & 1u : any(v)) && c0 < end) store(out, c0, end, zero);
         }
     }
 };
@@ -288,47 +337,38 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     float t[NV][4];
     mine.load(t, s, score_phase(s) == phase);
     float m[1] = {-INFINITY};
+    mine.each([&](int j, const auto& o) {
+        score_logits<CAP>(a.g, w, t[j], o.column());
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (mine.any(v)) {
-            score_logits<CAP>(a.g, w, t[v], mine.column(v));
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                t[v][k] = mine.has(v, k) ? t[v][k] : -INFINITY;
-                m[0] = fmaxf(m[0], t[v][k]);
-            }
+        for (int k = 0; k < 4; ++k) {
+            t[j][k] = o.has(k) ? t[j][k] : -INFINITY;
+            m[0] = fmaxf(m[0], t[j][k]);
         }
-    }
+    });
     team_fold<FoldMax, THREADS, T>(m, sh, turn, cs);
     const float top = m[0] == -INFINITY ? 0.0f : m[0];
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    mine.each([&](int j, const auto&) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (mine.any(v)) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                t[v][k] = score_exp(t[v][k] - top);
-                part[k] = part[k] + t[v][k];
-            }
+        for (int k = 0; k < 4; ++k) {
+            t[j][k] = score_exp(t[j][k] - top);
+            part[k] = part[k] + t[j][k];
         }
-    }
+    });
     float z[1] = {(part[0] + part[1]) + (part[2] + part[3])};
     team_fold<FoldSum, THREADS, T>(z, sh, turn, cs);
     const float inv = z[0] == 0.0f ? 0.0f : __frcp_rn(z[0]);
     const bool usual = z[0] < INFINITY;                  // else NaN, which must not reach the masked columns
+    mine.each([&](int j, const auto& o) {
+        float p[4];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (mine.any(v)) {
-            float p[4];
+        for (int k = 0; k < 4; ++k) p[k] = t[j][k] * inv;
+        if (!usual) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) p[k] = t[v][k] * inv;
-            if (!usual) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) p[k] = mine.has(v, k) ? p[k] : 0.0f;
-            }
-            mine.store(out, v, span.end, p);
+            for (int k = 0; k < 4; ++k) p[k] = o.has(k) ? p[k] : 0.0f;
         }
-    }
+        mine.store(out, o.column(), span.end, p);
+    });
 }
 
 template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
@@ -357,42 +397,36 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     mine.load(dp, gr, score_phase(gr) == phase);
     if constexpr (CAP) mine.load(s, sr, score_phase(sr) == phase);
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    mine.each([&](int j, const auto& o) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (mine.any(v)) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (ALIGNED) {                           // whole fours were read: masked columns hold anything
-                    p[v][k] = mine.has(v, k) ? p[v][k] : 0.0f;
-                    dp[v][k] = mine.has(v, k) ? dp[v][k] : 0.0f;
-                    if constexpr (CAP) s[v][k] = mine.has(v, k) ? s[v][k] : 0.0f;
-                }
-                part[k] = fmaf(p[v][k], dp[v][k], part[k]);
+        for (int k = 0; k < 4; ++k) {
+            if (ALIGNED) {                               // whole fours were read: masked columns hold anything
+                p[j][k] = o.has(k) ? p[j][k] : 0.0f;
+                dp[j][k] = o.has(k) ? dp[j][k] : 0.0f;
+                if constexpr (CAP) s[j][k] = o.has(k) ? s[j][k] : 0.0f;
             }
+            part[k] = fmaf(p[j][k], dp[j][k], part[k]);
         }
-    }
+    });
     float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
     team_fold<FoldSum, THREADS, T>(d, sh, turn, cs);
     const bool usual = fabsf(d[0]) < INFINITY;           // else 0 * (0 - D) is NaN in the masked columns
     float slope_sum = 0.0f;
+    mine.each([&](int j, const auto& o) {
+        float r[4];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        if (mine.any(v)) {
-            float r[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                r[k] = p[v][k] * (dp[v][k] - d[0]);
-                if (!usual && !mine.has(v, k)) r[k] = 0.0f;
-            }
-            if (a.slope_part) {
-                const float from = (float)(mine.column(v) - w.centre);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) slope_sum = fmaf(fabsf(from + (float)k) + w.beyond, r[k], slope_sum);
-            }
-            score_slow<CAP>(a.g, r, s[CAP ? v : 0]);
-            mine.store(out, v, span.end, r);
+        for (int k = 0; k < 4; ++k) {
+            r[k] = p[j][k] * (dp[j][k] - d[0]);
+            if (!usual && !o.has(k)) r[k] = 0.0f;
         }
-    }
+        if (a.slope_part) {
+            const float from = (float)(o.column() - w.centre);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) slope_sum = fmaf(fabsf(from + (float)k) + w.beyond, r[k], slope_sum);
+        }
+        score_slow<CAP>(a.g, r, s[CAP ? j : 0]);
+        mine.store(out, o.column(), span.end, r);
+    });
     if (a.slope_part) {
         double sum[1] = {(double)slope_sum};
         team_fold<FoldSum, THREADS, T>(sum, sh_slope, turn, cs);
@@ -595,20 +629,25 @@ struct ScoreCall {
 };
 constexpr const char* kScoreName = "score_softmax";
 
-template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
+enum Ways { kForward = 1, kBackward = 2, kBoth = 3 };    // which kernels a shape is compiled for
+
+template <int THREADS, int T, int NV, int WAYS, bool CAP, bool DOCS, bool ALIGNED>
 int rows_with(const ScoreCall& c) {
     const int64_t blocks = ceil_div(c.a.rows, (int64_t)(THREADS / T)) * c.cs;
-    if (!c.backward) return launch_clusters(kScoreName, score_softmax_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, c.cs, c.st, c.a, c.cs);
-    return launch_clusters(kScoreName, score_softmax_backward_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, c.cs, c.st, c.a, c.cs);
+    if constexpr (WAYS & kBackward)
+        if (c.backward) return launch_clusters(kScoreName, score_softmax_backward_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, c.cs, c.st, c.a, c.cs);
+    if constexpr (WAYS & kForward)
+        return launch_clusters(kScoreName, score_softmax_kernel<THREADS, T, NV, CAP, DOCS, ALIGNED>, blocks, THREADS, 0, c.cs, c.st, c.a, c.cs);
+    return CTB_OK;                                       // not reached: the shapes below are chosen by direction
 }
-template <int THREADS, int T, int NV>
+template <int THREADS, int T, int NV, int WAYS>
 int rows_as(const ScoreCall& c) {
     if (c.cap) {
-        if (c.docs) return c.aligned ? rows_with<THREADS, T, NV, true, true, true>(c) : rows_with<THREADS, T, NV, true, true, false>(c);
-        return c.aligned ? rows_with<THREADS, T, NV, true, false, true>(c) : rows_with<THREADS, T, NV, true, false, false>(c);
+        if (c.docs) return c.aligned ? rows_with<THREADS, T, NV, WAYS, true, true, true>(c) : rows_with<THREADS, T, NV, WAYS, true, true, false>(c);
+        return c.aligned ? rows_with<THREADS, T, NV, WAYS, true, false, true>(c) : rows_with<THREADS, T, NV, WAYS, true, false, false>(c);
     }
-    if (c.docs) return c.aligned ? rows_with<THREADS, T, NV, false, true, true>(c) : rows_with<THREADS, T, NV, false, true, false>(c);
-    return c.aligned ? rows_with<THREADS, T, NV, false, false, true>(c) : rows_with<THREADS, T, NV, false, false, false>(c);
+    if (c.docs) return c.aligned ? rows_with<THREADS, T, NV, WAYS, false, true, true>(c) : rows_with<THREADS, T, NV, WAYS, false, true, false>(c);
+    return c.aligned ? rows_with<THREADS, T, NV, WAYS, false, false, true>(c) : rows_with<THREADS, T, NV, WAYS, false, false, false>(c);
 }
 
 template <bool CAP, bool DOCS>
@@ -657,23 +696,23 @@ int launch_scores(ScoreCall& c) {
     // keys with a warp each spent most instructions on finding their place: 98304 rows 21.8 us, so 8.0);
     // wider forward rows eight fours a lane, backward rows, with two or three operands, four.
     c.cs = 1;
-    if (n <= 32) return rows_as<256, 8, 1>(c);
-    if (n <= 64) return rows_as<256, 8, 2>(c);
-    if (n <= 128) return rows_as<256, 8, 4>(c);
-    if (n <= 256) return rows_as<256, 16, 4>(c);
-    if (n <= 512) return rows_as<256, 32, 4>(c);
-    if (n <= 1024) return c.backward ? rows_as<256, 64, 4>(c) : rows_as<256, 32, 8>(c);
-    if (n <= 2048) return c.backward ? rows_as<256, 128, 4>(c) : rows_as<256, 64, 8>(c);
+    if (n <= 32) return rows_as<256, 8, 1, kBoth>(c);
+    if (n <= 64) return rows_as<256, 8, 2, kBoth>(c);
+    if (n <= 128) return rows_as<256, 8, 4, kBoth>(c);
+    if (n <= 256) return rows_as<256, 16, 4, kBoth>(c);
+    if (n <= 512) return rows_as<256, 32, 4, kBoth>(c);
+    if (n <= 1024) return c.backward ? rows_as<256, 64, 4, kBackward>(c) : rows_as<256, 32, 8, kForward>(c);
+    if (n <= 2048) return c.backward ? rows_as<256, 128, 4, kBackward>(c) : rows_as<256, 64, 8, kForward>(c);
     // Few long rows: a cluster of CTAs holds each, as many as it takes to occupy the machine while each has 2048
     // columns.  (With rows enough, clusters cost more than they bring: forward, 6144 rows of 16384 keys, 1 CTA
     // 143 us, 2 268, 4 490; gradients 217 swept by one CTA, 361 held by four.)
     const int64_t most = c.backward ? 8192 : 16384;      // columns in the registers of one CTA
     while (c.cs < kMaxCluster && a.rows * c.cs * 2 <= c.sm_count && n / (c.cs * 2) >= 2048) c.cs *= 2;
-    if (c.cs > 1 && n <= most * c.cs) return c.backward ? rows_as<512, 512, 4>(c) : rows_as<512, 512, 8>(c);
+    if (c.cs > 1 && n <= most * c.cs) return c.backward ? rows_as<512, 512, 4, kBackward>(c) : rows_as<512, 512, 8, kForward>(c);
     c.cs = 1;
-    if (n <= 4096) return c.backward ? rows_as<256, 256, 4>(c) : rows_as<256, 128, 8>(c);
-    if (n <= 8192 && !c.backward) return rows_as<256, 256, 8>(c);
-    if (n <= most) return c.backward ? rows_as<512, 512, 4>(c) : rows_as<512, 512, 8>(c);
+    if (n <= 4096) return c.backward ? rows_as<256, 256, 4, kBackward>(c) : rows_as<256, 128, 8, kForward>(c);
+    if (n <= 8192 && !c.backward) return rows_as<256, 256, 8, kForward>(c);
+    if (n <= most) return c.backward ? rows_as<512, 512, 4, kBackward>(c) : rows_as<512, 512, 8, kForward>(c);
     return sweep(c);
 }
 
