@@ -12,6 +12,7 @@ library and a CUDA device and raises otherwise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 from dataclasses import dataclass
@@ -680,7 +681,9 @@ def _device_scope(index: int):
 
 
 def _stream_of(index: int) -> int:
-    return _torch().cuda.current_stream(index).cuda_stream
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # without a Stream object: 1.2 us less per call
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def _new_like(x, view):
@@ -689,9 +692,10 @@ def _new_like(x, view):
     if isinstance(x, DView):
         out = _new_out(x, x.shape)
         return out, _raw_view(out)
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if not x.is_contiguous():
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         return out, _raw_view(out)
+    out = torch.empty_like(x)
     v = View.from_buffer_copy(view)
     v.base = out.data_ptr()
     return out, v
@@ -702,13 +706,18 @@ def _address(cview):
     return None if cview is None else ctypes.addressof(cview)
 
 
+@functools.lru_cache(maxsize=None)
+def _cuda_device(index: int):
+    return _torch().device("cuda", index)
+
+
 def _scratch(nbytes: int, index: int):
     """(tensor, address, size) of one call's scratch, from torch's allocator: ordered on the current stream,
     and a captured graph's own when the call is captured."""
     if not nbytes:
         return None, None, 0
     torch = _torch()
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=_cuda_device(index))
     return ws, ws.data_ptr(), nbytes
 
 
@@ -860,7 +869,7 @@ def _grad_norm(grads, max_norm, p, out, norm):
     _on_device(dev, "grad_norm", (norm,))
     with _device_scope(dev):
         if norm is None:
-            norm = torch.empty(1, dtype=torch.float64 if grads.has_f64 else torch.float32, device=torch.device("cuda", dev))
+            norm = torch.empty(1, dtype=torch.float64 if grads.has_f64 else torch.float32, device=_cuda_device(dev))
         ws, at, nbytes = _scratch(lib().ctb_grad_norm_workspace_bytes(len(grads)), dev)
         if max_norm is None:
             check(lib().ctb_grad_norm(grads.c, len(grads), float(p), _raw_view(norm), at, nbytes, _stream_of(dev)))
