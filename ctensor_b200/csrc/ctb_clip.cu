@@ -12,7 +12,9 @@
 // Bound by HBM: 4 bytes per Float32 element for the norm and 8 more where the gradients have to be
 // scaled (what the first launch read last is still in L2 and is scaled first).  Measured: 1.07 billion
 // gradients in 193 tensors, scaled out of place, 1978 us = 6.51 TB/s over 12 bytes per element; the norm of
-// 202 million alone 122 us = 6.6 TB/s; four small tensors 6.3 us, two launches.  Squares and sums are fp64: a
+// 202 million alone 122 us = 6.6 TB/s; four small tensors 6.2 us, two launches; 196
+// tensors of 1 to 140000 values, side by side at every alignment, 10.7 us; 50 million values, the two sides at
+// different alignments, 131 us.  Squares and sums are fp64: a
 // square of an fp32 value neither overflows nor vanishes there.
 #include "ctb_clip.cuh"
 #include "ctb_team.cuh"
@@ -24,13 +26,16 @@ namespace {
 constexpr int kClipThreads = 256;
 constexpr int kClipLoads = 8;                            // 32-byte loads in flight per thread
 constexpr int kClipVecBytes = 32;
+constexpr int kClipRagged = 4;                           // and in a tensor's ragged first or last chunk
+constexpr int kClipApart = 16;                           // elements in flight per thread where two sides differ in alignment
 constexpr int kClipChunkBytes = kClipThreads * kClipLoads * kClipVecBytes;      // 64 KiB
 // Resident blocks: eight loads a thread and three blocks read 202 million gradients in 122 us, four loads and five or
 // six blocks in 130 and 140 (spilled sums), eight and four in 127.  The scaling pass, which stores as well, is
 // launched with four blocks an SM and its registers left free: bounding them to four spills (2034 us for 1.07 billion).
 constexpr int kNormBlocksPerSm = 3, kScaleBlocksPerSm = 4;
 constexpr int kClipMaxBlocks = 1024;                     // partials of one launch
-constexpr int kClipSmallTable = 128, kClipLargeTable = 1024;
+// Tables: every launch carries a whole one, 28 bytes an entry (300 tiny tensors with 1024 entries 11.5 us).
+constexpr int kClipSmallTable = 128, kClipMidTable = 384, kClipLargeTable = 1024;
 
 // Tensors of one launch.  Tensor t is cut into chunks of 64 KiB counted from its first element's
 // address rounded down to 32 bytes, so that all vector accesses are aligned wherever it starts;
@@ -71,6 +76,30 @@ template <int KIND> __device__ __forceinline__ double clip_block_fold(double v, 
 #pragma unroll
     for (int i = 1; i < kClipThreads / 32; ++i) r = clip_fold<KIND>(r, smem[i]);
     return r;
+}
+
+// The vector at `p`, zeros where that lies outside [lo, hi); and its way back.
+template <typename T> __device__ __forceinline__ Vec<T, ClipVec<T>::kElems> clip_load_some(const T* src, int64_t p, int64_t lo, int64_t hi) {
+    constexpr int VEC = ClipVec<T>::kElems;
+    Vec<T, VEC> v;
+    if (p >= lo && p + VEC <= hi) {
+        v = ldg_stream(reinterpret_cast<const Vec<T, VEC>*>(src + p));
+    } else {
+        const bool some = p + VEC > lo && p < hi;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v.v[k] = some && p + k >= lo && p + k < hi ? src[p + k] : (T)0;
+    }
+    return v;
+}
+template <typename T> __device__ __forceinline__ void clip_store_some(T* dst, int64_t p, int64_t lo, int64_t hi, const Vec<T, ClipVec<T>::kElems>& v) {
+    constexpr int VEC = ClipVec<T>::kElems;
+    if (p >= lo && p + VEC <= hi) {
+        stg_stream(reinterpret_cast<Vec<T, VEC>*>(dst + p), v);
+    } else if (p + VEC > lo && p < hi) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if (p + k >= lo && p + k < hi) dst[p + k] = v.v[k];
+    }
 }
 
 // The chunks of one block: [lo, hi).
@@ -117,18 +146,16 @@ clip_norm_kernel(const __grid_constant__ ClipTable<N> t, double* __restrict__ pa
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) acc[k] = clip_term<KIND>(acc[k], (double)v[i].v[k]);
         } else {                                                       // a tensor's ragged first or last chunk
+#pragma unroll 1
+            for (int64_t p = at; p < end; p += kClipRagged * kClipThreads * VEC) {
+                if (p >= chunk_end) break;
+                V v[kClipRagged];
 #pragma unroll
-            for (int i = 0; i < kClipLoads; ++i) {
-                const int64_t p = at + i * (kClipThreads * VEC);
-                if (p >= phase && p + VEC <= end) {
-                    const V v = ldg_stream(reinterpret_cast<const V*>(src + p));
+                for (int i = 0; i < kClipRagged; ++i) v[i] = clip_load_some<T>(src, p + i * (kClipThreads * VEC), phase, end);
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[k] = clip_term<KIND>(acc[k], (double)v.v[k]);
-                } else {
+                for (int i = 0; i < kClipRagged; ++i)
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k)
-                        if (p + k >= phase && p + k < end) acc[k] = clip_term<KIND>(acc[k], (double)src[p + k]);
-                }
+                    for (int k = 0; k < VEC; ++k) acc[k] = clip_term<KIND>(acc[k], (double)v[i].v[k]);
             }
         }
     }
@@ -193,8 +220,14 @@ clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const double* __restri
         const int64_t begin = (int64_t)(c - t.first[which]) * CHUNK;
         if (!together) {                                    // other alignment on the two sides: element by element
             const int64_t stop = begin + CHUNK < end ? begin + CHUNK : end;
-            for (int64_t p = begin + threadIdx.x; p < stop; p += kClipThreads)
-                if (p >= phase) dst[p] = clipped ? src[p] * factor : src[p];
+            for (int64_t p = begin + threadIdx.x; p < stop; p += kClipThreads * kClipApart) {
+                T v[kClipApart];
+#pragma unroll
+                for (int i = 0; i < kClipApart; ++i) v[i] = p + i * kClipThreads >= phase && p + i * kClipThreads < stop ? src[p + i * kClipThreads] : (T)0;
+#pragma unroll
+                for (int i = 0; i < kClipApart; ++i)
+                    if (p + i * kClipThreads >= phase && p + i * kClipThreads < stop) dst[p + i * kClipThreads] = clipped ? v[i] * factor : v[i];
+            }
             continue;
         }
         const int64_t at = begin + (int64_t)threadIdx.x * VEC;
@@ -209,12 +242,18 @@ clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const double* __restri
                 stg_stream(reinterpret_cast<V*>(dst + at + i * (kClipThreads * VEC)), v[i]);
             }
         } else {
+#pragma unroll 1
+            for (int64_t p = at; p < end; p += kClipRagged * kClipThreads * VEC) {
+                if (p >= begin + CHUNK) break;
+                V v[kClipRagged];                           // loads ahead of stores: these may be to the same tensor
 #pragma unroll
-            for (int i = 0; i < kClipLoads; ++i) {
-                const int64_t p = at + i * (kClipThreads * VEC);
+                for (int i = 0; i < kClipRagged; ++i) v[i] = clip_load_some<T>(src, p + i * (kClipThreads * VEC), phase, end);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    if (p + k >= phase && p + k < end) dst[p + k] = src[p + k] * factor;
+                for (int i = 0; i < kClipRagged; ++i) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) v[i].v[k] = v[i].v[k] * factor;
+                    clip_store_some<T>(dst, p + i * (kClipThreads * VEC), phase, end, v[i]);
+                }
             }
         }
     }
@@ -282,6 +321,7 @@ int clip_phase(int phase, const ClipTensor* list, int64_t count, ClipCall& call)
     for (int64_t at = 0; at < count; at += kClipLargeTable) {
         const int64_t n = count - at < kClipLargeTable ? count - at : kClipLargeTable;
         const int rc = n <= kClipSmallTable ? clip_launch_table<KIND, T, kClipSmallTable>(phase, list + at, n, call)
+                       : n <= kClipMidTable ? clip_launch_table<KIND, T, kClipMidTable>(phase, list + at, n, call)
                                             : clip_launch_table<KIND, T, kClipLargeTable>(phase, list + at, n, call);
         if (rc) return rc;
     }

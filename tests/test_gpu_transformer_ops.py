@@ -419,6 +419,32 @@ def test_clip_starts_at_every_phase(ct):
             assert torch.equal(flat[:at], keep[:at]) and torch.equal(flat[at + n:], keep[at + n:])
 
 
+@pytest.mark.parametrize("count", [128, 129, 384, 385, 1024, 1025])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_clip_many_ragged_tensors_side_by_side(ct, count, dtype):
+    """Views of one buffer, so at every phase, up to a little more than the longest list of a launch and up to
+    two stretches of whole vectors; in place and out of place, at the same and at another phase."""
+    g = gen(count)
+    half = U if dtype == torch.float32 else 2.0 ** -53
+    slack = 64 * 2.0 ** -53
+    lengths = [(1, 3, 8, 31, 1023, 8191, 8192, 8193, 16384, 16385, 24577, 33001)[(7 * i) % 12 if i % 9 == 0 else i % 5] for i in range(count)]
+    flat = torch.randn(sum(lengths), device=DEV, generator=g, dtype=dtype)
+    views = lambda buf, lead: list(buf[lead:lead + flat.numel()].split(lengths))
+    total = norm_of([flat], 2)
+    want = flat.double() / 4
+    for lead in (0, 3):
+        target = torch.full((flat.numel() + 8,), 5.0, device=DEV, dtype=dtype)
+        n = ct.clip_grad_norm(views(flat, 0), total / 4, out=views(target, lead))
+        assert abs(float(n) - total) <= (half + slack) * total
+        within(target[lead:lead + flat.numel()], want, (2.1 * half + slack) * want.abs(), "out of place")
+        assert bool((target[:lead] == 5).all()) and bool((target[lead + flat.numel():] == 5).all())
+    keep = flat.clone()
+    ct.clip_grad_norm(views(flat, 0), total * 2)
+    assert torch.equal(flat, keep)
+    ct.clip_grad_norm(views(flat, 0), total / 4)
+    within(flat, want, (2.1 * half + slack) * want.abs(), "in place")
+
+
 def test_clip_mixed_types_permuted_views_and_one_tensor_twice(ct):
     g = gen(9)
     a, b = randn(g, 40, 50).t(), randn(g, 30, 20).double()
