@@ -13,7 +13,7 @@
 // Rows that fit are held in the registers of part of a warp, a warp or a CTA and read once; longer rows are swept
 // twice by one or more CTAs (second sweep from L2), few long ones held by a cluster.  Measured (bytes that
 // have to move over time, share of the 6.54 TB/s of a copy): [8,12,1024,1024] causal forward 96 us, 6.3 TB/s (0.96),
-// backward 126 us, 6.4 (0.98); capped 100 us (0.93) and 176 us (0.87); five packed documents, capped: 84 us (0.81),
+// backward 126 us, 6.4 (0.98); capped 100 us (0.93) and 155 us (0.99); five packed documents, capped: 84 us (0.81),
 // instructions bound it (three quarters of the issue slots: a row that is nearly all zeros still looks at
 // every document number), gradients 130 us; [1,12,512,16384] 143 us (0.86); swept rows of 100000: 165 us (0.57), gradients 185 (0.76).
 #include "ctb_scores.cuh"
@@ -125,8 +125,9 @@ __device__ __forceinline__ ScoreDocs score_docs(const ScoreArgs& a, const ScoreP
     return d;
 }
 
-// The admitted ones of the columns c0 .. c0 + 3, as bits.
-template <bool DOCS>
+// The admitted ones of the columns c0 .. c0 + 3, as bits.  HELD: for a row in registers (a swept row has none to
+// spare: gradients of 16384 keys 141 us, so 203).
+template <bool DOCS, bool HELD>
 __device__ __forceinline__ uint32_t score_admitted(const ScoreDocs& docs, const ScorePlace& w, int c0) {
     const int hi = min(max(w.live - c0, 0), 4), lo = min(max(-c0, 0), 4);
     uint32_t bits = (15u >> (4 - hi)) & (15u << lo);
@@ -135,10 +136,19 @@ __device__ __forceinline__ uint32_t score_admitted(const ScoreDocs& docs, const 
             const int4 d = *reinterpret_cast<const int4*>(docs.p + c0);
             bits = (uint32_t)(d.x == w.doc) | (uint32_t)(d.y == w.doc) << 1 | (uint32_t)(d.z == w.doc) << 2 | (uint32_t)(d.w == w.doc) << 3;
         } else {
+            if (HELD) {                                  // loads ahead of comparisons
+                int d[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if ((bits >> k) & 1u)
-                    if (docs.p[(int64_t)(c0 + k) * docs.si] != w.doc) bits &= ~(1u << k);
+                for (int k = 0; k < 4; ++k) d[k] = (bits >> k) & 1u ? docs.p[(int64_t)(c0 + k) * docs.si] : w.doc;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (d[k] != w.doc) bits &= ~(1u << k);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if ((bits >> k) & 1u)
+                        if (docs.p[(int64_t)(c0 + k) * docs.si] != w.doc) bits &= ~(1u << k);
+            }
         }
     }
     return bits;
@@ -249,7 +259,7 @@ struct ScoreShare {
             }
         } else if (kBits) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS>(docs, w, column(v)) << (4 * v);
+            for (int v = 0; v < NV; ++v) bits |= score_admitted<DOCS, true>(docs, w, column(v)) << (4 * v);
         }
         if (kSparse) {
             uint32_t all = __reduce_or_sync(0xFFFFFFFFu, bits);
@@ -371,8 +381,11 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     });
 }
 
+// Registers: 64 with a cap or ragged rows, 48 else; a spilled word or two costs less than a quarter of the rows in
+// flight (capped [8,12,1024,1024]: 176 us, so 155; CTAs of 512, one or two an SM: [2,8,1024,8192] 420 and 293).
+// With documents the compiler's own choice is the better one (0: no bound; 75 us at [64,12,256,256], 91 with one).
 template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : DOCS ? 0 : CAP || !ALIGNED ? 4 : 5)
 score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     const int cs = T == 512 ? ctas : 1;                  // only whole CTAs of 512 threads come in clusters
     static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
@@ -469,7 +482,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
-            bits[u] = at < live_end ? score_admitted<DOCS>(docs, w, (int)(at * 4) - phase) : 0u;
+            bits[u] = at < live_end ? score_admitted<DOCS, false>(docs, w, (int)(at * 4) - phase) : 0u;
         }
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
@@ -509,7 +522,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
-            bits[u] = at < live_end ? score_admitted<DOCS>(docs, w, (int)(at * 4) - phase) : 0u;
+            bits[u] = at < live_end ? score_admitted<DOCS, false>(docs, w, (int)(at * 4) - phase) : 0u;
         }
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
@@ -553,7 +566,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
             const int c0 = (int)(at * 4) - phase;
-            const uint32_t bits = at < live_end ? score_admitted<DOCS>(docs, w, c0) : 0u;
+            const uint32_t bits = at < live_end ? score_admitted<DOCS, false>(docs, w, c0) : 0u;
             score_load(p[u], pr, c0, bits, p_aligned);
             score_load(dp[u], gr, c0, bits, g_aligned);
         }
@@ -572,7 +585,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
         for (int u = 0; u < kSweepBatch; ++u) {
             const int64_t at = f + (int64_t)u * kSweepThreads;
             const int c0 = (int)(at * 4) - phase;
-            bits[u] = at < live_end ? score_admitted<DOCS>(docs, w, c0) : 0u;
+            bits[u] = at < live_end ? score_admitted<DOCS, false>(docs, w, c0) : 0u;
             score_load(p[u], pr, c0, bits[u], p_aligned);
             score_load(dp[u], gr, c0, bits[u], g_aligned);
             if (CAP) score_load(s[u], sr, c0, bits[u], s_aligned);
@@ -655,13 +668,19 @@ int sweep_with(const ScoreCall& c, int cs) {
     if (c.backward) return launch_clusters(kScoreName, score_softmax_backward_sweep_kernel<CAP, DOCS>, c.a.rows * cs, kSweepThreads, 0, cs, c.st, c.a, cs);
     return launch_clusters(kScoreName, score_softmax_sweep_kernel<CAP, DOCS>, c.a.rows * cs, kSweepThreads, 0, cs, c.st, c.a, cs);
 }
-// CTAs per row: until what the resident CTAs (two per SM) read twice takes half of L2's 126 MB, for rows longer
-// than that would be read from HBM twice (12 heads, gradients of 64 queries x 100000 keys: 1 CTA 229 us, 4 188, 8 219;
-// 512 x 16384: 1 CTA 217, 2 246); or, with few rows, until the machine is occupied while each CTA has 4096 keys.
-int sweep(const ScoreCall& c) {
+// CTAs per row beyond what one CTA holds: until what the resident CTAs (two per SM) read twice takes half of L2's
+// 126 MB, for rows longer than that would be read from HBM twice (12 heads, gradients of 64 queries x 100000 keys: 1
+// CTA 229 us, 4 188, 8 219; 512 x 16384: 1 CTA 217, 2 246); or, with few rows, until the last round of CTAs is
+// at least four fifths full while each CTA has 4096 keys.
+int sweep_ctas(const ScoreCall& c) {
     const int64_t row_bytes = c.a.g.keys * 4 * (c.backward ? (c.cap ? 3 : 2) : 1);
+    const int64_t slots = 2 * c.sm_count;
+    auto uneven = [&](int64_t ctas) { return ceil_div(ctas, slots) * slots * 4 > ctas * 5; };
     int cs = 1;
-    while (cs < kMaxCluster && (row_bytes / cs * 2 * c.sm_count > (int64_t(64) << 20) || (c.a.rows * cs < 2 * c.sm_count && c.a.g.keys / (2 * cs) >= 4096))) cs *= 2;
+    while (cs < kMaxCluster && (row_bytes / cs * slots > (int64_t(64) << 20) || (uneven(c.a.rows * cs) && c.a.g.keys / (2 * cs) >= 4096))) cs *= 2;
+    return cs;
+}
+int sweep(const ScoreCall& c, int cs) {
     if (c.cap) return c.docs ? sweep_with<true, true>(c, cs) : sweep_with<true, false>(c, cs);
     return c.docs ? sweep_with<false, true>(c, cs) : sweep_with<false, false>(c, cs);
 }
@@ -713,7 +732,10 @@ int launch_scores(ScoreCall& c) {
     if (n <= 4096) return c.backward ? rows_as<256, 256, 4, kBackward>(c) : rows_as<256, 128, 8, kForward>(c);
     if (n <= 8192 && !c.backward) return rows_as<256, 256, 8, kForward>(c);
     if (n <= most) return c.backward ? rows_as<512, 512, 4, kBackward>(c) : rows_as<512, 512, 8, kForward>(c);
-    return sweep(c);
+    // Rows that would be swept by clusters are held by them if they fit.
+    c.cs = sweep_ctas(c);
+    if (c.cs > 1 && n <= most * c.cs) return c.backward ? rows_as<512, 512, 4, kBackward>(c) : rows_as<512, 512, 8, kForward>(c);
+    return sweep(c, c.cs);
 }
 
 }  // namespace
