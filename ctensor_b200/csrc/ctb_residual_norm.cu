@@ -239,10 +239,11 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
     if (stats && tid == 0 && rank == 0) *reinterpret_cast<float4*>(stats + row * 4) = st;
 }
 
-// RMS norms on both sides need one fold per row instead of two: with u = scale * gate * w_post * f and
-// X = x + scale * gate * b_post the stream is y = X + rstd_f * u, so
-//     sum(y^2) = sum(X^2) + 2 rstd_f sum(X u) + rstd_f^2 sum(u^2)
-// and all four sums (fp64) are known after one pass over x and f.  Where the block's output cancels the stream to
+// RMS norms on both sides need one fold per row instead of two: with u = scale * gate * w_post * f the stream is
+// y = x + rstd_f * u, so
+//     sum(y^2) = sum(x^2) + 2 rstd_f sum(x u) + rstd_f^2 sum(u^2)
+// and all four sums (fp64) are known after one pass over x and f.  (A bias behind the first norm would have to be
+// rounded into x before that norm is known, one rounding more; such rows take the general kernel.)  Where the block's output cancels the stream to
 // less than a thousandth, those sums would lose what the norm magnifies: such a row takes the second fold.  For rows of up to 2048 columns: [16384, 1536]
 // 69 us against 74; wider rows, which hold more of it per thread, lose ([4096, 4096] 60 against 52).
 template <int THREADS, int T, int E, int VEC>
@@ -259,26 +260,18 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
     load_share<T, E, VEC>(u, f.p + row * f.stride, width, tid);
     const float* gate = g.gate.p + (int64_t)fast_div((uint32_t)row, g.by_gate_rows) * g.gate.stride;
     const float one_gate = g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
-    double s[4] = {0.0, 0.0, 0.0, 0.0};                  // f^2, X^2, X u, u^2
+    double s[4] = {0.0, 0.0, 0.0, 0.0};                  // f^2, x^2, x u, u^2
 #pragma unroll
     for (int i = 0; i < E / VEC; ++i) {
         const int c = col_of<T, VEC>(i, tid);
         if (c < width) {
-            float k[VEC], X[VEC];
+            float k[VEC];
 #pragma unroll
             for (int q = 0; q < VEC; ++q) k[q] = one_gate;
             if (g.gate_mode == kGateRow) {
                 load_part<T, VEC>(k, gate, c);
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) k[q] = k[q] * g.scale;
-            }
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) X[q] = xv[i * VEC + q];
-            if (g.post_bias) {
-                float b[VEC];
-                load_part<T, VEC>(b, g.post_bias, c);
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) xv[i * VEC + q] = X[q] = fmaf(k[q], b[q], X[q]);
             }
             if (g.post_weight) {
                 float w[VEC];
@@ -288,12 +281,12 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
             }
 #pragma unroll
             for (int q = 0; q < VEC; ++q) {
-                const double fd = u[i * VEC + q], Xd = X[q];
+                const double fd = u[i * VEC + q], xd = xv[i * VEC + q];
                 u[i * VEC + q] = u[i * VEC + q] * k[q];
                 const double ud = u[i * VEC + q];
                 s[0] = fma(fd, fd, s[0]);
-                s[1] = fma(Xd, Xd, s[1]);
-                s[2] = fma(Xd, ud, s[2]);
+                s[1] = fma(xd, xd, s[1]);
+                s[2] = fma(xd, ud, s[2]);
                 s[3] = fma(ud, ud, s[3]);
             }
         }
@@ -861,7 +854,7 @@ int forward_as(const ForwardCall& c) {
     const char* who = "residual_norm";
     const int64_t ctas = ceil_div(c.g.rows, (int64_t)(THREADS / T));
     if constexpr (T < THREADS) {
-        if (c.f.p && c.g.post_kind == CTB_NORM_RMS && c.g.pre_kind == CTB_NORM_RMS)
+        if (c.f.p && c.g.post_kind == CTB_NORM_RMS && c.g.pre_kind == CTB_NORM_RMS && !c.g.post_bias)
             return launch_clusters(who, residual_rms_kernel<THREADS, T, E, VEC>, ctas, THREADS, 0, 1, c.st, c.g, c.x, c.f, c.y, c.h, c.stats);
         return launch_clusters(who, residual_norm_kernel<THREADS, T, E, VEC>, ctas, THREADS, 0, 1, c.st, c.g, c.x, c.f, c.y, c.h, c.stats, 1);
     } else {

@@ -258,6 +258,17 @@ def test_residual_norm_widths(ct, cols, kinds):
         check_norm(ct, x, f, vectors(g, kinds[0], True, biased, cols), vectors(g, kinds[1], True, biased, cols), make_gate(g, gate, 1, rows, cols), 0.5, dy, dh)
 
 
+@pytest.mark.parametrize("cols", [63, 65, 127, 129, 301, 511, 1023, 1027, 1141, 2047, 3001, 4095, 4097])
+@pytest.mark.parametrize("kinds", [(1, 0), (2, 1), (2, 2)], ids=str)
+def test_residual_norm_odd_widths(ct, cols, kinds):
+    """Rows that go element by element, at the ends of what each share of a thread holds."""
+    g = gen(cols)
+    rows = 5 if cols > 4096 else 41
+    x, f, dy, dh = (randn(g, 1, rows, cols) for _ in range(4))
+    for gate, biased in (("none", True), ("channel", False), ("full", True)):
+        check_norm(ct, x, f, vectors(g, kinds[0], True, biased, cols), vectors(g, kinds[1], True, biased, cols), make_gate(g, gate, 1, rows, cols), 0.5, dy, dh)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 147, 300, 2500])
 @pytest.mark.parametrize("cols", [48, 768, 1536, 3000])
 def test_residual_norm_rows(ct, rows, cols):
