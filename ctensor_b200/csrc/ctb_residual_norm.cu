@@ -22,7 +22,8 @@
 // [32768, 768] 68 us (0.90), [4096, 8192] 97 us (0.84: two folds one behind the other); backward with one norm
 // [16384, 1536] 85 us (0.91), RMS on both sides [4096, 5120] 95 us (0.81), with a gate for every element 117 us
 // (0.88), [4096, 8192] in clusters 176 us (0.70); LayerNorms on both sides [16384, 1024] 88 us (0.70), registers
-// for four sums per column leave 12 warps on an SM; rows of odd length, element by element, 0.3 to 0.6.
+// for four sums per column leave 12 warps on an SM; rows of odd length go
+// element by element: [16000, 1999] with one norm forward 97 us (0.81), backward 140 us (0.70), two norms 0.56 and 0.35.
 #include "ctb_residual_norm.cuh"
 #include "ctb_team.cuh"
 
@@ -878,7 +879,7 @@ struct BwdShape {
 enum BwdKind { kBwdLean, kBwdFullPre, kBwdFull, kBwdScalarPre, kBwdScalar, kBwdAny };
 BwdShape bwd_shape(int64_t cols, BwdKind kind) {
     for (int team : {32, 64, 96, 128, 192, 256}) {
-        if (cols > team * kBwdShare || ((kind == kBwdScalarPre || kind == kBwdScalar) && team != 32 && team != 128)) continue;
+        if (cols > team * kBwdShare || ((kind == kBwdScalarPre || kind == kBwdScalar) && team != 32 && team != 128 && team != 256)) continue;
         // four sums per column and the weights beside them: 170 registers a thread
         if ((kind == kBwdFull || kind == kBwdScalar) && team <= 192) return {384, team, 1, 1};
         return {team == 96 ? 480 : (team == 192 ? 384 : 512), team, 1, 1};
@@ -953,7 +954,7 @@ int backward_narrow(BwdCall& c) {
         return backward_as<THREADS, T, kBwdShare, 1, BwdFlags<false, true, true, 1>>(c);
     }
     if (!c.vec) {
-        if constexpr (T == 32 || T == 128 || T == 512) return c.post ? backward_gate<FULL_THREADS, T, true, true, 1>(c) : backward_gate<THREADS, T, false, true, 1>(c);
+        if constexpr (T == 32 || T == 128 || T == 256 || T == 512) return c.post ? backward_gate<FULL_THREADS, T, true, true, 1>(c) : backward_gate<THREADS, T, false, true, 1>(c);
     }
     if (!c.full) return backward_fast<THREADS, T, false>(c);
     return c.post ? backward_gate<FULL_THREADS, T, true, true>(c) : backward_gate<THREADS, T, false, true>(c);
@@ -981,11 +982,17 @@ int launch_residual_norm(const ResidualNormGeom& geom, RowsIn x, RowsIn f, float
                      is_aligned(g.post_weight, 16) && is_aligned(g.post_bias, 16) && is_aligned(g.pre_weight, 16) && is_aligned(g.pre_bias, 16) &&
                      (g.gate_mode != kGateRow || rows_aligned(g.gate));
     const ForwardCall c{g, x, f, y, h, stats, st};
-    if (!vec) {
+    if (!vec) {                                          // a share that fits: [30000, 301] 36 us, 86 with that of 2048 columns
+        if (g.cols <= 64) return forward_as<256, 32, 2, 1>(c);
+        if (g.cols <= 128) return forward_as<256, 32, 4, 1>(c);
         if (g.cols <= 256) return forward_as<256, 32, 8, 1>(c);
+        if (g.cols <= 512) return forward_as<256, 64, 8, 1>(c);
+        if (g.cols <= 1024) return forward_as<256, 128, 8, 1>(c);
         if (g.cols <= 2048) return forward_as<256, 128, 16, 1>(c);
+        if (g.cols <= 4096) return forward_as<512, 512, 8, 1>(c);
         return forward_as<512, 512, 16, 1>(c);
     }
+    if (g.cols <= 128) return forward_as<256, 32, 4, 4>(c);
     if (g.cols <= 256) return forward_as<256, 32, 8, 4>(c);
     if (g.cols <= 512) return forward_as<256, 32, 16, 4>(c);
     if (g.cols <= 768) return forward_as<288, 96, 8, 4>(c);
