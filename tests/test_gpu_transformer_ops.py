@@ -86,6 +86,43 @@ def test_score_softmax_and_its_gradients(ct, shape, kind):
         within(dslopes, ws, sbound, "slope gradients")
 
 
+@pytest.mark.parametrize("shape", [(2, 4, 37, 20001), (2, 4, 37, 16400), (2, 2, 10, 30001), (1, 3, 11, 20000), (1, 2, 2, 140000)], ids=str)
+@pytest.mark.parametrize("kind", ["plain", "causal-prefix-lengths-cap", "docs", "docs-causal-lengths-slopes-cap-start"])
+def test_score_long_rows(ct, shape, kind):
+    """As many rows as CTAs run at once (each swept by one), and fewer (held or swept by clusters)."""
+    test_score_softmax_and_its_gradients(ct, shape, kind)
+
+
+@pytest.mark.parametrize("keys", [60, 128, 1000, 1001, 4096, 5000, 20000])
+def test_score_special_values_in_documents(ct, keys):
+    """Every third key in the query's document, with infinities and NaN there and elsewhere."""
+    inf, nan = math.inf, math.nan
+    g = gen(keys)
+    docs = (torch.arange(keys, device=DEV, dtype=torch.int32) % 3)[None].contiguous()
+    ok = docs[0] == 1
+    s = randn(g, 1, 1, 5, keys)
+    s[..., ~ok] = nan
+    s[0, 0, 0, 4] = inf
+    s[0, 0, 1, 4] = -inf
+    s[0, 0, 2, 4] = nan
+    s[0, 0, 3, ok] = -inf
+    r = ct.ScoreRules(query_docs=ints([[1] * 5]), key_docs=docs)
+    p = ct.score_softmax(s, r)[0, 0]
+    assert not bool(p[:, ~ok].any())
+    assert bool(p[0, ok].isnan().any()) and bool(p[2, ok].isnan().all()) and not bool(p[3].any())
+    assert float(p[1, 4]) == 0.0
+    for i in (1, 4):
+        finite = ok & s[0, 0, i].isfinite()                    # -inf adds exactly nothing; the bound is one of finite logits
+        t = s[0, 0, i, finite].double()[None, None, None]
+        want = torch.softmax(t, -1)
+        within(p[i, finite][None, None, None], want, ref.score_bound(t, want, {}), "probabilities")
+    dp = randn(g, 1, 1, 5, keys)
+    dp[0, 0, 0, 4], dp[0, 0, 0, 5] = inf, nan                  # one in the document, one outside
+    q = p.clone().nan_to_num(0.25)[None, None]
+    ds, _ = ct.score_softmax_backward(dp, q, r)
+    assert not bool(ds[..., ~ok].any()) and bool(ds[0, 0, 1:].isfinite().all()) and not bool(ds[0, 0, 0, ok].isfinite().any())
+
+
 def test_score_rows_of_many_sequences_and_a_long_cache(ct):
     """One query per sequence over 140,001 keys (a cluster of CTAs per row), ragged lengths."""
     g = gen(5)
