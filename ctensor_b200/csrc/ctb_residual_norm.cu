@@ -104,7 +104,7 @@ __device__ __forceinline__ float inverse_root(double v) {
 // cancellation that fp64 would notice until |mean| / sigma is about 1e6.
 template <int THREADS, int T, int E>
 __device__ __forceinline__ void row_statistics(const float (&v)[E], int kind, float eps, double inv_cols, TeamSlots<THREADS, 2, double>& sh,
-                                               int& turn, int cs, float* mean, float* rstd) {
+                                               FoldTurn& turn, float* mean, float* rstd) {
     double s[2] = {0.0, 0.0}, odd[2] = {0.0, 0.0};
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
@@ -116,7 +116,7 @@ __device__ __forceinline__ void row_statistics(const float (&v)[E], int kind, fl
     }
     s[0] = s[0] + odd[0];
     s[1] = s[1] + odd[1];
-    team_fold<FoldSum, THREADS, T>(s, sh, turn, cs);
+    team_fold<FoldSum, THREADS, T>(s, sh, turn);
     double var = s[1] * inv_cols;
     *mean = 0.0f;
     if (kind == CTB_NORM_LAYER) {
@@ -137,6 +137,7 @@ template <int THREADS, int T, int E, int VEC>
 __global__ void __launch_bounds__(THREADS, (kForwardCtas<THREADS, T, E, VEC>))
 residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ y, float* __restrict__ h, float* __restrict__ stats, int cs) {
     __shared__ TeamSlots<THREADS, 2, double> sh;
+    const TeamEntry entry(cs);
     const int tid = threadIdx.x % T;
     const uint32_t rank = cs > 1 ? cluster_rank() : 0;
     const int64_t row = (int64_t)(blockIdx.x / cs) * (THREADS / T) + threadIdx.x / T;
@@ -144,7 +145,6 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
     const int64_t slice = cs > 1 ? ((g.cols + cs - 1) / cs + 3) / 4 * 4 : g.cols;
     const int64_t begin = slice * rank;
     const int width = (int)(begin >= g.cols ? 0 : (g.cols - begin < slice ? g.cols - begin : slice));
-    int turn = 0;
     constexpr bool STAGED = kStageX<THREADS, T, E, VEC>;
     __shared__ __align__(16) float staged[STAGED ? E * THREADS : 1];
     float v[E], fv[E];
@@ -158,10 +158,11 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
     } else {
         load_share<T, E, VEC>(v, x.p + row * x.stride + begin, width, tid);
     }
+    FoldTurn turn = entry.met();
     float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
     if (f.p) {
         load_share<T, E, VEC>(fv, f.p + row * f.stride + begin, width, tid);
-        if (g.post_kind != CTB_NORM_NONE) row_statistics<THREADS, T, E>(fv, g.post_kind, g.post_eps, g.inv_cols, sh, turn, cs, &st.x, &st.y);
+        if (g.post_kind != CTB_NORM_NONE) row_statistics<THREADS, T, E>(fv, g.post_kind, g.post_eps, g.inv_cols, sh, turn, &st.x, &st.y);
         const float* gate = g.gate.p + (int64_t)fast_div((uint32_t)row, g.by_gate_rows) * g.gate.stride;
         const float one_gate = g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
         if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -213,7 +214,7 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
         }
     }
     if (g.pre_kind != CTB_NORM_NONE) {
-        row_statistics<THREADS, T, E>(v, g.pre_kind, g.pre_eps, g.inv_cols, sh, turn, cs, &st.z, &st.w);
+        row_statistics<THREADS, T, E>(v, g.pre_kind, g.pre_eps, g.inv_cols, sh, turn, &st.z, &st.w);
 #pragma unroll
         for (int i = 0; i < E / VEC; ++i) {
             const int c = col_of<T, VEC>(i, tid);
@@ -255,7 +256,7 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
     const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
     if (row >= g.rows) return;                           // whole teams leave together
     const int width = (int)g.cols;
-    int turn = 0;
+    FoldTurn turn = TeamEntry(1).met();
     float xv[E], u[E];
     load_share<T, E, VEC>(xv, x.p + row * x.stride, width, tid);
     load_share<T, E, VEC>(u, f.p + row * f.stride, width, tid);
@@ -292,7 +293,7 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
             }
         }
     }
-    team_fold<FoldSum, THREADS, T>(s, sh, turn, 1);
+    team_fold<FoldSum, THREADS, T>(s, sh, turn);
     const float rf = inverse_root(s[0] * g.inv_cols + (double)g.post_eps);
     const double r = rf;
     double sy = fma(r, fma(r, s[3], 2.0 * s[2]), s[1]);
@@ -305,7 +306,7 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
         }
         s[0] = square;
         s[1] = s[2] = s[3] = 0.0;
-        team_fold<FoldSum, THREADS, T>(s, sh, turn, 1);
+        team_fold<FoldSum, THREADS, T>(s, sh, turn);
         sy = s[0];
     }
     const float ry = inverse_root(sy * g.inv_cols + (double)g.pre_eps);
@@ -389,6 +390,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
     __shared__ TeamSlots<THREADS, 1, float> sh_gate;
     constexpr int SLOT = E * THREADS;
     constexpr int TEAMS = THREADS / T;
+    const TeamEntry entry(cs);
     const ResidualNormGeom& g = a.g;
     const int tid = threadIdx.x % T;
     const uint32_t rank = cs > 1 ? cluster_rank() : 0;
@@ -399,7 +401,6 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
     const int64_t begin = slice * rank;
     const int width = (int)(begin >= g.cols ? 0 : (g.cols - begin < slice ? g.cols - begin : slice));
     const float inv = (float)g.inv_cols;
-    int turn = 0, gate_turn = 0;
 
     float pre_w[E], pre_b[FULL ? E : 1], post_w[POST ? E : 1], post_b[POST && FULL ? E : 1], gate_sum[GATE ? E : 1];
 #pragma unroll
@@ -496,6 +497,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
     if (lo < hi) next_st = *stats;
     int stage_at = 0, ahead_at = (a.stages - 1) * STAGE;
     int64_t out_at = lo * g.cols + begin + tid * VEC;
+    FoldTurn turn = entry.met(), gate_turn = turn;
     for (int64_t row = lo; row < hi; ++row, out_at += g.cols) {
         const float4 st = next_st;
         fetch(ahead_at);                                 // into the place of the row before this one, which is done with
@@ -608,7 +610,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
             if constexpr (SUMS == 2) v[1] = s_a;
             if constexpr (SUMS >= 4) { v[1] = s_kef; v[2] = s_kfy; v[3] = s_a; }
             if constexpr (SUMS == 8) { v[4] = s_ke; v[5] = s_k; v[6] = s_kf; v[7] = s_ky; }
-            team_fold<FoldSum, THREADS, T>(v, sh, turn, cs);
+            team_fold<FoldSum, THREADS, T>(v, sh, turn);
             if (SCALAR && row > lo) collect(row - 1, left == g.gate_rows ? group - 1 : group, (int)(row - 1 - lo) & 1);
             s_ay = v[0];
             if constexpr (SUMS == 2) s_a = v[1];
@@ -698,7 +700,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
             leave(scalar_sum, (int)(row - lo) & 1);
         } else if (scalar_gate) {
             float one[1] = {scalar_sum};
-            team_fold<FoldSum, THREADS, T>(one, sh_gate, gate_turn, cs);
+            team_fold<FoldSum, THREADS, T>(one, sh_gate, gate_turn);
             scalar_gate_sum = scalar_gate_sum + one[0];
         }
         // a gate that rows share: its sum so far goes out when the next row belongs to another gate row

@@ -328,6 +328,7 @@ template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS, (ALIGNED ? 1280 : 1024) / THREADS)
 score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     const int cs = T == 512 ? ctas : 1;                  // only whole CTAs of 512 threads come in clusters
+    const TeamEntry entry(cs);
     static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
     __shared__ TeamSlots<THREADS, 1, float> sh;
     const int tid = threadIdx.x % T;
@@ -343,7 +344,6 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     const ScoreSpan span = score_span<T>(a, place, keys, phase, cs);
     mine.init(score_docs<DOCS>(a, w, phase), span.sees(w), span.from, tid, phase);
     mine.zeros(out, span.end);
-    int turn = 0;
     float t[NV][4];
     mine.load(t, s, score_phase(s) == phase);
     float m[1] = {-INFINITY};
@@ -355,7 +355,8 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
             m[0] = fmaxf(m[0], t[j][k]);
         }
     });
-    team_fold<FoldMax, THREADS, T>(m, sh, turn, cs);
+    FoldTurn turn = entry.met();
+    team_fold<FoldMax, THREADS, T>(m, sh, turn);
     const float top = m[0] == -INFINITY ? 0.0f : m[0];
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     mine.each([&](int j, const auto&) {
@@ -366,7 +367,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
         }
     });
     float z[1] = {(part[0] + part[1]) + (part[2] + part[3])};
-    team_fold<FoldSum, THREADS, T>(z, sh, turn, cs);
+    team_fold<FoldSum, THREADS, T>(z, sh, turn);
     const float inv = z[0] == 0.0f ? 0.0f : __frcp_rn(z[0]);
     const bool usual = z[0] < INFINITY;                  // else NaN, which must not reach the masked columns
     mine.each([&](int j, const auto& o) {
@@ -388,6 +389,7 @@ template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : DOCS ? 0 : CAP || !ALIGNED ? 4 : 5)
 score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     const int cs = T == 512 ? ctas : 1;                  // only whole CTAs of 512 threads come in clusters
+    const TeamEntry entry(cs);
     static_assert(NV <= 8, "admitted columns are kept as 4 * NV bits");
     __shared__ TeamSlots<THREADS, 1, float> sh;
     __shared__ TeamSlots<THREADS, 1, double> sh_slope;
@@ -404,7 +406,6 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     const ScoreSpan span = score_span<T>(a, place, keys, phase, cs);
     mine.init(score_docs<DOCS>(a, w, phase), span.sees(w), span.from, tid, phase);
     mine.zeros(out, span.end);
-    int turn = 0;
     float p[NV][4], dp[NV][4], s[CAP ? NV : 1][4];
     mine.load(p, pr, score_phase(pr) == phase);
     mine.load(dp, gr, score_phase(gr) == phase);
@@ -422,7 +423,8 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
         }
     });
     float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
-    team_fold<FoldSum, THREADS, T>(d, sh, turn, cs);
+    FoldTurn turn = entry.met();
+    team_fold<FoldSum, THREADS, T>(d, sh, turn);
     const bool usual = fabsf(d[0]) < INFINITY;           // else 0 * (0 - D) is NaN in the masked columns
     float slope_sum = 0.0f;
     mine.each([&](int j, const auto& o) {
@@ -442,7 +444,7 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     });
     if (a.slope_part) {
         double sum[1] = {(double)slope_sum};
-        team_fold<FoldSum, THREADS, T>(sum, sh_slope, turn, cs);
+        team_fold<FoldSum, THREADS, T>(sum, sh_slope, turn);
         if (tid == 0 && place.present && (cs == 1 || cluster_rank() == 0)) a.slope_part[row] = sum[0];
     }
 }
@@ -462,6 +464,7 @@ __device__ __forceinline__ SweepSpan sweep_span(int64_t keys, int phase, int cs)
 template <bool CAP, bool DOCS>
 __global__ void __launch_bounds__(kSweepThreads)
 score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
+    const TeamEntry entry(cs);
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     const int64_t row = blockIdx.x / cs;
     const ScorePlace w = score_place(a, {(uint32_t)row, true});
@@ -473,7 +476,6 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
-    int turn = 0;
     // first sweep: the thread's maximum and its sum of exponentials relative to that maximum
     float m = -INFINITY, z = 0.0f;
     for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
@@ -510,10 +512,11 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
         z = z + ((part[0] + part[1]) + (part[2] + part[3]));
     }
     float top[1] = {m};
-    team_fold<FoldMax, kSweepThreads, kSweepThreads>(top, sh, turn, cs);
+    FoldTurn turn = entry.met();
+    team_fold<FoldMax, kSweepThreads, kSweepThreads>(top, sh, turn);
     const float from = top[0] == -INFINITY ? 0.0f : top[0];
     float sum[1] = {m == -INFINITY ? z : z * score_exp(m - from)};
-    team_fold<FoldSum, kSweepThreads, kSweepThreads>(sum, sh, turn, cs);
+    team_fold<FoldSum, kSweepThreads, kSweepThreads>(sum, sh, turn);
     const float inv = sum[0] == 0.0f ? 0.0f : __frcp_rn(sum[0]);
     // second sweep
     for (int64_t f = span.lo + threadIdx.x; f < span.hi; f += kSweepThreads * kSweepBatch) {
@@ -546,6 +549,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
 template <bool CAP, bool DOCS>
 __global__ void __launch_bounds__(kSweepThreads)
 score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
+    const TeamEntry entry(cs);
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     __shared__ TeamSlots<kSweepThreads, 1, double> sh_slope;
     const int64_t row = blockIdx.x / cs;
@@ -558,7 +562,6 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
-    int turn = 0;
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
         float p[kSweepBatch][4], dp[kSweepBatch][4];
@@ -576,7 +579,8 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
             for (int k = 0; k < 4; ++k) part[k] = fmaf(p[u][k], dp[u][k], part[k]);
     }
     float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
-    team_fold<FoldSum, kSweepThreads, kSweepThreads>(d, sh, turn, cs);
+    FoldTurn turn = entry.met();
+    team_fold<FoldSum, kSweepThreads, kSweepThreads>(d, sh, turn);
     double slope_sum = 0.0;
     for (int64_t f = span.lo + threadIdx.x; f < span.hi; f += kSweepThreads * kSweepBatch) {
         float p[kSweepBatch][4], dp[kSweepBatch][4], s[kSweepBatch][4];
@@ -613,7 +617,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     }
     if (a.slope_part) {
         double sum[1] = {slope_sum};
-        team_fold<FoldSum, kSweepThreads, kSweepThreads>(sum, sh_slope, turn, cs);
+        team_fold<FoldSum, kSweepThreads, kSweepThreads>(sum, sh_slope, turn);
         if (threadIdx.x == 0 && (cs == 1 || cluster_rank() == 0)) a.slope_part[row] = sum[0];
     }
 }
@@ -627,8 +631,8 @@ score_slope_fold_kernel(const double* __restrict__ part, int64_t batch, int64_t 
     wait_for_previous();
     for (int64_t b = 0; b < batch; ++b)
         for (int64_t i = threadIdx.x; i < queries; i += 256) sum[0] = sum[0] + part[(b * heads + h) * queries + i];
-    int turn = 0;
-    team_fold<FoldSum, 256, 256>(sum, sh, turn, 1);
+    FoldTurn turn = TeamEntry(1).met();
+    team_fold<FoldSum, 256, 256>(sum, sh, turn);
     if (threadIdx.x == 0) out[h] = (float)-sum[0];
 }
 

@@ -12,8 +12,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 // The address of this CTA's shared object `p` in the CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t peer_shared(const void* p, uint32_t rank) {
@@ -32,6 +35,36 @@ struct FoldSum {
 struct FoldMax {      // like fmaxf, ignores a NaN
     static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
     static __device__ __forceinline__ float none() { return -INFINITY; }
+};
+
+// A CTA's shared memory may be written by another of its cluster only once it is known to run.  A kernel therefore
+// makes a TeamEntry first of all, which arrives at the cluster's barrier, and gets the FoldTurn that every fold asks
+// for from met(), which waits there: the row's loads lie between the two.  Every thread of a cluster calls
+// both; with one CTA to a team (cs == 1) neither does anything.
+class FoldTurn {
+public:
+    const int cs;                                        // CTAs of a team
+    int slot = 0;
+
+private:
+    __device__ __forceinline__ explicit FoldTurn(int ctas) : cs(ctas) {}
+    friend class TeamEntry;
+};
+class TeamEntry {
+public:
+    __device__ __forceinline__ explicit TeamEntry(int ctas) : cs_(ctas) {
+        if (cs_ > 1) cluster_arrive();
+    }
+    __device__ __forceinline__ FoldTurn met() const {
+        if (cs_ > 1) {
+            __syncwarp();
+            cluster_wait();
+        }
+        return FoldTurn(cs_);
+    }
+
+private:
+    const int cs_;
 };
 
 // Two sets of slots used in turn: a slot is written again only after every reader has passed the barrier
@@ -54,12 +87,12 @@ __device__ __forceinline__ void lane_fold(S (&v)[N], const S* p, int count) {
     for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, x, n);
 }
 
-// Folds N (a power of two) values over a team of T threads of a CTA of THREADS, and over the `cs` CTAs of
-// a cluster when cs > 1 (a team is then a whole CTA).  Every thread of the team calls it and gets the same
+// Folds N (a power of two) values over a team of T threads of a CTA of THREADS, and over the CTAs of a
+// cluster when turn.cs > 1 (a team is then a whole CTA).  Every thread of the team calls it and gets the same
 // bits.  Within a warp the values are folded in halves — a lane passes on half of its values, then half of
 // the rest — so that eight sums cost 9 shuffles instead of 40; lane l then holds value l / (32 / N).
 template <typename OP, int THREADS, int T, int N, typename S>
-__device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& sh, int& turn, int cs) {
+__device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& sh, FoldTurn& turn) {
     if constexpr (T < 32) {                              // several teams in a warp, all of whose lanes take part
 #pragma unroll
         for (int n = 0; n < N; ++n)
@@ -87,20 +120,20 @@ __device__ __forceinline__ void team_fold(S (&v)[N], TeamSlots<THREADS, N, S>& s
         return;
     }
     const int warp = threadIdx.x >> 5, team = threadIdx.x / T;
-    if (T == THREADS && cs > 1) {
+    if (T == THREADS && turn.cs > 1) {
         // every warp leaves its values with every CTA: one barrier for warps and CTAs together
         const uint32_t rank = cluster_rank();
         const S mine = __shfl_sync(0xffffffffu, v[0], (lane % N) * (32 / N));
-        for (int peer = lane / N; peer < cs; peer += 32 / N) store_peer(peer_shared(&sh.warps[turn][rank * (THREADS / 32) + warp][lane % N], peer), mine);
+        for (int peer = lane / N; peer < turn.cs; peer += 32 / N) store_peer(peer_shared(&sh.warps[turn.slot][rank * (THREADS / 32) + warp][lane % N], peer), mine);
         __syncwarp();
         cluster_barrier();
-        lane_fold<OP, N>(v, &sh.warps[turn][0][0], cs * (THREADS / 32));
+        lane_fold<OP, N>(v, &sh.warps[turn.slot][0][0], turn.cs * (THREADS / 32));
     } else {
-        if (lane % (32 / N) == 0) sh.warps[turn][warp][lane / (32 / N)] = v[0];
+        if (lane % (32 / N) == 0) sh.warps[turn.slot][warp][lane / (32 / N)] = v[0];
         asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(T) : "memory");
-        lane_fold<OP, N>(v, &sh.warps[turn][team * (T / 32)][0], T / 32);
+        lane_fold<OP, N>(v, &sh.warps[turn.slot][team * (T / 32)][0], T / 32);
     }
-    turn ^= 1;
+    turn.slot ^= 1;
 }
 
 // How many clusters of `cs` CTAs of this kernel the current device runs at once.

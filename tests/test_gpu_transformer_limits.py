@@ -1,0 +1,56 @@
+"""GPU tests of the transformer-step operators where their kernels' limits lie: clusters of CTAs, far documents, very
+many rows, values near the ends of their types; against plain forms in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import transformer_ref as ref
+from test_gpu_transformer_ops import DEV, gen, ints, randn, vectors, within
+from transformer_ref import U
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- clusters of CTAs -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("keys", [5000, 30001, 140000])
+def test_clusters_whose_ctas_have_nothing_to_load(ct, keys):
+    """Rows in clusters (held and swept, both directions) of which most CTAs see no admitted key and so come to the
+    cluster's first exchange as soon as they start, many launches in a row."""
+    g = gen(keys)
+    B, H = 6, 2
+    s, dp = randn(g, B, H, 1, keys) * 3, randn(g, B, H, 1, keys)
+    rules = {"scale": 0.5, "causal": True, "cap": 6.0, "key_lengths": ints([0, 1, 7, 600, 2100, keys]), "slopes": randn(g, H).abs() * 0.01}
+    r = ct.ScoreRules(**rules)
+    want = ref.score_softmax(s.double(), rules)
+    runs = []
+    for _ in range(20):
+        p = ct.score_softmax(s, r)
+        runs.append((p, *ct.score_softmax_backward(dp, p, r, scores=s, want_slopes=True)))
+    p, ds, dslopes = runs[0]
+    within(p, want, ref.score_bound(s.double(), want, rules), "probabilities")
+    w, ws, bound, sbound = ref.score_gradients(s.double(), p.double(), dp.double(), rules)
+    within(ds, w, bound, "score gradients")
+    within(dslopes, ws, sbound, "slope gradients")
+    assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(run, runs[0]))
+
+
+@pytest.mark.parametrize("cols", [8196, 16388, 32768])
+def test_clusters_of_norm_rows_many_times(ct, cols):
+    """Rows in clusters, the last CTA's slice smaller than the others', many launches in a row."""
+    g = gen(cols)
+    x, f, dy, dh = (randn(g, 9, cols) for _ in range(4))
+    pre, post = vectors(g, 2, True, False, cols), vectors(g, 2, True, False, cols)
+    params = ct.ResidualNorm(pre=2, pre_weight=pre[1], post=2, post_weight=post[1])
+    runs = []
+    for _ in range(20):
+        y, h, stats = ct.residual_norm(x, f, params)
+        n = ct.residual_norm_backward(f, y, stats, params, grad_y=dy, grad_h=dh)
+        runs.append((y, h, stats, n.x, n.f, n.pre_weight, n.post_weight))
+    y = runs[0][0]
+    want = x.double() + ref.normed(f.double(), 2, post[1].double(), None, 1e-5)
+    within(y, want, ref.norm_bound(f.double(), 2, post[1].double(), None, 1e-5) + U * (4 * (want - x.double()).abs() + want.abs()), "y")
+    grads = ref.residual_norm_gradients(f.double(), y.double(), (2, pre[1].double(), None), (2, post[1].double(), None), None, 1.0, dy.double(), dh.double())
+    for name, t in zip(("x", "f", "pre_weight", "post_weight"), runs[0][3:]):
+        within(t, grads[name][0], grads[name][1] + 1e-36, "gradient of " + name)
+    assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(run, runs[0]))
