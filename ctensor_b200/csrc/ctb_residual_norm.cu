@@ -802,12 +802,18 @@ residual_norm_fold_kernel(const __grid_constant__ FoldJobs j) {
             const int64_t t = group + 1, start = j.rows * t / j.teams;
             group = start / j.gate_rows;
             // a gate row begins here, or the one that does not began before the team ahead, whose job it then is
-            if (start % j.gate_rows == 0 || j.rows * (t - 1) / j.teams > group * j.gate_rows) return;
+            if (start % j.gate_rows == 0 || j.rows * (t - 1) / j.teams > group * j.gate_rows) {
+                wait_for_previous();                     // also with nothing to add: no block of this launch ends ahead of
+                return;                                  // the one before it, which later work in the stream relies on
+            }
         }
         const int64_t r0 = group * j.gate_rows, r1 = r0 + j.gate_rows - 1;
         first = ((r0 + 1) * j.teams - 1) / j.rows + group;
         last = ((r1 + 1) * j.teams - 1) / j.rows + group;
-        if (first == last) return;                       // one team's: it wrote the sum itself
+        if (first == last) {                             // one team's: it wrote the sum itself
+            wait_for_previous();
+            return;
+        }
         width = j.gate_width;
         part = j.gate_part;
         out = j.gate + group * width;

@@ -54,3 +54,27 @@ def test_clusters_of_norm_rows_many_times(ct, cols):
     for name, t in zip(("x", "f", "pre_weight", "post_weight"), runs[0][3:]):
         within(t, grads[name][0], grads[name][1] + 1e-36, "gradient of " + name)
     assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(run, runs[0]))
+
+
+# ---- the second launch of the norm gradients ----------------------------------------------------------------
+@pytest.mark.parametrize("cols", [200, 4096])
+@pytest.mark.parametrize("last", ["row", "value"])
+def test_gate_gradients_that_need_no_second_launch(ct, cols, last):
+    """No weights, and gate rows that end where a team's rows do on a machine of 148 SMs, so nothing is left to add
+    up; what comes next in the stream reads the results at once."""
+    g = gen(cols)
+    sequences, rows = 296, 8
+    x, f, dy, dh = (randn(g, sequences, rows, cols) for _ in range(4))
+    gate = randn(g, sequences, 1, cols if last == "row" else 1)
+    params = ct.ResidualNorm(pre=2, post=2)
+    y, h, stats = ct.residual_norm(x, f, params, gate=gate)
+    want = ref.residual_norm_gradients(f.double(), y.double(), (2, None, None), (2, None, None), gate.double(), 1.0, dy.double(), dh.double())
+    torch.cuda.synchronize()
+    for _ in range(20):
+        n = ct.residual_norm_backward(f, y, stats, params, grad_y=dy, grad_h=dh, gate=gate)
+        read = [t.clone() for t in (n.x, n.f, n.gate)]
+        for t in (n.x, n.f, n.gate):
+            t.fill_(math.nan)                            # the next call's results lie in the same memory
+        for name, t in zip(("x", "f", "gate"), read):
+            within(t, want[name][0], want[name][1] + 1e-36, "gradient of " + name)
+        del n
