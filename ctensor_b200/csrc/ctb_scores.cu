@@ -50,6 +50,7 @@ struct ScorePlace {
     int live;                           // keys [0, live) may be admitted
     int centre;                         // the key position nearest to the query's within [0, live)
     float beyond;                       // |pos - centre|
+    int near;                           // distances from `centre` are counted from here on in the bias
     float slope;
     int doc;
 };
@@ -73,6 +74,7 @@ __device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, ScoreRow r
     w.live = max(w.live, 0);
     w.centre = 0;
     w.beyond = w.slope = 0.0f;
+    w.near = 0;
     if (g.slopes) {
         w.centre = (int)max(min(pos, (int64_t)w.live - 1), (int64_t)0);
         w.beyond = (float)(pos > w.centre ? pos - w.centre : w.centre - pos);
@@ -190,16 +192,32 @@ __device__ __forceinline__ float score_exp(float x) {
     return r;
 }
 // t of a four's columns.  The bias is taken from the key nearest to the query, which changes no probability
-// (a softmax does not see a constant) and keeps t small where the query is far from every key.
-template <bool CAP>
+// (a softmax does not see a constant) and keeps t small where the query is far from every key.  Without documents that
+// is the centre.  With them the admitted keys may be anywhere, and the team agrees on one of them to count from (any will
+// do: t is then no larger than the distances differ): a query 100000 keys behind its document would else have logits of
+// 5e4 at a slope of 1/2, where a step of Float32 is 0.004.
+template <bool CAP, bool DOCS>
 __device__ __forceinline__ void score_logits(const ScoreGeom& g, const ScorePlace& w, float (&t)[4], int c0) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) t[k] = CAP ? g.cap * tanhf(t[k] * g.over_cap) : t[k] * g.scale;
     if (g.slopes) {
-        const float from = (float)(c0 - w.centre);
+        if (DOCS) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = fmaf(-w.slope, fabsf(from + (float)k), t[k]);
+            for (int k = 0; k < 4; ++k) t[k] = fmaf(-w.slope, (float)(abs(c0 + k - w.centre) - w.near), t[k]);
+        } else {
+            const float from = (float)(c0 - w.centre);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = fmaf(-w.slope, fabsf(from + (float)k), t[k]);
+        }
     }
+}
+constexpr int kNoKey = 0x7FFFFFFF;
+// The distance from the centre that the team counts from: the smallest of its threads' (kNoKey: none), to Float32.
+template <int THREADS, int T>
+__device__ __forceinline__ int score_near(int near, TeamSlots<THREADS, 1, float>& sh, FoldTurn& turn) {
+    float most[1] = {near == kNoKey ? -INFINITY : -(float)near};
+    team_fold<FoldMax, THREADS, T>(most, sh, turn);
+    return most[0] == -INFINITY ? 0 : (int)-most[0];
 }
 template <bool CAP>
 __device__ __forceinline__ void score_slow(const ScoreGeom& g, float (&r)[4], const float* s) {     // r *= scale * (1 - tanh^2)
@@ -335,7 +353,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     const ScoreRow place = score_row_of<THREADS, T>(a, cs);
     if (T >= 32 && !place.present) return;               // whole teams leave together; never in a cluster
     const int64_t row = place.row;
-    const ScorePlace w = score_place(a, place);
+    ScorePlace w = score_place(a, place);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float* s = score_row(a.s, w);
@@ -346,16 +364,20 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     mine.zeros(out, span.end);
     float t[NV][4];
     mine.load(t, s, score_phase(s) == phase);
+    FoldTurn turn = entry.met();
+    if (DOCS && a.g.slopes) {
+        const int at = __ffs(mine.bits) - 1;             // the thread's first admitted key
+        w.near = score_near<THREADS, T>(at < 0 ? kNoKey : abs(mine.column(at >> 2) + (at & 3) - w.centre), sh, turn);
+    }
     float m[1] = {-INFINITY};
     mine.each([&](int j, const auto& o) {
-        score_logits<CAP>(a.g, w, t[j], o.column());
+        score_logits<CAP, DOCS>(a.g, w, t[j], o.column());
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             t[j][k] = o.has(k) ? t[j][k] : -INFINITY;
             m[0] = fmaxf(m[0], t[j][k]);
         }
     });
-    FoldTurn turn = entry.met();
     team_fold<FoldMax, THREADS, T>(m, sh, turn);
     const float top = m[0] == -INFINITY ? 0.0f : m[0];
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -467,7 +489,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     const TeamEntry entry(cs);
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     const int64_t row = blockIdx.x / cs;
-    const ScorePlace w = score_place(a, {(uint32_t)row, true});
+    ScorePlace w = score_place(a, {(uint32_t)row, true});
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float* s = score_row(a.s, w);
@@ -476,6 +498,8 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
+    const bool far = DOCS && a.g.slopes;                 // every thread counts from its own first admitted key for now
+    if (far) w.near = kNoKey;
     // first sweep: the thread's maximum and its sum of exponentials relative to that maximum
     float m = -INFINITY, z = 0.0f;
     for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
@@ -488,11 +512,16 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
         }
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
+        if (far && w.near == kNoKey) {
+#pragma unroll
+            for (int u = kSweepBatch - 1; u >= 0; --u)
+                if (bits[u]) w.near = abs((int)((f + (int64_t)u * kSweepThreads) * 4) - phase + __ffs(bits[u]) - 1 - w.centre);
+        }
         float top = m;
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) {
             if (!bits[u]) continue;
-            score_logits<CAP>(a.g, w, t[u], (int)((f + (int64_t)u * kSweepThreads) * 4) - phase);
+            score_logits<CAP, DOCS>(a.g, w, t[u], (int)((f + (int64_t)u * kSweepThreads) * 4) - phase);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 t[u][k] = (bits[u] >> k) & 1u ? t[u][k] : -INFINITY;
@@ -511,8 +540,13 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
             }
         z = z + ((part[0] + part[1]) + (part[2] + part[3]));
     }
-    float top[1] = {m};
     FoldTurn turn = entry.met();
+    if (far) {
+        const int mine = w.near;
+        w.near = score_near<kSweepThreads, kSweepThreads>(mine, sh, turn);
+        if (m != -INFINITY) m = fmaf(-w.slope, (float)(mine - w.near), m);
+    }
+    float top[1] = {m};
     team_fold<FoldMax, kSweepThreads, kSweepThreads>(top, sh, turn);
     const float from = top[0] == -INFINITY ? 0.0f : top[0];
     float sum[1] = {m == -INFINITY ? z : z * score_exp(m - from)};
@@ -536,7 +570,7 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
             const int c0 = (int)(at * 4) - phase;
             float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (bits[u]) {
-                score_logits<CAP>(a.g, w, t[u], c0);
+                score_logits<CAP, DOCS>(a.g, w, t[u], c0);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     if ((bits[u] >> k) & 1u) p[k] = score_exp(t[u][k] - from) * inv;

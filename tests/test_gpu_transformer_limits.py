@@ -78,3 +78,57 @@ def test_gate_gradients_that_need_no_second_launch(ct, cols, last):
         for name, t in zip(("x", "f", "gate"), read):
             within(t, want[name][0], want[name][1] + 1e-36, "gradient of " + name)
         del n
+
+
+# ---- distance bias with documents ----------------------------------------------------------------------------
+def far_bound(s, p, rules):
+    """ref.score_bound with the bias counted from the nearest admitted key, documents among the rules or not."""
+    ok = ref.admitted(s.shape, rules, s.device)
+    bare = {k: v for k, v in rules.items() if k != "slopes"}
+    d = torch.where(ok, ref.distance(s.shape, rules, s.device), math.inf)
+    near = d.amin(-1, keepdim=True)
+    d = torch.where(ok, d - torch.where(near == math.inf, 0.0, near), 0.0)
+    T = torch.where(ok, ref.logits(torch.where(ok, s, 0.0), bare).abs(), 0.0) + rules["slopes"].double().abs()[None, :, None, None] * d
+    return p * U * (22.0 * T.amax(-1, keepdim=True) + 83.0) + 1e-37
+
+
+def far_rules(g, H, Q, K):
+    """Two sequences; in the first the queries see the 60 first keys only, in the second a few keys in every 1000th
+    stretch, or none; slopes from 1/2 up."""
+    docs = torch.full((2, K), 9, dtype=torch.int32, device=DEV)
+    docs[0, :60] = 1
+    docs[1, 7::1000] = 1
+    docs[1, 8::1000] = 2
+    who = torch.ones(2, Q, dtype=torch.int32, device=DEV)
+    who[1, ::2], who[1, -1] = 2, 5
+    return {"scale": 0.5, "query_docs": who, "key_docs": docs, "slopes": 0.5 + torch.rand(H, device=DEV, generator=g)}
+
+
+@pytest.mark.parametrize("keys", [100, 700, 3001, 8192, 16384, 30001, 120000])
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+def test_score_bias_of_far_documents(ct, keys, cap):
+    g = gen(keys)
+    B, H, Q = 2, 3, 5
+    s = randn(g, B, H, Q, keys) * 3
+    rules = dict(far_rules(g, H, Q, keys), cap=cap)
+    for start in (None, ints([keys - 1, 0]), ints([2_000_000, -2_000_000])):
+        if start is not None:
+            rules["query_start"] = start
+        p = ct.score_softmax(s, ct.ScoreRules(**rules))
+        want = ref.score_softmax(s.double(), rules)
+        within(p, want, far_bound(s.double(), want, rules), f"probabilities from {start}")
+
+
+def test_score_bias_of_far_documents_beyond_exact_floats(ct):
+    """Positions that Float32 does not tell apart."""
+    g = gen(4)
+    K = 20_000_001
+    s = randn(g, 1, 1, 2, K)
+    docs = torch.zeros(1, K, dtype=torch.int32, device=DEV)
+    docs[0, 1001:1101] = 1
+    rules = {"query_docs": ints([[1, 1]]), "key_docs": docs, "slopes": torch.full((1,), 0.3, device=DEV), "causal": True}
+    p = ct.score_softmax(s, ct.ScoreRules(**rules))[..., :2000]
+    assert float(p[..., :1001].sum()) == 0
+    t = s[..., 1001:1101].double() - 0.3000000119 * torch.arange(99, -1, -1, device=DEV)
+    want = torch.softmax(t, -1)
+    within(p[..., 1001:1101], want, want * U * (22.0 * t.abs().amax(-1, keepdim=True) + 83.0), "probabilities")
