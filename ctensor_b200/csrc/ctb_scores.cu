@@ -44,6 +44,7 @@ __device__ __forceinline__ ScoreRow score_row_of(const ScoreArgs& a, int cs) {
     const bool present = row < a.rows;
     return {present ? (uint32_t)row : (uint32_t)(a.rows - 1), present};
 }
+constexpr int kNoKey = 0x7FFFFFFF;
 // Where a row is and what its query may look at.
 struct ScorePlace {
     uint32_t row, b, h, i;
@@ -193,9 +194,8 @@ __device__ __forceinline__ float score_exp(float x) {
 }
 // t of a four's columns.  The bias is taken from the key nearest to the query, which changes no probability
 // (a softmax does not see a constant) and keeps t small where the query is far from every key.  Without documents that
-// is the centre.  With them the admitted keys may be anywhere, and the team agrees on one of them to count from (any will
-// do: t is then no larger than the distances differ): a query 100000 keys behind its document would else have logits of
-// 5e4 at a slope of 1/2, where a step of Float32 is 0.004.
+// is the centre.  With them the nearest admitted key may be anywhere, and the team looks for it (`near`): a query 100000
+// keys behind its document would else have logits of 5e4 at a slope of 1/2, where a step of Float32 is 0.004.
 template <bool CAP, bool DOCS>
 __device__ __forceinline__ void score_logits(const ScoreGeom& g, const ScorePlace& w, float (&t)[4], int c0) {
 #pragma unroll
@@ -211,8 +211,7 @@ __device__ __forceinline__ void score_logits(const ScoreGeom& g, const ScorePlac
         }
     }
 }
-constexpr int kNoKey = 0x7FFFFFFF;
-// The distance from the centre that the team counts from: the smallest of its threads' (kNoKey: none), to Float32.
+// The smallest of the team's distances (kNoKey: none), the same in every thread; beyond 2^24 to Float32, which is as good.
 template <int THREADS, int T>
 __device__ __forceinline__ int score_near(int near, TeamSlots<THREADS, 1, float>& sh, FoldTurn& turn) {
     float most[1] = {near == kNoKey ? -INFINITY : -(float)near};
@@ -303,6 +302,17 @@ struct ScoreShare {
         }
     }
     __device__ __forceinline__ int column(int v) const { return first + v * T * 4; }
+    // The smallest distance from the centre of the thread's admitted keys (with kBits): it is the last one's up to the
+    // centre or the first one's behind it.
+    __device__ __forceinline__ int nearest(const ScorePlace& w) const {
+        const int ahead = w.centre - first, v = ahead / (4 * T);       // v: of the last four that begins up to the centre
+        const int count = ahead < 0 ? 0 : min(4 * v + min(ahead - v * 4 * T, 3) + 1, 32);
+        const uint32_t upto = (uint32_t)((1ull << count) - 1ull);
+        const int below = 31 - __clz(bits & upto), above = __ffs(bits & ~upto) - 1;
+        int d = below < 0 ? kNoKey : w.centre - (column(below >> 2) + (below & 3));
+        if (above >= 0) d = min(d, column(above >> 2) + (above & 3) - w.centre);
+        return d;
+    }
     __device__ __forceinline__ bool any(int v) const { return kBits ? ((bits >> (4 * v)) & 15u) != 0 : rest > v * T * 4; }
     // values of the fours that have an admitted column; others are 0 or keep what they held
     __device__ __forceinline__ void load(float (&x)[NV][4], const float* row, bool aligned) const {
@@ -365,10 +375,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     float t[NV][4];
     mine.load(t, s, score_phase(s) == phase);
     FoldTurn turn = entry.met();
-    if (DOCS && a.g.slopes) {
-        const int at = __ffs(mine.bits) - 1;             // the thread's first admitted key
-        w.near = score_near<THREADS, T>(at < 0 ? kNoKey : abs(mine.column(at >> 2) + (at & 3) - w.centre), sh, turn);
-    }
+    if (DOCS && a.g.slopes) w.near = score_near<THREADS, T>(mine.nearest(w), sh, turn);
     float m[1] = {-INFINITY};
     mine.each([&](int j, const auto& o) {
         score_logits<CAP, DOCS>(a.g, w, t[j], o.column());
@@ -476,6 +483,24 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
 constexpr int kSweepThreads = 512;
 constexpr int kSweepBatch = 4;                           // fours in flight per thread and operand
 
+// The smallest distance of an admitted key from the centre, looked for outwards from there by every CTA of the row for
+// itself: one step for a query next to its document, a pass over the documents for one far away (512 rows of 40000 keys, four
+// of five queries far from theirs, 481 us; without slopes 383).
+__device__ __forceinline__ int sweep_near(const ScoreDocs& docs, const ScorePlace& w, TeamSlots<kSweepThreads, 1, float>& sh, FoldTurn& turn) {
+    const int farthest = max(w.centre, w.live - 1 - w.centre);
+    int near = kNoKey;
+    for (int from = 0; from <= farthest; from += kSweepThreads * kSweepBatch) {
+#pragma unroll
+        for (int u = 0; u < kSweepBatch; ++u) {
+            const int d = from + u * kSweepThreads + (int)threadIdx.x;
+            const bool before = d <= w.centre && w.live > 0, behind = d < w.live - w.centre;
+            if ((before && docs.p[(w.centre - d) * docs.si] == w.doc) || (behind && docs.p[(w.centre + d) * docs.si] == w.doc)) near = min(near, d);
+        }
+        if (__syncthreads_or(near != kNoKey)) break;
+    }
+    return score_near<kSweepThreads, kSweepThreads>(near, sh, turn);
+}
+
 struct SweepSpan { int64_t lo, hi; };
 __device__ __forceinline__ SweepSpan sweep_span(int64_t keys, int phase, int cs) {
     const int64_t fours = (keys + phase + 3) / 4, share = (fours + cs - 1) / cs;
@@ -498,8 +523,8 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
-    const bool far = DOCS && a.g.slopes;                 // every thread counts from its own first admitted key for now
-    if (far) w.near = kNoKey;
+    FoldTurn turn = entry.met();
+    if (DOCS && a.g.slopes) w.near = sweep_near(docs, w, sh, turn);
     // first sweep: the thread's maximum and its sum of exponentials relative to that maximum
     float m = -INFINITY, z = 0.0f;
     for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
@@ -512,11 +537,6 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
         }
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) score_load(t[u], s, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u], aligned);
-        if (far && w.near == kNoKey) {
-#pragma unroll
-            for (int u = kSweepBatch - 1; u >= 0; --u)
-                if (bits[u]) w.near = abs((int)((f + (int64_t)u * kSweepThreads) * 4) - phase + __ffs(bits[u]) - 1 - w.centre);
-        }
         float top = m;
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u) {
@@ -539,12 +559,6 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
                 for (int k = 0; k < 4; ++k) part[k] = part[k] + score_exp(t[u][k] - from);
             }
         z = z + ((part[0] + part[1]) + (part[2] + part[3]));
-    }
-    FoldTurn turn = entry.met();
-    if (far) {
-        const int mine = w.near;
-        w.near = score_near<kSweepThreads, kSweepThreads>(mine, sh, turn);
-        if (m != -INFINITY) m = fmaf(-w.slope, (float)(mine - w.near), m);
     }
     float top[1] = {m};
     team_fold<FoldMax, kSweepThreads, kSweepThreads>(top, sh, turn);

@@ -82,14 +82,23 @@ def test_gate_gradients_that_need_no_second_launch(ct, cols, last):
 
 # ---- distance bias with documents ----------------------------------------------------------------------------
 def far_bound(s, p, rules):
-    """ref.score_bound with the bias counted from the nearest admitted key, documents among the rules or not."""
+    """|error| of a probability when the bias is counted from the nearest admitted key, documents among the rules or not.
+    As ref.score_bound, but key by key: a logit t of a value and a bias of together T is off by 8 U T, its difference x to the
+    maximum, rounded and multiplied by a rounded log2(e), by 3 U |x| more, an exponential by 4 U; a probability by
+    that of its own key, that of the sum (each key's weighted with its probability), and 79 U for sum, reciprocal and product."""
     ok = ref.admitted(s.shape, rules, s.device)
     bare = {k: v for k, v in rules.items() if k != "slopes"}
+    t = ref.logits(torch.where(ok, s, 0.0), bare)
     d = torch.where(ok, ref.distance(s.shape, rules, s.device), math.inf)
     near = d.amin(-1, keepdim=True)
     d = torch.where(ok, d - torch.where(near == math.inf, 0.0, near), 0.0)
-    T = torch.where(ok, ref.logits(torch.where(ok, s, 0.0), bare).abs(), 0.0) + rules["slopes"].double().abs()[None, :, None, None] * d
-    return p * U * (22.0 * T.amax(-1, keepdim=True) + 83.0) + 1e-37
+    bias = rules["slopes"].double()[None, :, None, None] * d
+    T = torch.where(ok, t.abs(), 0.0) + bias.abs()
+    x = torch.where(ok, t - bias, -math.inf)
+    top = x.amax(-1, keepdim=True)
+    x = torch.where(ok, torch.where(top == -math.inf, 0.0, top) - x, 0.0)
+    each = torch.where(ok, 8.0 * T + 3.0 * x + 4.0, 0.0)
+    return p * U * (each + (p * each).sum(-1, keepdim=True) + 79.0) + 1e-37
 
 
 def far_rules(g, H, Q, K):
@@ -132,3 +141,19 @@ def test_score_bias_of_far_documents_beyond_exact_floats(ct):
     t = s[..., 1001:1101].double() - 0.3000000119 * torch.arange(99, -1, -1, device=DEV)
     want = torch.softmax(t, -1)
     within(p[..., 1001:1101], want, want * U * (22.0 * t.abs().amax(-1, keepdim=True) + 83.0), "probabilities")
+
+
+@pytest.mark.parametrize("keys", [90, 1024, 1027, 5000, 16384, 30001, 120000])
+@pytest.mark.parametrize("causal", [False, True])
+def test_score_bias_in_packed_documents(ct, keys, causal):
+    """Queries inside their documents: the keys next to them, which have most of the weight, keep all their bits."""
+    g = gen(keys + 5)
+    B, H, Q = 1, 2, 8
+    s = randn(g, B, H, Q, keys)
+    docs = (torch.arange(keys, device=DEV, dtype=torch.int32) * 3 // keys)[None].contiguous()
+    at = keys - 3 * Q
+    rules = {"causal": causal, "query_docs": docs[:, at:at + Q].contiguous(), "key_docs": docs, "query_start": ints([at]),
+             "slopes": torch.tensor([0.5, 0.01], device=DEV)}
+    p = ct.score_softmax(s, ct.ScoreRules(**rules))
+    want = ref.score_softmax(s.double(), rules)
+    within(p, want, far_bound(s.double(), want, rules), "probabilities")
