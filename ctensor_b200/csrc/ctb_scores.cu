@@ -5,6 +5,10 @@
 //   D = sum_j p_j * dp_j,  ds_j = scale * (1 - tanh^2) * p_j * (dp_j - D)
 //   dslope = -sum_j |pos - j| * p_j * (dp_j - D)
 //
+// In both directions a row's distances are counted from the nearest of its keys: what they have in common changes no
+// probability, and in dslope it is multiplied by sum_j p_j * (dp_j - D) = 0 (left in, it would bring in D's rounding: slopes'
+// gradients of queries 3 million keys away were off by 1e-3).
+//
 // Causal, prefix and length rules admit a run of keys [0, live); only the document rule is decided key by
 // key.  Fours of keys without an admitted one are neither read nor evaluated, their results are written as
 // zeros ahead of the loads.
@@ -50,8 +54,7 @@ struct ScorePlace {
     uint32_t row, b, h, i;
     int live;                           // keys [0, live) may be admitted
     int centre;                         // the key position nearest to the query's within [0, live)
-    float beyond;                       // |pos - centre|
-    int near;                           // distances from `centre` are counted from here on in the bias
+    int near;                           // distances from `centre` are counted from here on
     float slope;
     int doc;
 };
@@ -74,11 +77,10 @@ __device__ __forceinline__ ScorePlace score_place(const ScoreArgs& a, ScoreRow r
     }
     w.live = max(w.live, 0);
     w.centre = 0;
-    w.beyond = w.slope = 0.0f;
+    w.slope = 0.0f;
     w.near = 0;
     if (g.slopes) {
         w.centre = (int)max(min(pos, (int64_t)w.live - 1), (int64_t)0);
-        w.beyond = (float)(pos > w.centre ? pos - w.centre : w.centre - pos);
         w.slope = g.slopes[w.h * g.slope_stride];
     }
     w.doc = g.query_docs.p ? g.query_docs.p[w.b * g.query_docs.sb + w.i * g.query_docs.si] : 0;
@@ -211,12 +213,28 @@ __device__ __forceinline__ void score_logits(const ScoreGeom& g, const ScorePlac
         }
     }
 }
+// Whether the key at the centre is of another document than the query, which is rare: [8,12,1024,1024] with slopes and 5
+// documents 79.5 us and its gradients 142, 80.6 and 155 when every row looks for its nearest key; 512 rows of 40000, swept,
+// 399 us, 484 far from their documents.  The same in all lanes of a warp.
+template <int T>
+__device__ __forceinline__ bool score_apart(const ScoreDocs& docs, const ScorePlace& w) {
+    const bool apart = docs.p[w.centre * docs.si] != w.doc;
+    return T < 32 ? __any_sync(0xFFFFFFFFu, apart) : apart;
+}
 // The smallest of the team's distances (kNoKey: none), the same in every thread; beyond 2^24 to Float32, which is as good.
 template <int THREADS, int T>
 __device__ __forceinline__ int score_near(int near, TeamSlots<THREADS, 1, float>& sh, FoldTurn& turn) {
     float most[1] = {near == kNoKey ? -INFINITY : -(float)near};
     team_fold<FoldMax, THREADS, T>(most, sh, turn);
     return most[0] == -INFINITY ? 0 : (int)-most[0];
+}
+// sum + the distances times r, over a four's columns
+template <bool DOCS>
+__device__ __forceinline__ float score_slope(const ScorePlace& w, float sum, int c0, const float (&r)[4]) {
+    const float from = (float)(c0 - w.centre);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum = fmaf(DOCS ? (float)(abs(c0 + k - w.centre) - w.near) : fabsf(from + (float)k), r[k], sum);
+    return sum;
 }
 template <bool CAP>
 __device__ __forceinline__ void score_slow(const ScoreGeom& g, float (&r)[4], const float* s) {     // r *= scale * (1 - tanh^2)
@@ -375,7 +393,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     float t[NV][4];
     mine.load(t, s, score_phase(s) == phase);
     FoldTurn turn = entry.met();
-    if (DOCS && a.g.slopes) w.near = score_near<THREADS, T>(mine.nearest(w), sh, turn);
+    if (DOCS && a.g.slopes && score_apart<T>(score_docs<DOCS>(a, w, phase), w)) w.near = score_near<THREADS, T>(mine.nearest(w), sh, turn);
     float m[1] = {-INFINITY};
     mine.each([&](int j, const auto& o) {
         score_logits<CAP, DOCS>(a.g, w, t[j], o.column());
@@ -426,7 +444,7 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     const ScoreRow place = score_row_of<THREADS, T>(a, cs);
     if (T >= 32 && !place.present) return;
     const int64_t row = place.row;
-    const ScorePlace w = score_place(a, place);
+    ScorePlace w = score_place(a, place);
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
@@ -453,6 +471,7 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
     });
     float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
     FoldTurn turn = entry.met();
+    if (DOCS && a.slope_part && score_apart<T>(score_docs<DOCS>(a, w, phase), w)) w.near = score_near<THREADS, T>(mine.nearest(w), sh, turn);
     team_fold<FoldSum, THREADS, T>(d, sh, turn);
     const bool usual = fabsf(d[0]) < INFINITY;           // else 0 * (0 - D) is NaN in the masked columns
     float slope_sum = 0.0f;
@@ -463,11 +482,7 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
             r[k] = p[j][k] * (dp[j][k] - d[0]);
             if (!usual && !o.has(k)) r[k] = 0.0f;
         }
-        if (a.slope_part) {
-            const float from = (float)(o.column() - w.centre);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) slope_sum = fmaf(fabsf(from + (float)k) + w.beyond, r[k], slope_sum);
-        }
+        if (a.slope_part) slope_sum = score_slope<DOCS>(w, slope_sum, o.column(), r);
         score_slow<CAP>(a.g, r, s[CAP ? j : 0]);
         mine.store(out, o.column(), span.end, r);
     });
@@ -483,29 +498,21 @@ score_softmax_backward_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
 constexpr int kSweepThreads = 512;
 constexpr int kSweepBatch = 4;                           // fours in flight per thread and operand
 
-// The smallest distance of an admitted key from the centre, looked for outwards from there by every CTA of the row for
-// itself: one step for a query next to its document, a pass over the documents for one far away (512 rows of 40000 keys, four
-// of five queries far from theirs, 481 us; without slopes 383).
-__device__ __forceinline__ int sweep_near(const ScoreDocs& docs, const ScorePlace& w, TeamSlots<kSweepThreads, 1, float>& sh, FoldTurn& turn) {
-    const int farthest = max(w.centre, w.live - 1 - w.centre);
-    int near = kNoKey;
-    for (int from = 0; from <= farthest; from += kSweepThreads * kSweepBatch) {
-#pragma unroll
-        for (int u = 0; u < kSweepBatch; ++u) {
-            const int d = from + u * kSweepThreads + (int)threadIdx.x;
-            const bool before = d <= w.centre && w.live > 0, behind = d < w.live - w.centre;
-            if ((before && docs.p[(w.centre - d) * docs.si] == w.doc) || (behind && docs.p[(w.centre + d) * docs.si] == w.doc)) near = min(near, d);
-        }
-        if (__syncthreads_or(near != kNoKey)) break;
-    }
-    return score_near<kSweepThreads, kSweepThreads>(near, sh, turn);
-}
-
 struct SweepSpan { int64_t lo, hi; };
 __device__ __forceinline__ SweepSpan sweep_span(int64_t keys, int phase, int cs) {
     const int64_t fours = (keys + phase + 3) / 4, share = (fours + cs - 1) / cs;
     const int64_t lo = share * (cs > 1 ? cluster_rank() : 0);
     return {lo, min(fours, lo + share)};
+}
+
+// The smaller one of `near` and the distances of a four's admitted keys from the centre.
+__device__ __forceinline__ int nearest_of_four(const ScorePlace& w, int near, int c0, uint32_t bits) {
+    if (bits) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if ((bits >> k) & 1u) near = min(near, abs(c0 + k - w.centre));
+    }
+    return near;
 }
 
 template <bool CAP, bool DOCS>
@@ -524,7 +531,20 @@ score_softmax_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs) {
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
     FoldTurn turn = entry.met();
-    if (DOCS && a.g.slopes) w.near = sweep_near(docs, w, sh, turn);
+    if (DOCS && a.g.slopes && score_apart<kSweepThreads>(docs, w)) {         // a pass over the documents alone
+        int near = kNoKey;
+        for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
+            uint32_t bits[kSweepBatch];
+#pragma unroll
+            for (int u = 0; u < kSweepBatch; ++u) {
+                const int64_t at = f + (int64_t)u * kSweepThreads;
+                bits[u] = at < live_end ? score_admitted<DOCS, true>(docs, w, (int)(at * 4) - phase) : 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < kSweepBatch; ++u) near = nearest_of_four(w, near, (int)((f + (int64_t)u * kSweepThreads) * 4) - phase, bits[u]);
+        }
+        w.near = score_near<kSweepThreads, kSweepThreads>(near, sh, turn);
+    }
     // first sweep: the thread's maximum and its sum of exponentials relative to that maximum
     float m = -INFINITY, z = 0.0f;
     for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
@@ -601,7 +621,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     __shared__ TeamSlots<kSweepThreads, 1, float> sh;
     __shared__ TeamSlots<kSweepThreads, 1, double> sh_slope;
     const int64_t row = blockIdx.x / cs;
-    const ScorePlace w = score_place(a, {(uint32_t)row, true});
+    ScorePlace w = score_place(a, {(uint32_t)row, true});
     const int keys = (int)a.g.keys;
     float* out = a.out + row * (int64_t)keys;
     const float *pr = score_row(a.p, w), *gr = score_row(a.dp, w), *sr = CAP ? score_row(a.s, w) : nullptr;
@@ -610,6 +630,8 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     const ScoreDocs docs = score_docs<DOCS>(a, w, phase);
     const SweepSpan span = sweep_span(keys, phase, cs);
     const int64_t live_end = min(span.hi, ((int64_t)w.live + phase + 3) / 4);
+    const bool apart = DOCS && a.slope_part && score_apart<kSweepThreads>(docs, w);
+    int near = kNoKey;
     float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int64_t f = span.lo + threadIdx.x; f < live_end; f += kSweepThreads * kSweepBatch) {
         float p[kSweepBatch][4], dp[kSweepBatch][4];
@@ -620,6 +642,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
             const uint32_t bits = at < live_end ? score_admitted<DOCS, false>(docs, w, c0) : 0u;
             score_load(p[u], pr, c0, bits, p_aligned);
             score_load(dp[u], gr, c0, bits, g_aligned);
+            if (apart) near = nearest_of_four(w, near, c0, bits);
         }
 #pragma unroll
         for (int u = 0; u < kSweepBatch; ++u)
@@ -628,6 +651,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
     }
     float d[1] = {(part[0] + part[1]) + (part[2] + part[3])};
     FoldTurn turn = entry.met();
+    if (apart) w.near = score_near<kSweepThreads, kSweepThreads>(near, sh, turn);
     team_fold<FoldSum, kSweepThreads, kSweepThreads>(d, sh, turn);
     double slope_sum = 0.0;
     for (int64_t f = span.lo + threadIdx.x; f < span.hi; f += kSweepThreads * kSweepBatch) {
@@ -652,11 +676,7 @@ score_softmax_backward_sweep_kernel(const __grid_constant__ ScoreArgs a, int cs)
             if (bits[u]) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) r[k] = (bits[u] >> k) & 1u ? p[u][k] * (dp[u][k] - d[0]) : 0.0f;
-                if (a.slope_part) {
-                    const float from = (float)(c0 - w.centre);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) slope_part = fmaf(fabsf(from + (float)k) + w.beyond, r[k], slope_part);
-                }
+                if (a.slope_part) slope_part = score_slope<DOCS>(w, slope_part, c0, r);
                 score_slow<CAP>(a.g, r, s[u]);
             }
             score_store(out, c0, keys, r);

@@ -437,7 +437,8 @@ int ctb_score_softmax(const ctb_view* scores, const ctb_score_rules* rules, cons
 /* grad_scores = scale * (1 - tanh^2) * p * (grad - sum_j p * grad) at the admitted keys, 0 elsewhere (`grad`
  * and `probs` are not looked at there).  `probs`: what ctb_score_softmax returned; `scores` is needed when
  * cap > 0 and may be NULL otherwise.  grad_slopes (may be NULL): Float32 [heads], contiguous,
- *   grad_slopes[h] = -sum over b, i, j of |pos - j| * p * (grad - sum_j p * grad).
+ *   grad_slopes[h] = -sum over b, i, j of |pos - j| * p * (grad - sum_j p * grad)
+ * (a row's distances counted from its nearest key: its probabilities add up to 1, so the rest drops out).
  * `workspace`: 256-byte aligned device memory of ctb_score_softmax_workspace_bytes(probs) bytes, used for
  * grad_slopes only; NULL: the library's per-device workspace (see ctb_reduce). */
 size_t ctb_score_softmax_workspace_bytes(const ctb_view* probs);

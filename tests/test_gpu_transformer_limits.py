@@ -157,3 +157,32 @@ def test_score_bias_in_packed_documents(ct, keys, causal):
     p = ct.score_softmax(s, ct.ScoreRules(**rules))
     want = ref.score_softmax(s.double(), rules)
     within(p, want, far_bound(s.double(), want, rules), "probabilities")
+
+@pytest.mark.parametrize("keys", [60, 700, 1001, 5000, 16384, 30001, 120000])
+@pytest.mark.parametrize("docs", [False, True])
+def test_slope_gradients_of_far_keys(ct, keys, docs):
+    """A row's gradients of the logits add up to nothing, so the distance that all of its keys have in common does not
+    count.  Probabilities that are multiples of 1/16 and add up to exactly one, so that it does not count in the
+    formula in 64 bits either."""
+    g = gen(keys + 1)
+    B, H, Q = 2, 2, 3
+    rules = far_rules(g, H, Q, keys) if docs else {"slopes": torch.rand(H, device=DEV, generator=g)}
+    if not docs:
+        rules["query_start"] = ints([3_000_000, -1_000_000])
+    ok = ref.admitted((B, H, Q, keys), rules, DEV).expand(B, H, Q, keys)
+    p = torch.zeros(B, H, Q, keys, device=DEV)
+    for b in range(B):
+        for h in range(H):
+            for q in range(Q):
+                allowed = ok[b, h, q].nonzero()[:, 0]
+                if len(allowed):
+                    pick = allowed[torch.randint(0, len(allowed), (16,), device=DEV, generator=g)]
+                    p[b, h, q].index_put_((pick,), torch.full((16,), 1 / 16, device=DEV), accumulate=True)
+    dp = randn(g, B, H, Q, keys)
+    ds, dslopes = ct.score_softmax_backward(dp, p, ct.ScoreRules(**rules), want_slopes=True)
+    w, ws, bound, _ = ref.score_gradients(p.double(), p.double(), dp.double(), rules)
+    within(ds, w, bound, "score gradients")
+    d = torch.where(ok, ref.distance(p.shape, rules, DEV), math.inf)
+    near = d.amin(-1, keepdim=True)
+    d = torch.where(ok, d - torch.where(near == math.inf, 0.0, near), 0.0)
+    within(dslopes, ws, (d * (bound + 36.0 * U * w.abs())).sum((0, 2, 3)) + 2 * U * ws.abs(), "slope gradients")
