@@ -46,3 +46,20 @@ def ct():
         pytest.skip("no CUDA device")
     ctensor_b200.lib()
     return ctensor_b200
+
+
+@pytest.fixture(autouse=True)
+def views_outlive_their_calls(request, monkeypatch):
+    """Where a test module hands out the bare address of a view (its function `address`), the view lives as long as the
+    test: an argument written in place, `params(pre_weight=Arr((7,)))`, would else be freed ahead of the call that reads it."""
+    address = getattr(request.module, "address", None)
+    if address is None:
+        yield
+        return
+    kept = []
+
+    def keep(x):
+        kept.append(x)
+        return address(x)
+    monkeypatch.setattr(request.module, "address", keep)
+    yield
