@@ -349,8 +349,11 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
 //     sum(k dx fhat) = sum(k e fhat) - rstd_y * (m1 * sum(k fhat) + m2 * sum(k fhat yhat))
 // and all eight sums are taken together.  Without a LayerNorm (m1 and the mean of k dx drop out) three remain.
 //
-// Column sums (weights, biases, a gate shared by rows) stay in registers until the team's last row — a shared
-// gate's until its last row in the team — and go out as partials, which a second launch adds in order.
+// Column sums (weights, biases, a gate shared by rows) stay in registers, as Float32, until the team's last row — a shared
+// gate's until its last row in the team — and go out as partials, which a second launch adds in order, in fp64.  A
+// team has at most kTeamRows rows and a CTA at most 16 teams, so that a sum is off by no more than 256 half steps however many
+// rows there are: beyond it there are several times as many CTAs as run at once ([1000000,128] 487 us, 481 with teams of 422 rows).
+// (Sums of a CTA's teams in fp64 would add 0.7 us to [8192,768]'s 30.8.)
 enum { kInY = 0, kInDh = 1, kInDy = 2, kInF = 3, kInGate = 4, kInCount = 5 };
 
 struct ResidualBwd {
@@ -901,10 +904,11 @@ BwdShape bwd_shape(int64_t cols, BwdKind kind) {
     if ((small || kind == kBwdFull) && cs <= kMaxCluster) return {in_cluster, in_cluster, cs, 2};
     return {alone, alone, cluster_for(cols, alone * kBwdShare), 1};
 }
-// Teams that walk the rows, at most one per row: `ctas` CTAs (clusters) run at once.
+// Teams that walk the rows, at most one per row and at most kTeamRows rows each: `ctas` CTAs (clusters) run at once.
+constexpr int64_t kTeamRows = 240;
 int64_t bwd_teams(int64_t rows, const BwdShape& s, int64_t ctas) {
-    const int64_t teams = ctas * (s.threads / s.team);
-    return teams > rows ? rows : (teams < 1 ? 1 : teams);
+    const int64_t at_once = ctas * (s.threads / s.team), teams = at_once < 1 ? 1 : at_once;
+    return teams > rows ? rows : teams * ceil_div(rows, teams * kTeamRows);
 }
 constexpr int kMaxSms = 256;                             // what the size query, which names no device, allows for
 
@@ -974,7 +978,9 @@ size_t residual_norm_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_gr
     int64_t teams = 0, parts = 0;
     for (BwdKind kind : {kBwdLean, kBwdFullPre, kBwdFull, kBwdScalarPre, kBwdScalar, kBwdAny}) {
         const BwdShape shape = bwd_shape(cols, kind);
-        const int64_t t = bwd_teams(rows, shape, (int64_t)kMaxSms * shape.ctas / shape.cs), p = ceil_div(t, (int64_t)(shape.threads / shape.team));
+        // no more than this, however many of them run at once
+        const int64_t most = (int64_t)kMaxSms * shape.ctas / shape.cs * (shape.threads / shape.team) + ceil_div(rows, kTeamRows);
+        const int64_t t = most > rows ? rows : most, p = ceil_div(t, (int64_t)(shape.threads / shape.team));
         teams = t > teams ? t : teams;
         parts = p > parts ? p : parts;
     }

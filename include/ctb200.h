@@ -471,7 +471,7 @@ int ctb_residual_norm(const ctb_view* x, const ctb_view* f, const ctb_view* gate
  * gradients of y and h.  grad_y may be NULL (zero) unless pre_kind is CTB_NORM_NONE, whose grad_h is NULL.
  * Every member of `grads` may be NULL (not wanted); x, f: contiguous, the rows' shape; gate: contiguous, the
  * gate's shape (summed over the dims in which it was broadcast); weights and biases: [cols].  Column sums are
- * Float32 within up to a few thousand rows of one team and fp64 across teams, always in the same order.
+ * Float32 over at most 240 consecutive rows and over up to 16 such sums, fp64 beyond, always in the same order.
  * `workspace`: 256-byte aligned device memory of at least ctb_residual_norm_workspace_bytes(y, gate) bytes
  * (gate as given to the call); NULL: the library's per-device workspace (see ctb_reduce). */
 typedef struct ctb_residual_norm_grads {

@@ -186,3 +186,50 @@ def test_slope_gradients_of_far_keys(ct, keys, docs):
     near = d.amin(-1, keepdim=True)
     d = torch.where(ok, d - torch.where(near == math.inf, 0.0, near), 0.0)
     within(dslopes, ws, (d * (bound + 36.0 * U * w.abs())).sum((0, 2, 3)) + 2 * U * ws.abs(), "slope gradients")
+
+
+# ---- column sums over very many rows ---------------------------------------------------------------------------
+@pytest.mark.parametrize("what", ["bias", "gate", "all"])
+@pytest.mark.parametrize("rows,cols", [(3_700_001, 4), (2_000_001, 68), (400_000, 260)])
+def test_column_sums_over_many_rows(ct, what, rows, cols):
+    """Ones among which every thousandth is 2^24: a Float32 sum that has met one of those loses the ones that follow.  At most
+    240 rows and up to 16 such sums are added in Float32 (239 U + 15 U), the result is rounded (U)."""
+    values = torch.ones(rows, 1, device=DEV)
+    values[::1000] = 2.0 ** 24
+    incoming = values.expand(rows, cols).contiguous()
+    want = float(values.double().sum())
+    one = torch.ones(cols, device=DEV)
+    x = randn(gen(rows), rows, cols)
+    near = lambda got: within(got, torch.full((cols,), want, device=DEV, dtype=torch.float64), torch.full((cols,), 260 * U * want, device=DEV, dtype=torch.float64), what)
+    if what == "bias":
+        params = ct.ResidualNorm(pre=1, pre_weight=one, pre_bias=one)
+        _, _, stats = ct.residual_norm(x, None, params)
+        near(ct.residual_norm_backward(None, x, stats, params, grad_h=incoming).pre_bias)
+    elif what == "gate":
+        params = ct.ResidualNorm(pre=0)
+        f = torch.ones_like(x)
+        y, _, stats = ct.residual_norm(x, f, params, gate=one)
+        near(ct.residual_norm_backward(f, y, stats, params, grad_y=incoming, gate=one).gate)
+    else:
+        params = ct.ResidualNorm(pre=1, pre_weight=one, pre_bias=one, post=1, post_weight=one, post_bias=one)
+        y, _, stats = ct.residual_norm(x, x, params, gate=one)
+        near(ct.residual_norm_backward(x, y, stats, params, grad_y=x, grad_h=incoming, gate=one).pre_bias)
+
+
+@pytest.mark.parametrize("gate", ["batch", "sequence", "token", "channel"])
+@pytest.mark.parametrize("cols", [36, 7])
+def test_more_teams_than_run_at_once(ct, gate, cols):
+    """So many rows that teams come in several waves: gate rows shared inside and across teams, every gradient."""
+    g = gen(cols)
+    B, T = 1003, 1201
+    x, f, dy, dh = (randn(g, B, T, cols) for _ in range(4))
+    w = [1 + 0.3 * randn(g, cols) for _ in range(2)]
+    shape = {"batch": (B, 1, cols), "sequence": (B, 1, 1), "token": (B, T, 1), "channel": (cols,)}[gate]
+    gate = randn(g, *shape)
+    params = ct.ResidualNorm(pre=2, pre_weight=w[0], post=2, post_weight=w[1], scale=0.5)
+    y, _, stats = ct.residual_norm(x, f, params, gate=gate)
+    got = ct.residual_norm_backward(f, y, stats, params, grad_y=dy, grad_h=dh, gate=gate)
+    want = ref.residual_norm_gradients(f.double(), y.double(), (2, w[0].double(), None), (2, w[1].double(), None), gate.double(), 0.5, dy.double(), dh.double())
+    for name in ("x", "f", "gate", "post_weight", "pre_weight"):
+        value, bound = want[name]
+        within(getattr(got, name), value, bound + 1e-36, "gradient of " + name)
