@@ -246,8 +246,10 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
 //     sum(y^2) = sum(x^2) + 2 rstd_f sum(x u) + rstd_f^2 sum(u^2)
 // and all four sums (fp64) are known after one pass over x and f.  (A bias behind the first norm would have to be
 // rounded into x before that norm is known, one rounding more; such rows take the general kernel.)  Where the block's output cancels the stream to
-// less than a thousandth, those sums would lose what the norm magnifies: such a row takes the second fold.  For rows of up to 2048 columns: [16384, 1536]
-// 69 us against 74; wider rows, which hold more of it per thread, lose ([4096, 4096] 60 against 52).
+// less than a thousandth, those sums would lose what the norm magnifies: such a row takes the second fold; so does a row near
+// the ends of Float32, whose u overflows or is subnormal where n itself is neither, and it is normed before it is scaled.  For
+// rows of up to 2048 columns: [16384, 1536] 69 us against 74; wider rows, which hold more of it per thread, lose ([4096, 4096]
+// 60 against 52).
 template <int THREADS, int T, int E, int VEC>
 __global__ void __launch_bounds__(THREADS, 4)
 residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ y, float* __restrict__ h, float* __restrict__ stats) {
@@ -297,45 +299,78 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
     const float rf = inverse_root(s[0] * g.inv_cols + (double)g.post_eps);
     const double r = rf;
     double sy = fma(r, fma(r, s[3], 2.0 * s[2]), s[1]);
-    if (sy < 1e-6 * s[1]) {                              // the same in every thread of the team
+    // y = x + by * u and its norm; `sy`: the sum of its squares
+    auto finish = [&](float by) {
+        const float ry = inverse_root(sy * g.inv_cols + (double)g.pre_eps);
+#pragma unroll
+        for (int i = 0; i < E / VEC; ++i) {
+            const int c = col_of<T, VEC>(i, tid);
+            if (c < width) {
+                float out[VEC];
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) out[q] = fmaf(by, u[i * VEC + q], xv[i * VEC + q]);
+                store_part<VEC>(y + row * g.cols, c, out);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) out[q] = out[q] * ry;
+                if (g.pre_weight) {
+                    float w[VEC];
+                    load_part<T, VEC>(w, g.pre_weight, c);
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) out[q] = out[q] * w[q];
+                }
+                if (g.pre_bias) {
+                    float w[VEC];
+                    load_part<T, VEC>(w, g.pre_bias, c);
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) out[q] = out[q] + w[q];
+                }
+                store_part<VEC>(h + row * g.cols, c, out);
+            }
+        }
+        if (stats && tid == 0) *reinterpret_cast<float4*>(stats + row * 4) = make_float4(0.0f, rf, 0.0f, ry);
+    };
+    auto fold_again = [&](float by) {
         double square = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const double d = col_of<T, VEC>(e / VEC, tid) < width ? fmaf(rf, u[e], xv[e]) : 0.0f;
+            const double d = col_of<T, VEC>(e / VEC, tid) < width ? fmaf(by, u[e], xv[e]) : 0.0f;
             square = fma(d, d, square);
         }
         s[0] = square;
         s[1] = s[2] = s[3] = 0.0;
         team_fold<FoldSum, THREADS, T>(s, sh, turn);
         sy = s[0];
-    }
-    const float ry = inverse_root(sy * g.inv_cols + (double)g.pre_eps);
+    };
+    // (both conditions are the same in every thread of the team)
+    if (s[0] < INFINITY && (!(s[3] < INFINITY) || rf > 1048576.0f)) {
+        load_share<T, E, VEC>(u, f.p + row * f.stride, width, tid);
+        const float* const row_gate = g.gate.p + (int64_t)fast_div((uint32_t)row, g.by_gate_rows) * g.gate.stride;
+        const float by = g.gate_mode == kGateScalar ? row_gate[0] * g.scale : g.scale;
 #pragma unroll
-    for (int i = 0; i < E / VEC; ++i) {
-        const int c = col_of<T, VEC>(i, tid);
-        if (c < width) {
-            float out[VEC];
+        for (int i = 0; i < E / VEC; ++i) {
+            const int c = col_of<T, VEC>(i, tid);
+            if (c < width) {
+                float k[VEC];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) out[q] = fmaf(rf, u[i * VEC + q], xv[i * VEC + q]);
-            store_part<VEC>(y + row * g.cols, c, out);
+                for (int q = 0; q < VEC; ++q) u[i * VEC + q] = u[i * VEC + q] * rf;
+                if (g.post_weight) {
+                    load_part<T, VEC>(k, g.post_weight, c);
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) out[q] = out[q] * ry;
-            if (g.pre_weight) {
-                float w[VEC];
-                load_part<T, VEC>(w, g.pre_weight, c);
+                    for (int q = 0; q < VEC; ++q) u[i * VEC + q] = u[i * VEC + q] * k[q];
+                }
+                if (g.gate_mode == kGateRow) {
+                    load_part<T, VEC>(k, row_gate, c);
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) out[q] = out[q] * w[q];
+                    for (int q = 0; q < VEC; ++q) u[i * VEC + q] = u[i * VEC + q] * k[q];
+                }
             }
-            if (g.pre_bias) {
-                float w[VEC];
-                load_part<T, VEC>(w, g.pre_bias, c);
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) out[q] = out[q] + w[q];
-            }
-            store_part<VEC>(h + row * g.cols, c, out);
         }
+        fold_again(by);
+        finish(by);
+        return;
     }
-    if (stats && tid == 0) *reinterpret_cast<float4*>(stats + row * 4) = make_float4(0.0f, rf, 0.0f, ry);
+    if (sy < 1e-6 * s[1]) fold_again(rf);
+    finish(rf);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------

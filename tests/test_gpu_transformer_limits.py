@@ -233,3 +233,29 @@ def test_more_teams_than_run_at_once(ct, gate, cols):
     for name in ("x", "f", "gate", "post_weight", "pre_weight"):
         value, bound = want[name]
         within(getattr(got, name), value, bound + 1e-36, "gradient of " + name)
+
+
+# ---- norms of rows near the ends of Float32 -------------------------------------------------------------------
+@pytest.mark.parametrize("cols", [20, 33, 768, 1001, 2048, 2052, 4100])
+@pytest.mark.parametrize("gate", ["none", "full", "token"])
+@pytest.mark.parametrize("size,weight", [(1e37, 50.0), (1e20, 1e20), (1e-30, 1e-12), (1e-38, 1.0)])
+def test_rms_norms_of_extreme_rows(ct, cols, gate, size, weight):
+    """Whatever the rows' size, only their direction counts: y, the next norm and df are those of rows of ordinary size."""
+    g = gen(cols)
+    B, T = 2, 3
+    f = randn(g, B, T, cols) * size
+    f[0, 0] = randn(g, cols)                             # an ordinary row among them
+    shape = {"none": None, "full": (B, T, cols), "token": (B, T, 1)}[gate]
+    gate = None if shape is None else randn(g, *shape).abs() + 0.5
+    w = (1.0 + torch.rand(cols, device=DEV, generator=g)) * weight
+    x = torch.zeros_like(f)
+    params = ct.ResidualNorm(pre=2, pre_eps=0.0, post=2, post_weight=w, post_eps=0.0, scale=0.5)
+    y, h, stats = ct.residual_norm(x, f, params, gate=gate)
+    n = ref.normed(f.double(), 2, w.double(), None, 0.0)
+    factor = 0.5 if gate is None else 0.5 * gate.double()
+    want = factor * n
+    within(y, want, abs(factor) * ref.norm_bound(f.double(), 2, w.double(), None, 0.0) + 4 * U * want.abs(), "y")
+    want = ref.normed(y.double(), 2, None, None, 0.0)
+    within(h, want, ref.norm_bound(y.double(), 2, None, None, 0.0) + U * want.abs(), "h")
+    _, rstd = ref.row_numbers(f.double(), 2, 0.0)
+    within(stats[..., 1], rstd[..., 0], 3 * U * rstd[..., 0], "rstd")
