@@ -187,8 +187,9 @@ __device__ __forceinline__ void score_store(float* row, int c0, int keys, const 
 }
 
 // e^x = 2^(x log2 e).  x is a difference of logits (were the logits themselves kept in units of log 2, a row of
-// the type's lowest values would overflow).  The instruction's relative error is below 2^-22, results below
-// 2^-126 are 0.
+// the type's lowest values would overflow).  Not the most exact form: the product's rounding is |x| half steps of the
+// result, as many as the difference x itself brings along, the constant's a quarter of that, and the instruction's relative error
+// is below 2^-22 (4 half steps).  Results below 2^-126 are 0.
 __device__ __forceinline__ float score_exp(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));

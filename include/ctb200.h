@@ -423,7 +423,8 @@ int ctb_optimizer_step(int kind, const ctb_view* param, const ctb_view* grad, fl
  * initialised).  A query that is admitted to no key, or only to scores of -inf, gets a row of zeros.
  * An admitted NaN or +inf makes its row NaN in the admitted places, as the formula says.
  * Unlike ctb_softmax_lastdim, whose mask and exponential follow the reference's chain, masked places are
- * left out rather than lowered, and the exponential is the accurate one.
+ * left out rather than lowered, and e^x of a difference x to the row's maximum is within 1.25 |x| + 4 half steps
+ * of Float32 (each 2^-24 of the result), or 0 where it is below 2^-126.
  * Every pointer of ctb_score_rules may be NULL (that rule is then absent; query_docs and key_docs come
  * together): query_start, key_lengths, prefix: Int32 [batch]; query_docs: Int32 [batch, queries];
  * key_docs: Int32 [batch, keys]; slopes: Float32 [heads]; any strides.  Values outside 0..keys mean what

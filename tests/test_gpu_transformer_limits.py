@@ -259,3 +259,20 @@ def test_rms_norms_of_extreme_rows(ct, cols, gate, size, weight):
     within(h, want, ref.norm_bound(y.double(), 2, None, None, 0.0) + U * want.abs(), "h")
     _, rstd = ref.row_numbers(f.double(), 2, 0.0)
     within(stats[..., 1], rstd[..., 0], 3 * U * rstd[..., 0], "rstd")
+
+
+# ---- the exponential ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("keys", [2, 1026, 20001])
+def test_score_exponential(ct, keys):
+    """Differences x that are exact, from 1/8 to where results end: e^x within 1.25 |x| + 4 half steps, the
+    sum of two, reciprocal and product one more each."""
+    x = torch.arange(1, 8 * 104, device=DEV) / 8.0
+    s = torch.full((1, 1, len(x), keys), -math.inf, device=DEV)
+    s[0, 0, :, 0], s[0, 0, :, keys - 1] = 0.0, -x
+    p = ct.score_softmax(s, ct.ScoreRules())[0, 0]
+    e = torch.exp(-x.double())
+    each = 1.25 * x.double() + 4
+    want = e / (1 + e)
+    slack = torch.where(e < 2.0 ** -125, 2.0 ** -125, 0.0)
+    within(p[:, keys - 1], want, want * U * (each + each * e + 8) + slack, "the smaller one")
+    within(p[:, 0], 1 / (1 + e), U * (each * e + 8), "the larger one")
