@@ -10,6 +10,7 @@
 #include <memory>
 #include <mutex>
 #include <set>
+#include <tuple>
 
 #include "include/ctb_host.h"
 #include "include/ops_dispatch.h"
@@ -366,12 +367,12 @@ void zero_grad(Tensor& param) {
 
 double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, double p) {
     std::map<int, std::vector<ctb_view>> by_device;
-    std::set<const void*> seen;
+    std::set<std::tuple<const void*, size_t, size_t>> seen;      // slices of one buffer count each
     for (const Tensor* param : params) {
         if (!param || !has_grad(*param)) continue;
         Tensor g;
         g.impl = param->impl->grad;
-        if (g.numel() == 0 || !seen.insert(g.impl->data->data.get()).second) continue;
+        if (g.numel() == 0 || !seen.insert({g.impl->data->data.get(), g.impl->offset, g.numel()}).second) continue;
         by_device[device_index_of(g.device())].push_back(view_of(g, "clip_grad_norm"));
     }
     if (by_device.empty()) by_device[g_device];

@@ -9,6 +9,7 @@
 #include <cstring>
 #include <mutex>
 #include <set>
+#include <tuple>
 
 #include "include/ctb_gen1.h"
 #include "include/opsmp.h"
@@ -218,10 +219,11 @@ double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, doubl
         cell = (double*)q;
     }
     std::vector<ctb_view> views;
-    std::set<const void*> seen;
+    std::set<std::tuple<const void*, int64_t, size_t>> seen;     // slices of one buffer count each
     for (const Tensor* param : params) {
         if (!param || !has_grad(*param) || param->numel() == 0) continue;
-        if (seen.insert(param->impl->storage->grad.get()).second) views.push_back(grad_view_of(*param));
+        const ctb_view g = grad_view_of(*param);
+        if (seen.insert({g.base, g.offset, param->numel()}).second) views.push_back(g);
     }
     std::vector<const ctb_view*> list;
     for (const ctb_view& v : views) list.push_back(&v);

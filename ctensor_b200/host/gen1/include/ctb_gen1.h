@@ -44,7 +44,7 @@ void optimizer_step(ctb_opt::Kind kind, Tensor& param, float* state1, float* sta
 // Clears the gradient buffer on the GPU (Optimizer::zero_grad, root train_utils.h:37-44).
 void zero_grad(Tensor& param);
 // What Optimizer::clip_grad_norm does with its parameters (null ones and those without a gradient
-// buffer are passed over, a buffer that several share counts once).
+// buffer are passed over, a gradient that several share counts once, slices of one buffer count each).
 double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, double p);
 
 }  // namespace ctb_gen1

@@ -116,7 +116,8 @@ void optimizer_step(OptimizerKind kind, Tensor& param, float* state1, float* sta
 // Clears the parameter's gradient buffer on the GPU (Optimizer::zero_grad, :37-46).
 void zero_grad(Tensor& param);
 // What Optimizer::clip_grad_norm does with its parameters (null ones and those without a gradient
-// buffer are passed over, a buffer that several share counts once; on several GPUs too).
+// buffer are passed over, a gradient that several share counts once, slices of one buffer count each; on
+// several GPUs too).
 double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, double p);
 
 // Hook behind Tensor::backward(); the autograd library installs its backward(root) here.
