@@ -246,17 +246,39 @@ int32_t* bad_label_flag(int index) {
     return (int32_t*)flags[index].get();
 }
 std::vector<size_t> broadcast_of(const Tensor& a, const Tensor& b) { return broadcast_shape(a, b); }
-// One double per device and host thread that a norm is written to (managed: the host reads it).
-double* norm_cell(int index) {
-    static thread_local std::vector<std::shared_ptr<void>> cells;
-    if ((int)cells.size() <= index) cells.resize(index + 1);
-    if (!cells[index]) {
+// A double that one call's norm is written to (managed: the host reads it).  Cells go back to a list per device, so
+// there are never more of them than calls at once, however many threads come and go.
+class NormCell {
+public:
+    explicit NormCell(int index) : index_(index) {
+        {
+            std::lock_guard<std::mutex> lk(mutex());
+            std::vector<double*>& idle = cells()[index_];
+            if (!idle.empty()) {
+                at_ = idle.back();
+                idle.pop_back();
+                return;
+            }
+        }
         void* p = nullptr;
         check(ctb_alloc_managed(&p, sizeof(double), /*zero=*/1));
-        cells[index] = std::shared_ptr<void>(p, [](void*) {});           // lives as long as the thread's context
+        at_ = (double*)p;
     }
-    return (double*)cells[index].get();
-}
+    ~NormCell() {
+        std::lock_guard<std::mutex> lk(mutex());
+        cells()[index_].push_back(at_);
+    }
+    NormCell(const NormCell&) = delete;
+    NormCell& operator=(const NormCell&) = delete;
+    double* get() const { return at_; }
+
+private:
+    // never destroyed: a thread may still clip while the process ends
+    static std::mutex& mutex() { static std::mutex& m = *new std::mutex; return m; }
+    static std::map<int, std::vector<double*>>& cells() { static auto& c = *new std::map<int, std::vector<double*>>; return c; }
+    int index_;
+    double* at_ = nullptr;
+};
 ctb_view scalar_view(double* p) {
     ctb_view v;
     std::memset(&v, 0, sizeof v);
@@ -379,14 +401,14 @@ double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, doubl
     // one call per GPU; the norm comes back through managed memory
     auto call = [&](int index, const std::vector<ctb_view>& views, double limit, bool scale) {
         use_device(index);
-        double* out = norm_cell(index);
-        const ctb_view vn = scalar_view(out);
+        const NormCell out(index);
+        const ctb_view vn = scalar_view(out.get());
         std::vector<const ctb_view*> list;
         for (const ctb_view& v : views) list.push_back(&v);
         if (scale) check(ctb_clip_grad_norm(list.data(), (int)list.size(), limit, p, nullptr, &vn, nullptr, 0, nullptr));
         else check(ctb_grad_norm(list.data(), (int)list.size(), p, &vn, nullptr, 0, nullptr));
         check(ctb_sync(nullptr));
-        return *out;
+        return *out.get();
     };
     if (by_device.size() == 1) return call(by_device.begin()->first, by_device.begin()->second, max_norm, true);
     if (!(max_norm >= 0.0)) throw std::runtime_error("clip_grad_norm: max_norm must not be negative or NaN");

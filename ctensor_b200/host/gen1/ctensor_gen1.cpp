@@ -209,15 +209,43 @@ void zero_grad(Tensor& param) {
     after_op();
 }
 
+namespace {
+// A double that one call's norm is written to (managed: the host reads it).  Cells go back to a list, so there
+// are never more of them than calls at once, however many threads come and go.
+class NormCell {
+public:
+    NormCell() {
+        {
+            std::lock_guard<std::mutex> lk(mutex());
+            if (!cells().empty()) {
+                at_ = cells().back();
+                cells().pop_back();
+                return;
+            }
+        }
+        void* p = nullptr;
+        check(ctb_alloc_managed(&p, sizeof(double), /*zero=*/1));
+        at_ = (double*)p;
+    }
+    ~NormCell() {
+        std::lock_guard<std::mutex> lk(mutex());
+        cells().push_back(at_);
+    }
+    NormCell(const NormCell&) = delete;
+    NormCell& operator=(const NormCell&) = delete;
+    double* get() const { return at_; }
+
+private:
+    // never destroyed: a thread may still clip while the process ends
+    static std::mutex& mutex() { static std::mutex& m = *new std::mutex; return m; }
+    static std::vector<double*>& cells() { static auto& c = *new std::vector<double*>; return c; }
+    double* at_ = nullptr;
+};
+}  // namespace
+
 double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, double p) {
     ensure_device();
-    // the norm comes back through managed memory
-    static thread_local double* cell = nullptr;
-    if (!cell) {
-        void* q = nullptr;
-        check(ctb_alloc_managed(&q, sizeof(double), /*zero=*/1));
-        cell = (double*)q;
-    }
+    const NormCell cell;
     std::vector<ctb_view> views;
     std::set<std::tuple<const void*, int64_t, size_t>> seen;     // slices of one buffer count each
     for (const Tensor* param : params) {
@@ -229,11 +257,11 @@ double clip_grad_norm(const std::vector<Tensor*>& params, double max_norm, doubl
     for (const ctb_view& v : views) list.push_back(&v);
     ctb_view vn;
     std::memset(&vn, 0, sizeof vn);
-    vn.base = cell;
+    vn.base = cell.get();
     vn.dtype = CTB_F64;
     check(ctb_clip_grad_norm(list.data(), (int)list.size(), max_norm, p, nullptr, &vn, nullptr, 0, nullptr));
     check(ctb_sync(nullptr));
-    return *cell;
+    return *cell.get();
 }
 
 void set_backward_entry(std::function<void(Tensor&)> f) { g_backward = std::move(f); }

@@ -1,4 +1,4 @@
-"""Gradient clipping through the C++ host layers where gradients share a buffer: the programs build everywhere and
+"""Gradient clipping through the C++ host layers where gradients share a buffer, and from many threads: the programs build everywhere and
 pass their checks on a GPU."""
 import os
 import subprocess
@@ -8,7 +8,9 @@ import pytest
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "ctensor_b200")
 PROGRAMS = {"test_clip_slices": ("ctensor_host", ["host/include"]),
-            "test_clip_slices_gen1": ("ctensor_gen1", ["host/gen1/include", "host/include"])}
+            "test_clip_slices_gen1": ("ctensor_gen1", ["host/gen1/include", "host/include"]),
+            "test_clip_threads": ("ctensor_host", ["host/include"]),
+            "test_clip_threads_gen1": ("ctensor_gen1", ["host/gen1/include", "host/include"])}
 
 
 def _build(name):
