@@ -3,7 +3,7 @@
 //   N = (sum over all tensors and elements of |g|^p)^(1/p), p = 1, 2 or infinity;
 //   g <- g * (max_norm / N)   if max_norm < N < infinity, else g as it is.
 //
-// Two launches whatever the number of tensors (one pair per 1024 of them): the first leaves one fp64
+// Two launches for every 1024 tensors: the first leaves one fp64
 // partial per block, every block of the second folds all partials in the same order (so all of them
 // agree on the factor bit for bit, with no atomics and no block that waits for another) and scales.
 // The list of tensors travels in the kernel's arguments: nothing is copied ahead of the launch and a
@@ -188,7 +188,9 @@ clip_finish_kernel(const double* __restrict__ partials, int count, void* norm, i
     if (threadIdx.x == 0) clip_store_norm(total, norm, norm_dtype);
 }
 
-// The factor is rounded to T once (the product once more): two roundings of 2^-24 for Float32.
+// The factor is rounded to T once (the product once more): two roundings of 2^-24 for Float32.  A factor so small that T
+// would hold it with fewer bits, or as 0, is applied in fp64 in two steps, of which the first is exact.
+template <typename T> __device__ __forceinline__ double clip_smallest() { return sizeof(T) == 4 ? 0x1p-100 : 0x1p-960; }
 template <int KIND, typename T, int N>
 __global__ void __launch_bounds__(kClipThreads)
 clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const double* __restrict__ partials, int count, double max_norm,
@@ -202,6 +204,8 @@ clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const double* __restri
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) clip_store_norm(total, norm, norm_dtype);
     const bool clipped = total > max_norm && total < INFINITY;
     const T factor = clipped ? (T)(max_norm / total) : (T)1;
+    const bool tiny = clipped && max_norm / total < clip_smallest<T>();
+    const double rest = max_norm * 0x1p512 / total;
     uint32_t lo, c;
     clip_range(t.first[t.count], &lo, &c);
     int which = lo < c ? clip_tensor_of(t, c - 1) : 0;
@@ -218,7 +222,7 @@ clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const double* __restri
         src -= phase;
         dst -= phase;
         const int64_t begin = (int64_t)(c - t.first[which]) * CHUNK;
-        if (!together) {                                    // other alignment on the two sides: element by element
+        if (!together || tiny) {                            // other alignment on the two sides: element by element
             const int64_t stop = begin + CHUNK < end ? begin + CHUNK : end;
             for (int64_t p = begin + threadIdx.x; p < stop; p += kClipThreads * kClipApart) {
                 T v[kClipApart];
@@ -226,7 +230,8 @@ clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const double* __restri
                 for (int i = 0; i < kClipApart; ++i) v[i] = p + i * kClipThreads >= phase && p + i * kClipThreads < stop ? src[p + i * kClipThreads] : (T)0;
 #pragma unroll
                 for (int i = 0; i < kClipApart; ++i)
-                    if (p + i * kClipThreads >= phase && p + i * kClipThreads < stop) dst[p + i * kClipThreads] = clipped ? v[i] * factor : v[i];
+                    if (p + i * kClipThreads >= phase && p + i * kClipThreads < stop)
+                        dst[p + i * kClipThreads] = tiny ? (T)((double)v[i] * 0x1p-512 * rest) : clipped ? v[i] * factor : v[i];
             }
             continue;
         }

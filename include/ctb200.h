@@ -485,7 +485,8 @@ int ctb_residual_norm_backward(const ctb_view* f, const ctb_view* y, const ctb_v
                                size_t workspace_bytes, void* stream);
 
 /* The norm of all gradients of a model as one vector, and scaling them down to a given norm before an
- * optimizer step: norm = (sum |g|^p)^(1/p) with p = 1, 2 or infinity, summed in fp64.
+ * optimizer step: norm = (sum |g|^p)^(1/p) with p = 1, 2 or infinity, summed in fp64 (with p = 2 so are the
+ * squares: those of Double64 values beyond 1e154 overflow, below 1e-162 they vanish).
  * `grads`: `count` Float32 / Double64 views, each dense (some permutation of a gap-free block of memory),
  * possibly empty; `norm`: one Float32 or Double64 element.
  * ctb_clip_grad_norm also multiplies every gradient by max_norm / norm when max_norm < norm < infinity (the

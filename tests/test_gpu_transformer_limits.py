@@ -276,3 +276,27 @@ def test_score_exponential(ct, keys):
     slack = torch.where(e < 2.0 ** -125, 2.0 ** -125, 0.0)
     within(p[:, keys - 1], want, want * U * (each + each * e + 8) + slack, "the smaller one")
     within(p[:, 0], 1 / (1 + e), U * (each * e + 8), "the larger one")
+
+
+# ---- clipping by very small factors ----------------------------------------------------------------------------
+@pytest.mark.parametrize("size,limit,p,dtype", [(3e38, 0.5, 2, torch.float32), (1e30, 1e-12, 2, torch.float32), (3e38, 1e-35, 1, torch.float32),
+                                                (1e35, 1e-20, math.inf, torch.float32), (1e300, 1e-15, math.inf, torch.float64),
+                                                (1e303, 1e-10, 1, torch.float64), (1e10, 1e-12, 2, torch.float32)])
+@pytest.mark.parametrize("out", [False, True])
+def test_clip_by_very_small_factors(ct, size, limit, p, dtype, out):
+    """The norm is finite and far above the limit: two roundings a value, the factor's and the product's."""
+    g = gen(11)
+    half = U if dtype == torch.float32 else 2.0 ** -53
+    grads = [((torch.rand(n, device=DEV, generator=g, dtype=torch.float64) - 0.5) * 2 * size).to(dtype) for n in (1, 7, 9000, 20001)]
+    flat = torch.cat(grads).double()
+    unit = flat / flat.abs().max()                       # the sums of squares stay in range
+    total = {1: unit.abs().sum(), 2: unit.square().sum().sqrt(), math.inf: unit.abs().max()}[p] * flat.abs().max()
+    assert bool(total.isfinite())
+    have = [t.clone() for t in grads]
+    outs = [torch.empty(t.numel() + 3, device=DEV, dtype=dtype)[3 * (i % 2):][:t.numel()] for i, t in enumerate(grads)] if out else None
+    n = ct.clip_grad_norm(have, limit, p, out=outs, norm=torch.empty(1, device=DEV, dtype=torch.float64))
+    assert abs(float(n) - float(total)) <= 100 * 2.0 ** -53 * float(total)
+    small = 2.0 ** -149 if dtype == torch.float32 else 2.0 ** -1074
+    for a, b in zip(grads, outs if out else have):
+        want = (a.double() / total) * limit              # in this order neither overflows nor vanishes
+        within(b, want, (2.0 * half + 110 * 2.0 ** -53) * want.abs() + small, "clipped")
