@@ -237,14 +237,18 @@ __device__ __forceinline__ float score_slope(const ScorePlace& w, float sum, int
     for (int k = 0; k < 4; ++k) sum = fmaf(DOCS ? (float)(abs(c0 + k - w.centre) - w.near) : fabsf(from + (float)k), r[k], sum);
     return sum;
 }
+// r *= scale * (1 - tanh^2), with 1 - tanh^2 x = 4 q / (1 + q)^2, q = e^(-2 |x|): far beyond the cap, where tanh is next to 1
+// and the difference would lose all its bits (at x = 9 it is 0), all of them count.
 template <bool CAP>
-__device__ __forceinline__ void score_slow(const ScoreGeom& g, float (&r)[4], const float* s) {     // r *= scale * (1 - tanh^2)
+__device__ __forceinline__ void score_slow(const ScoreGeom& g, float (&r)[4], const float* s) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         r[k] = r[k] * g.scale;
         if (CAP) {
-            const float th = tanhf(s[k] * g.over_cap);
-            r[k] = r[k] * fmaf(-th, th, 1.0f);
+            const float q = score_exp(-2.0f * fabsf(s[k] * g.over_cap));
+            float over;                                  // within 2 half steps
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over) : "f"(1.0f + q));
+            r[k] = r[k] * (q * over * (4.0f * over));
         }
     }
 }

@@ -300,3 +300,20 @@ def test_clip_by_very_small_factors(ct, size, limit, p, dtype, out):
     for a, b in zip(grads, outs if out else have):
         want = (a.double() / total) * limit              # in this order neither overflows nor vanishes
         within(b, want, (2.0 * half + 110 * 2.0 ** -53) * want.abs() + small, "clipped")
+
+
+# ---- the cap's slope far beyond the cap ---------------------------------------------------------------------------
+@pytest.mark.parametrize("keys", [64, 1001, 1024, 4096, 30001])
+def test_gradients_of_scores_far_beyond_the_cap(ct, keys):
+    """Scores of up to 40 caps: 1 - tanh^2 within (6.5 x + 12) half steps of itself (2 x of three rounded factors and 4 of the
+    exponential, twice the reciprocal's 2 and the sum's 1, products), whatever is left of it."""
+    g = gen(keys)
+    s = (torch.rand(1, 2, 3, keys, device=DEV, generator=g) - 0.5) * 160.0
+    p = torch.full_like(s, 1.0 / keys)
+    dp = randn(g, 1, 2, 3, keys)
+    rules = {"scale": 0.5, "cap": 1.0}
+    ds, _ = ct.score_softmax_backward(dp, p, ct.ScoreRules(**rules), scores=s)
+    x = s.double().abs() * 0.5
+    slow = 4.0 * torch.exp(-2.0 * x) / (1.0 + torch.exp(-2.0 * x)) ** 2
+    bare, _, bound, _ = ref.score_gradients(s.double(), p.double(), dp.double(), {"scale": 0.5})
+    within(ds, bare * slow, bound * slow * 1.0001 + (6.5 * x + 14.0) * U * (bare * slow).abs() + 2.0 ** -126, "score gradients")
