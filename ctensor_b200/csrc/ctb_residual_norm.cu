@@ -369,7 +369,7 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
         finish(by);
         return;
     }
-    if (sy < 1e-6 * s[1]) fold_again(rf);
+    if (!(sy >= 1e-6 * s[1])) fold_again(rf);            // also where infinities in x and f leave no number
     finish(rf);
 }
 

@@ -317,3 +317,26 @@ def test_gradients_of_scores_far_beyond_the_cap(ct, keys):
     slow = 4.0 * torch.exp(-2.0 * x) / (1.0 + torch.exp(-2.0 * x)) ** 2
     bare, _, bound, _ = ref.score_gradients(s.double(), p.double(), dp.double(), {"scale": 0.5})
     within(ds, bare * slow, bound * slow * 1.0001 + (6.5 * x + 14.0) * U * (bare * slow).abs() + 2.0 ** -126, "score gradients")
+
+
+# ---- infinities and NaN in rows with norms on both sides ------------------------------------------------------
+@pytest.mark.parametrize("cols", [8, 33, 768, 2048, 2052])
+@pytest.mark.parametrize("kind", [1, 2])
+def test_norms_of_rows_that_are_not_finite(ct, cols, kind):
+    """What the formula says, at every width: an infinite entry of the stream leaves an RMS norm's other entries 0."""
+    g = gen(cols)
+    inf, nan = math.inf, math.nan
+    x, f = randn(g, 8, cols), randn(g, 8, cols)
+    f[:, 3] = 1.0
+    for row, (where, value) in enumerate([(x, inf), (x, -inf), (x, nan), (f, inf), (f, -inf), (f, nan)]):
+        where[row, 3] = value
+    f[6, 3] = -1.0
+    x[6, 3] = inf
+    params = ct.ResidualNorm(pre=kind, post=kind, scale=0.5)
+    y, h, _ = ct.residual_norm(x, f, params)
+    want_y = x.double() + 0.5 * ref.normed(f.double(), kind, None, None, 1e-5)
+    want_h = ref.normed(want_y, kind, None, None, 1e-5)
+    for got, want in ((y, want_y), (h, want_h)):
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        close = want.isfinite()
+        assert bool(((got.double() - want)[close].abs() <= 1e-5 * (1 + want[close].abs())).all())
