@@ -675,7 +675,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                     w[q] = 1.0f;
                     gv[q] = one_gate;
                 }
-                if (FAST || a.out.x) store_part<VEC>(a.out.x, out, dx);
+                if (FAST || a.out.x) store_part<VEC>(a.out.x + out, 0, dx);
                 if (has_f) read_own<VEC>(fv, at + kInF * SLOT);
                 if (post) {
 #pragma unroll
@@ -717,7 +717,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
 #pragma unroll
                         for (int q = 0; q < VEC; ++q) gate_sum[GATE ? i * VEC + q : 0] += n[q];
                     } else {
-                        store_part<VEC>(a.out.gate, out, n);
+                        store_part<VEC>(a.out.gate + out, 0, n);
                     }
                 }
                 float df[VEC];
@@ -731,7 +731,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                     }
                     df[q] = post ? st.y * (dn * w[q] - fmaf(fv[q], c1, c0)) : dn;
                 }
-                if (FAST || a.out.f) store_part<VEC>(a.out.f, out, df);
+                if (FAST || a.out.f) store_part<VEC>(a.out.f + out, 0, df);
             }
         }
         if constexpr (SCALAR) {

@@ -340,3 +340,65 @@ def test_norms_of_rows_that_are_not_finite(ct, cols, kind):
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
         close = want.isfinite()
         assert bool(((got.double() - want)[close].abs() <= 1e-5 * (1 + want[close].abs())).all())
+
+
+# ---- more elements than 32 bits count ---------------------------------------------------------------------------
+def test_scores_of_more_than_2_31_elements(ct):
+    B, H, Q, K = 1, 2, 34_000, 32_768
+    s = torch.zeros(B, H, Q, K, device=DEV)
+    g = gen(9)
+    s[0, 1, -5:] = randn(g, 5, K) * 3
+    rules = {"scale": 0.7, "causal": True, "query_start": ints([5])}
+    p = ct.score_softmax(s, ct.ScoreRules(**rules))
+    tail = dict(rules, query_start=ints([5 + Q - 5]))
+    last = s[:, 1:, -5:].double()
+    want = ref.score_softmax(last, tail)
+    within(p[:, 1:, -5:], want, ref.score_bound(last, want, tail), "probabilities")
+    assert float(p[0, 0, 0, :6].sum()) == pytest.approx(1.0, abs=8 * U) and float(p[0, 1, 10, 16:].abs().sum()) == 0.0
+    dp = torch.zeros_like(s)
+    dp[0, 1, -5:] = randn(g, 5, K)
+    ds, _ = ct.score_softmax_backward(dp, p, ct.ScoreRules(**rules), out=s)
+    w, _, bound, _ = ref.score_gradients(last, p[:, 1:, -5:].double(), dp[:, 1:, -5:].double(), tail)
+    within(ds[:, 1:, -5:], w, bound, "score gradients")
+    assert float(ds[0, 0].abs().amax()) == 0.0
+
+
+@pytest.mark.parametrize("rows,cols", [(525_000, 4096), (263_000, 8196), (4_300_000, 501)])
+@pytest.mark.parametrize("norms", [(2, 2), (1, 0)], ids=str)
+def test_norms_of_more_than_2_31_elements(ct, rows, cols, norms):
+    """All rows alike, so they all have the result of one row by itself."""
+    g = gen(10)
+    x, f, dy, dh, gate = (randn(g, 1, cols) for _ in range(5))
+    w = 1 + 0.1 * randn(g, cols)
+    params = ct.ResidualNorm(pre=norms[0], pre_weight=w, post=norms[1], post_weight=w if norms[1] else None)
+    many = lambda t: t.expand(rows, t.shape[-1])
+    one = ct.residual_norm(x, f, params, gate=gate)
+    got = ct.residual_norm(many(x), many(f), params, gate=many(gate))
+    at = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device=DEV)
+    for a, b in zip(got, one):
+        assert torch.equal(a[at], many(b)[at])
+    del got, a
+    y, h, stats = one
+    one = ct.residual_norm_backward(f, y, stats, params, grad_y=dy, grad_h=dh, gate=gate)
+    for fast in (True, False):                           # without grad_y the general kernel runs
+        if not fast:
+            one = ct.residual_norm_backward(f, y, stats, params, grad_h=dh, gate=gate)
+        got = ct.residual_norm_backward(many(f), many(y), many(stats).contiguous(), params, grad_y=many(dy) if fast else None, grad_h=many(dh), gate=many(gate))
+        for n in ("x", "f", "gate"):
+            assert torch.equal(getattr(got, n)[at], many(getattr(one, n))[at]), n
+        want = one.pre_weight.double() * rows
+        within(got.pre_weight, want, 260 * U * want.abs() + 1e-30, "gradient of the weight")
+        del got
+
+
+def test_clipping_of_more_than_2_31_elements(ct):
+    x = torch.ones(2_200_000_001, device=DEV)
+    x[-5:] = torch.tensor([2.0, 4.0, 8.0, 16.0, 32.0], device=DEV)
+    total = math.sqrt(2_200_000_001 - 5 + 4 + 16 + 64 + 256 + 1024)
+    out = torch.empty(x.numel() + 1, device=DEV)[1:]
+    for grads, outs in (([x], [out]), ([x], None)):
+        got = float(ct.clip_grad_norm(grads, total / 2, out=outs, norm=torch.empty(1, device=DEV, dtype=torch.float64)))
+        assert abs(got - total) <= 1e-12 * total
+        y = out if outs else x
+        assert y[-7:].tolist() == [0.5, 0.5, 1.0, 2.0, 4.0, 8.0, 16.0] and float(y[0]) == 0.5
+        assert float(y[1_000_000_000:1_000_100_000].sum()) == 50_000.0
