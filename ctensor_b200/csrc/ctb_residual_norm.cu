@@ -241,6 +241,60 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
     if (stats && tid == 0 && rank == 0) *reinterpret_cast<float4*>(stats + row * 4) = st;
 }
 
+// A row of residual_rms_kernel (below) that is near the ends of Float32, normed before it is scaled, from memory.  A call of
+// its own: inlined, it took registers from all other rows ([1000000,128] 375 us, 428 so).
+template <int THREADS, int T, int VEC>
+__device__ __noinline__ void residual_rms_extreme_row(const ResidualNormGeom& g, const float* x, const float* f, float* y, float* h, float* stats, int64_t row,
+                                                      float rf, TeamSlots<THREADS, 4, double>& sh, FoldTurn turn) {
+    const int tid = threadIdx.x % T, width = (int)g.cols;
+    const float* gate = g.gate.p + (int64_t)fast_div((uint32_t)row, g.by_gate_rows) * g.gate.stride;
+    const float one_gate = g.gate_mode == kGateScalar ? gate[0] * g.scale : g.scale;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int c = tid * VEC; c < width; c += T * VEC) {
+        float n[VEC], k[VEC];
+        load_part<T, VEC>(n, f, c);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) n[q] = n[q] * rf;
+        if (g.post_weight) {
+            load_part<T, VEC>(k, g.post_weight, c);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) n[q] = n[q] * k[q];
+        }
+        if (g.gate_mode == kGateRow) {
+            load_part<T, VEC>(k, gate, c);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) n[q] = n[q] * k[q];
+        }
+        load_part<T, VEC>(k, x, c);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+            n[q] = fmaf(one_gate, n[q], k[q]);
+            s[0] = fma((double)n[q], (double)n[q], s[0]);
+        }
+        store_part<VEC>(y, c, n);
+    }
+    team_fold<FoldSum, THREADS, T>(s, sh, turn);
+    const float ry = inverse_root(s[0] * g.inv_cols + (double)g.pre_eps);
+    for (int c = tid * VEC; c < width; c += T * VEC) {
+        float n[VEC], k[VEC];
+        load_part<T, VEC>(n, y, c);                      // what this thread stored
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) n[q] = n[q] * ry;
+        if (g.pre_weight) {
+            load_part<T, VEC>(k, g.pre_weight, c);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) n[q] = n[q] * k[q];
+        }
+        if (g.pre_bias) {
+            load_part<T, VEC>(k, g.pre_bias, c);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) n[q] = n[q] + k[q];
+        }
+        store_part<VEC>(h, c, n);
+    }
+    if (stats && tid == 0) *reinterpret_cast<float4*>(stats) = make_float4(0.0f, rf, 0.0f, ry);
+}
+
 // RMS norms on both sides need one fold per row instead of two: with u = scale * gate * w_post * f the stream is
 // y = x + rstd_f * u, so
 //     sum(y^2) = sum(x^2) + 2 rstd_f sum(x u) + rstd_f^2 sum(u^2)
@@ -251,8 +305,8 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
 // rows of up to 2048 columns: [16384, 1536] 69 us against 74; wider rows, which hold more of it per thread, lose ([4096, 4096]
 // 60 against 52).
 template <int THREADS, int T, int E, int VEC>
-__global__ void __launch_bounds__(THREADS, 4)
-residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ y, float* __restrict__ h, float* __restrict__ stats) {
+__global__ void __launch_bounds__(THREADS, E == 2 ? 6 : E == 4 ? 5 : 4)
+residual_rms_kernel(const __grid_constant__ ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ y, float* __restrict__ h, float* __restrict__ stats) {
     __shared__ TeamSlots<THREADS, 4, double> sh;
     const int tid = threadIdx.x % T;
     const int64_t row = (int64_t)blockIdx.x * (THREADS / T) + threadIdx.x / T;
@@ -299,78 +353,51 @@ residual_rms_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__ 
     const float rf = inverse_root(s[0] * g.inv_cols + (double)g.post_eps);
     const double r = rf;
     double sy = fma(r, fma(r, s[3], 2.0 * s[2]), s[1]);
-    // y = x + by * u and its norm; `sy`: the sum of its squares
-    auto finish = [&](float by) {
-        const float ry = inverse_root(sy * g.inv_cols + (double)g.pre_eps);
-#pragma unroll
-        for (int i = 0; i < E / VEC; ++i) {
-            const int c = col_of<T, VEC>(i, tid);
-            if (c < width) {
-                float out[VEC];
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) out[q] = fmaf(by, u[i * VEC + q], xv[i * VEC + q]);
-                store_part<VEC>(y + row * g.cols, c, out);
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) out[q] = out[q] * ry;
-                if (g.pre_weight) {
-                    float w[VEC];
-                    load_part<T, VEC>(w, g.pre_weight, c);
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) out[q] = out[q] * w[q];
-                }
-                if (g.pre_bias) {
-                    float w[VEC];
-                    load_part<T, VEC>(w, g.pre_bias, c);
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) out[q] = out[q] + w[q];
-                }
-                store_part<VEC>(h + row * g.cols, c, out);
-            }
-        }
-        if (stats && tid == 0) *reinterpret_cast<float4*>(stats + row * 4) = make_float4(0.0f, rf, 0.0f, ry);
-    };
-    auto fold_again = [&](float by) {
+    // (both conditions are the same in every thread of the team)
+    if (s[0] < INFINITY && (!(s[3] < INFINITY) || rf > 1048576.0f)) {
+        residual_rms_extreme_row<THREADS, T, VEC>(g, x.p + row * x.stride, f.p + row * f.stride, y + row * g.cols, h + row * g.cols,
+                                                  stats ? stats + row * 4 : nullptr, row, rf, sh, turn);
+        return;
+    }
+    if (!(sy >= 1e-6 * s[1])) {                          // also where infinities in x and f leave no number
         double square = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const double d = col_of<T, VEC>(e / VEC, tid) < width ? fmaf(by, u[e], xv[e]) : 0.0f;
+            const double d = col_of<T, VEC>(e / VEC, tid) < width ? fmaf(rf, u[e], xv[e]) : 0.0f;
             square = fma(d, d, square);
         }
         s[0] = square;
         s[1] = s[2] = s[3] = 0.0;
         team_fold<FoldSum, THREADS, T>(s, sh, turn);
         sy = s[0];
-    };
-    // (both conditions are the same in every thread of the team)
-    if (s[0] < INFINITY && (!(s[3] < INFINITY) || rf > 1048576.0f)) {
-        load_share<T, E, VEC>(u, f.p + row * f.stride, width, tid);
-        const float* const row_gate = g.gate.p + (int64_t)fast_div((uint32_t)row, g.by_gate_rows) * g.gate.stride;
-        const float by = g.gate_mode == kGateScalar ? row_gate[0] * g.scale : g.scale;
-#pragma unroll
-        for (int i = 0; i < E / VEC; ++i) {
-            const int c = col_of<T, VEC>(i, tid);
-            if (c < width) {
-                float k[VEC];
-#pragma unroll
-                for (int q = 0; q < VEC; ++q) u[i * VEC + q] = u[i * VEC + q] * rf;
-                if (g.post_weight) {
-                    load_part<T, VEC>(k, g.post_weight, c);
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) u[i * VEC + q] = u[i * VEC + q] * k[q];
-                }
-                if (g.gate_mode == kGateRow) {
-                    load_part<T, VEC>(k, row_gate, c);
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) u[i * VEC + q] = u[i * VEC + q] * k[q];
-                }
-            }
-        }
-        fold_again(by);
-        finish(by);
-        return;
     }
-    if (!(sy >= 1e-6 * s[1])) fold_again(rf);            // also where infinities in x and f leave no number
-    finish(rf);
+    const float ry = inverse_root(sy * g.inv_cols + (double)g.pre_eps);
+#pragma unroll
+    for (int i = 0; i < E / VEC; ++i) {
+        const int c = col_of<T, VEC>(i, tid);
+        if (c < width) {
+            float out[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) out[q] = fmaf(rf, u[i * VEC + q], xv[i * VEC + q]);
+            store_part<VEC>(y + row * g.cols, c, out);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) out[q] = out[q] * ry;
+            if (g.pre_weight) {
+                float w[VEC];
+                load_part<T, VEC>(w, g.pre_weight, c);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) out[q] = out[q] * w[q];
+            }
+            if (g.pre_bias) {
+                float w[VEC];
+                load_part<T, VEC>(w, g.pre_bias, c);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) out[q] = out[q] + w[q];
+            }
+            store_part<VEC>(h + row * g.cols, c, out);
+        }
+    }
+    if (stats && tid == 0) *reinterpret_cast<float4*>(stats + row * 4) = make_float4(0.0f, rf, 0.0f, ry);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------
@@ -434,7 +461,8 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
     const uint32_t rank = cs > 1 ? cluster_rank() : 0;
     const int64_t team = (int64_t)(blockIdx.x / cs) * TEAMS + threadIdx.x / T;
     const bool present = team < a.teams;
-    const int64_t lo = present ? g.rows * team / a.teams : 0, hi = present ? g.rows * (team + 1) / a.teams : 0;
+    // (rows are fewer than 2^31, offsets are not)
+    const int lo = present ? (int)(g.rows * team / a.teams) : 0, hi = present ? (int)(g.rows * (team + 1) / a.teams) : 0;
     const int64_t slice = cs > 1 ? ((g.cols + cs - 1) / cs + 3) / 4 * 4 : g.cols;
     const int64_t begin = slice * rank;
     const int width = (int)(begin >= g.cols ? 0 : (g.cols - begin < slice ? g.cols - begin : slice));
@@ -508,7 +536,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
 #pragma unroll
     for (int q = 0; q < kInCount; ++q) next[q] = a.in[q].p + lo * a.in[q].stride + begin + tid * VEC;
     float* const mine = staged + threadIdx.x * VEC;
-    int64_t fetched = lo;
+    int fetched = lo;
     auto fetch = [&](int stage_at) {                     // always commits, so that groups count rows
         if (fetched < hi) {
 #pragma unroll
@@ -521,22 +549,21 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                     if (col_of<T, VEC>(i, tid) < width) copy_async<VEC * 4>(mine + stage_at + q * SLOT + i * THREADS * VEC, next[op] + i * T * VEC);
                 next[op] += a.in[op].stride;
             }
+            ++fetched;
         }
-        ++fetched;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     constexpr int STAGE = F::SLOTS * SLOT;
     const int ring = a.stages * STAGE;
     for (int s = 0; s + 1 < a.stages; ++s) fetch(s * STAGE);
-    int64_t group = fast_div((uint32_t)lo, g.by_gate_rows);
-    int64_t left = (group + 1) * g.gate_rows - lo;       // rows of this gate row that are still to come
+    int group = (int)fast_div((uint32_t)lo, g.by_gate_rows);
+    int left = (int)((group + 1) * g.gate_rows - lo);    // rows of this gate row that are still to come
     const float4* stats = reinterpret_cast<const float4*>(a.stats) + lo;
     float4 next_st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
     if (lo < hi) next_st = *stats;
     int stage_at = 0, ahead_at = (a.stages - 1) * STAGE;
-    int64_t out_at = lo * g.cols + begin + tid * VEC;
     FoldTurn turn = entry.met(), gate_turn = turn;
-    for (int64_t row = lo; row < hi; ++row, out_at += g.cols) {
+    for (int row = lo; row < hi; ++row) {
         const float4 st = next_st;
         fetch(ahead_at);                                 // into the place of the row before this one, which is done with
         if (row + 1 < hi) next_st = *++stats;
@@ -660,11 +687,12 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
         const float c0 = FULL && g.post_kind == CTB_NORM_LAYER ? (s_ke - (b0 * s_k + b1 * s_ky)) * inv : 0.0f;
         const float c1 = (s_kef - (b0 * s_kf + b1 * s_kfy)) * inv;
         float scalar_sum = 0.0f;
+        const int64_t out_at = row * g.cols + begin + tid * VEC;
 #pragma unroll
         for (int i = 0; i < E / VEC; ++i) {
             const int c = col_of<T, VEC>(i, tid);
             const float* at = in + i * THREADS * VEC;
-            const int64_t out = out_at + i * T * VEC;
+            const int out = i * T * VEC;
             if (c < width) {
                 float dx[VEC], fv[VEC], w[VEC], gv[VEC];
 #pragma unroll
@@ -675,7 +703,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                     w[q] = 1.0f;
                     gv[q] = one_gate;
                 }
-                if (FAST || a.out.x) store_part<VEC>(a.out.x + out, 0, dx);
+                if (FAST || a.out.x) store_part<VEC>(a.out.x + out_at, out, dx);
                 if (has_f) read_own<VEC>(fv, at + kInF * SLOT);
                 if (post) {
 #pragma unroll
@@ -717,7 +745,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
 #pragma unroll
                         for (int q = 0; q < VEC; ++q) gate_sum[GATE ? i * VEC + q : 0] += n[q];
                     } else {
-                        store_part<VEC>(a.out.gate + out, 0, n);
+                        store_part<VEC>(a.out.gate + out_at, out, n);
                     }
                 }
                 float df[VEC];
@@ -731,7 +759,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
                     }
                     df[q] = post ? st.y * (dn * w[q] - fmaf(fv[q], c1, c0)) : dn;
                 }
-                if (FAST || a.out.f) store_part<VEC>(a.out.f + out, 0, df);
+                if (FAST || a.out.f) store_part<VEC>(a.out.f + out_at, out, df);
             }
         }
         if constexpr (SCALAR) {
@@ -762,7 +790,7 @@ residual_norm_backward_kernel(const __grid_constant__ ResidualBwd a, int cs) {
             }
             if (!SCALAR) scalar_gate_sum = 0.0f;
             ++group;
-            left = g.gate_rows;
+            left = (int)g.gate_rows;
         }
     }
     if constexpr (SCALAR) {
