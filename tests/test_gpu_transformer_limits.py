@@ -342,6 +342,76 @@ def test_norms_of_rows_that_are_not_finite(ct, cols, kind):
         assert bool(((got.double() - want)[close].abs() <= 1e-5 * (1 + want[close].abs())).all())
 
 
+# ---- calls through the C functions that the Python binding does not make ------------------------------------------
+def call_backward(ct, f, y, gate, stats, params, dy, dh, grads):
+    """ctb_residual_norm_backward with the gradients in `grads` (name -> tensor) and no others, and a workspace of exactly
+    the size that was asked for, with a guard behind it."""
+    import ctypes
+    L, raw = ct.lib(), ct._raw_view
+    views = {k: raw(t) for k, t in grads.items()}
+    c = ct.CResidualNormGrads(*(ct._address(views.get(n)) for n, _ in ct.CResidualNormGrads._fields_))
+    yv, gv = raw(y), raw(gate)
+    need = L.ctb_residual_norm_workspace_bytes(yv, gv)
+    ws = torch.full((need + 1024,), 0xAB, dtype=torch.uint8, device=DEV)
+    ct.check(L.ctb_residual_norm_backward(raw(f), yv, gv, raw(stats), params.c, raw(dy), raw(dh), ctypes.byref(c), ws.data_ptr(), need,
+                                          torch.cuda.current_stream().cuda_stream))
+    assert bool((ws[need:] == 0xAB).all()), "written behind the workspace"
+
+
+WANTED = [("x",), ("gate",), ("f",), ("pre_weight",), ("post_weight", "post_bias"), ("pre_bias", "gate"), ("x", "f", "pre_weight"), ("x", "post_bias"),
+          ("x", "f", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias")]
+
+
+@pytest.mark.parametrize("wanted", WANTED, ids="-".join)
+@pytest.mark.parametrize("cols", [96, 301, 2304, 5124])
+@pytest.mark.parametrize("gate", ["channel", "batch", "sequence", "full"])
+def test_some_of_the_norm_gradients(ct, wanted, cols, gate):
+    """Any of the gradients without the others, at every 4-byte phase of what is written."""
+    g = gen(cols)
+    B, T = 6, 50
+    x, f, dy, dh = (randn(g, B, T, cols) for _ in range(4))
+    shape = {"channel": (cols,), "batch": (B, 1, cols), "sequence": (B, 1, 1), "full": (B, T, cols)}[gate]
+    gate = randn(g, *shape)
+    pre, post = vectors(g, 1, True, True, cols), vectors(g, 1, True, True, cols)
+    params = ct.ResidualNorm(pre=1, pre_weight=pre[1], pre_bias=pre[2], post=1, post_weight=post[1], post_bias=post[2], scale=0.5)
+    y, _, stats = ct.residual_norm(x, f, params, gate=gate)
+    d = lambda v: tuple(t.double() if torch.is_tensor(t) else t for t in v)
+    want = ref.residual_norm_gradients(f.double(), y.double(), d(pre), d(post), gate.double(), 0.5, dy.double(), dh.double())
+    like = {"x": x, "f": f, "gate": gate, "post_weight": post[1], "post_bias": post[2], "pre_weight": pre[1], "pre_bias": pre[2]}
+    for phase in (0, 3):
+        flats = {n: torch.full((like[n].numel() + 8,), 7.0, device=DEV) for n in wanted}
+        grads = {n: flats[n][phase:phase + like[n].numel()].view(like[n].shape) for n in wanted}
+        call_backward(ct, f, y, gate, stats, params, dy, dh, grads)
+        for n in wanted:
+            within(grads[n], want[n][0], want[n][1] + 1e-36, "gradient of " + n)
+            assert bool((flats[n][:phase] == 7).all()) and bool((flats[n][phase + like[n].numel():] == 7).all()), n
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 4), (149, 2050), (2400, 64), (300_000, 8), (5, 8200), (40_000, 12300)])
+@pytest.mark.parametrize("norms", [(2, 2), (1, 1), (1, 0)], ids=str)
+def test_workspace_of_the_size_asked_for(ct, rows, cols, norms):
+    """The kernels stay inside the workspace, whichever of them runs and however many teams there are."""
+    g = gen(rows)
+    if rows * cols > 200_000_000:
+        x = randn(g, 1, cols).expand(rows, cols).contiguous()
+    else:
+        x = randn(g, rows, cols)
+    one = torch.ones(cols, device=DEV)
+    for gate in (None, one, torch.ones(rows, 1, device=DEV)):
+        params = ct.ResidualNorm(pre=norms[0], pre_weight=one, pre_bias=one if norms[0] == 1 else None, post=norms[1], post_weight=one if norms[1] else None)
+        y, _, stats = ct.residual_norm(x, x, params, gate=gate)
+        grads = {"x": torch.empty_like(x), "f": torch.empty_like(x), "pre_weight": torch.empty_like(one)}
+        if norms[1]:
+            grads["post_weight"] = torch.empty_like(one)
+        if norms[0] == 1:
+            grads["pre_bias"] = torch.empty_like(one)
+        if gate is not None:
+            grads["gate"] = torch.empty_like(gate)
+        call_backward(ct, x, y, gate, stats, params, x, x, grads)
+        got = ct.residual_norm_backward(x, y, stats, params, grad_y=x, grad_h=x, gate=gate)
+        assert all(torch.equal(t, getattr(got, n)) for n, t in grads.items())
+
+
 # ---- more elements than 32 bits count ---------------------------------------------------------------------------
 def test_scores_of_more_than_2_31_elements(ct):
     B, H, Q, K = 1, 2, 34_000, 32_768
