@@ -18,12 +18,12 @@
 // (f, y, dy, dh in; dx, df out), 4 / 8 more with a gate for every element.  A row is owned by a team of
 // T threads (a warp to a CTA; for wide rows a cluster of CTAs that hold a slice of the columns each and
 // exchange their sums through distributed shared memory); every operand is read once.  Measured (share of the
-// 6.54 TB/s of a copy): forward with one norm [4096, 8192] 83 us, 6.5 TB/s (0.99), with RMS norms on both sides
-// [32768, 768] 68 us (0.90), [4096, 8192] 97 us (0.84: two folds one behind the other); backward with one norm
-// [16384, 1536] 85 us (0.91), RMS on both sides [4096, 5120] 95 us (0.81), with a gate for every element 117 us
-// (0.88), [4096, 8192] in clusters 176 us (0.70); LayerNorms on both sides [16384, 1024] 88 us (0.70), registers
-// for four sums per column leave 12 warps on an SM; rows of odd length go
-// element by element: [16000, 1999] with one norm forward 97 us (0.81), backward 140 us (0.70), two norms 0.56 and 0.35.
+// 6.54 TB/s of a copy, four sets of buffers in turn): forward with one norm [4096, 8192] 82 us, 6.5 TB/s (1.00), with RMS
+// norms on both sides [32768, 768] 65 us (0.95), [4096, 8192] 86 us (0.96), [4096, 5120] 61 us (0.85: two folds one behind the
+// other); backward with one norm [16384, 1536] 84 us (0.92), RMS on both sides [4096, 5120] 87 us (0.88), with a gate for every
+// element 116 us (0.89), [4096, 8192] in clusters 189 us (0.65); LayerNorms on both sides [16384, 1024] 70 us (0.88),
+// [8192, 4096] 177 us (0.69), registers for four sums per column leave 12 warps on an SM; rows of odd length go element by
+// element: [16000, 1999] with one norm forward 97 us (0.80), backward 137 us (0.72), two LayerNorms 0.53 and 0.36.
 #include "ctb_residual_norm.cuh"
 #include "ctb_team.cuh"
 
@@ -242,7 +242,7 @@ residual_norm_kernel(ResidualNormGeom g, RowsIn x, RowsIn f, float* __restrict__
 }
 
 // A row of residual_rms_kernel (below) that is near the ends of Float32, normed before it is scaled, from memory.  A call of
-// its own: inlined, it took registers from all other rows ([1000000,128] 375 us, 428 so).
+// its own: inlined, it took registers from all other rows ([1000000,128] 381 us, 428 so).
 template <int THREADS, int T, int VEC>
 __device__ __noinline__ void residual_rms_extreme_row(const ResidualNormGeom& g, const float* x, const float* f, float* y, float* h, float* stats, int64_t row,
                                                       float rf, TeamSlots<THREADS, 4, double>& sh, FoldTurn turn) {
@@ -409,7 +409,8 @@ residual_rms_kernel(const __grid_constant__ ResidualNormGeom g, RowsIn x, RowsIn
 // linear in them, dx = e - rstd_y * (m1 + yhat * m2) with e = dy + rstd_y * a, so with k = scale * gate * w_post
 //     sum(k dx)      = sum(k e)      - rstd_y * (m1 * sum(k)      + m2 * sum(k yhat))
 //     sum(k dx fhat) = sum(k e fhat) - rstd_y * (m1 * sum(k fhat) + m2 * sum(k fhat yhat))
-// and all eight sums are taken together.  Without a LayerNorm (m1 and the mean of k dx drop out) three remain.
+// and all eight sums are taken together.  Without a LayerNorm (m1 and the mean of k dx drop out) three remain.  (As
+// differences these sums are as exact as dx itself, whose elements are differences of the same size.)
 //
 // Column sums (weights, biases, a gate shared by rows) stay in registers, as Float32, until the team's last row — a shared
 // gate's until its last row in the team — and go out as partials, which a second launch adds in order, in fp64.  A

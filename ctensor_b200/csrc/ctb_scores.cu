@@ -16,10 +16,11 @@
 // Bound by HBM: 4 bytes per admitted score in, 4 per element out; backward 8 (12 with a cap) in, 4 out.
 // Rows that fit are held in the registers of part of a warp, a warp or a CTA and read once; longer rows are swept
 // twice by one or more CTAs (second sweep from L2), few long ones held by a cluster.  Measured (bytes that
-// have to move over time, share of the 6.54 TB/s of a copy): [8,12,1024,1024] causal forward 96 us, 6.3 TB/s (0.96),
-// backward 126 us, 6.4 (0.98); capped 100 us (0.93) and 155 us (0.99); five packed documents, capped: 84 us (0.81),
-// instructions bound it (three quarters of the issue slots: a row that is nearly all zeros still looks at
-// every document number), gradients 130 us; [1,12,512,16384] 143 us (0.86); swept rows of 100000: 165 us (0.57), gradients 185 (0.76).
+// have to move over time, share of the 6.54 TB/s of a copy): [8,12,1024,1024] causal forward 94 us, 6.4 TB/s (0.98),
+// backward 126 us, 6.4 (0.98); capped 100 us (0.93) and 148 us (1.04, a part from L2); five packed documents, capped: 83 us (0.82),
+// with slopes 86, instructions bound it (three quarters of the issue slots: a row that is nearly all zeros still looks at
+// every document number), gradients 129 and 152 us; [1,12,512,16384] 138 us (0.89); swept rows of 100000: 162 us (0.58),
+// gradients 186 (0.76).
 #include "ctb_scores.cuh"
 #include "ctb_team.cuh"
 
@@ -257,7 +258,7 @@ __device__ __forceinline__ void score_slow(const ScoreGeom& g, float (&r)[4], co
 // admitted is a comparison with `live` where rows are aligned and no documents are given, else kept as bits.
 // With documents few fours of a row may have an admitted key, anywhere in it: a warp then goes over those v that
 // have one in any of its lanes, the j-th of them held in the j-th registers, instead of over all with a test and a
-// branch each ([8,12,1024,1024] causal, capped, five packed documents: 91 us, so 84, gradients 155 and 130; all
+// branch each ([8,12,1024,1024] causal, capped, five packed documents: 91 us, so 83, gradients 155 and 129; all
 // keys in one document 97 and 101).
 template <int T, int NV, bool DOCS, bool ALIGNED>
 struct ScoreShare {
@@ -435,7 +436,7 @@ score_softmax_kernel(const __grid_constant__ ScoreArgs a, int ctas) {
 }
 
 // Registers: 64 with a cap or ragged rows, 48 else; a spilled word or two costs less than a quarter of the rows in
-// flight (capped [8,12,1024,1024]: 176 us, so 155; CTAs of 512, one or two an SM: [2,8,1024,8192] 420 and 293).
+// flight (capped [8,12,1024,1024], when 1 - tanh^2 still took a tanh: 176 us, so 155; CTAs of 512, one or two an SM: [2,8,1024,8192] 420 and 293).
 // With documents the compiler's own choice is the better one (0: no bound; 75 us at [64,12,256,256], 91 with one).
 template <int THREADS, int T, int NV, bool CAP, bool DOCS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : DOCS ? 0 : CAP || !ALIGNED ? 4 : 5)

@@ -74,6 +74,8 @@ Tensor tanh_backward(const Tensor& grad, const Tensor& t);
 //   score_softmax_backward  gradient of the scores (`scores` is needed with a cap) and, if asked for, of the slopes
 //   residual_norm           y = x + scale * gate * N_post(f), h = N_pre(y); without f, y is x
 //   residual_norm_backward  the gradients of everything that went in (absent where there was no such input)
+// Their results carry no autograd node, whatever requires_grad says: a backward() that reaches them goes no
+// further.  A training step calls the _backward functions itself and goes on from what they return.
 struct ScoreRules {
     double scale = 1.0, cap = 0.0;
     bool causal = false;
